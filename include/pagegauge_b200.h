@@ -9,7 +9,9 @@
  * host validation are kept verbatim so callers can match on them.
  *
  * Fixed geometry: head_dim 128, 16-token pages, NHD page layout
- * [pages, 16, Hkv, 128]; GQA group Hq/Hkv in 1..8.
+ * [pages, 16, Hkv, 128]; GQA group Hq/Hkv in 1..8.  The 4-bit cache keeps
+ * the geometry in records of its own (PG_INT4_RECORD_BYTES per page and KV
+ * head); pg_rotary takes any head size.
  *
  * Reference interfaces replaced (paths inside ahmed123hds/PageGauge):
  *   pg_rope_append_fp16          <- rope_append_fp16[_dynamic]
@@ -69,7 +71,8 @@ int32_t pg_abi_version(void);
 
 /* sizeof of pg_decode_args, pg_gemm_args, pg_segment, pg_plan_info and
  * pg_decode_item as compiled into the library (a binding checks its own
- * structure layouts against these before the first call).                */
+ * structure layouts against these before the first call); with n >= 8 also
+ * of pg_rotary_args, pg_int4_append_args and pg_int4_decode_args.         */
 int32_t pg_struct_sizes(int64_t* out, int32_t n);
 
 /* Read and clear the device guard word of the current device. */
@@ -387,6 +390,127 @@ int32_t pg_quantize_pages(const void* key, const void* value,
 int32_t pg_quantize_affine_group16(const void* values, int64_t num_pages, int32_t kv_heads,
                                    void* codes, void* bias, void* scale, void* reconstructed,
                                    void* stream);
+
+/* ---------------------------------------------------------------------- */
+/* Rotary positions and the 4-bit paged cache (no counterparts in the         */
+/* reference).                                                              */
+
+enum {
+  PG_DTYPE_F16 = 0,
+  PG_DTYPE_BF16 = 1,
+  PG_DTYPE_F32 = 2 /* pg_rotary and pg_int4_read */
+};
+
+/* Turn the first 2 * pairs dims of every query and key row by the angle of
+ * its token's position, in FP32 with one rounding at the end:
+ *   a' = a cos - b sin,  b' = b cos + a sin        (adjoint: sin negated)
+ * for (a, b) = dims (j, j + pairs), or (2j, 2j + 1) when interleaved; the
+ * other dims are copied.  Index 0: query rows, index 1: key rows (x[1] NULL
+ * or heads[1] = 0: none).  y may be x with the same strides (in place); any
+ * other overlap is not allowed.  cosine / sine are FP32
+ * [table_rows, pairs], rows table_stride apart.  A token whose position is
+ * outside the table is left as it is and reported (PG_DEV_BAD_POSITION).  */
+typedef struct pg_rotary_args {
+  const void* x[2]; /* [tokens, heads, head_dim], last dim contiguous */
+  void* y[2];
+  int64_t x_stride_t[2], x_stride_h[2], y_stride_t[2], y_stride_h[2]; /* elements */
+  int64_t tokens, table_stride, table_rows;
+  const float* cosine;
+  const float* sine;
+  const int32_t* positions; /* device [tokens] */
+  int32_t heads[2];
+  int32_t head_dim, pairs, interleaved, adjoint, dtype;
+} pg_rotary_args;
+
+int32_t pg_rotary(const pg_rotary_args* args, void* stream);
+
+/* The 4-bit cache: one record per (page of 16 tokens, KV head),
+ * [pages, Hkv, 2560] bytes, 16-byte aligned.  A token's key and value are
+ * held in four groups of 32 dims: s = f16((max - min) / 15),
+ * m = f16(min + 8 s), code z = clamp(rint((x - m) / s), -8, 7) + 8, and
+ * x ~ (z - 8) s + m.  Values past +-65504 are held as +-65504; a NaN makes
+ * its group NaN.  Token t of a record, with nibble 0 of a byte the low one:
+ *   key dim 32g + 8a + i:   byte 64t + 16a + 4g + i/2, nibble i%2
+ *   value dim 32g + 4a + i: byte 1024 + 64 row(t) + 8a + 2g + i/2, nibble
+ *                           i%2, row(t) = (t & 8) + 4 (t & 1) + (t / 2 & 3)
+ *   key s[4], m[4] (f16):   byte 2048 + 16t
+ *   value s[4], m[4] (f16): byte 2304 + 16t                                 */
+enum { PG_INT4_RECORD_BYTES = 2560 };
+
+/* Rotation (as pg_rotary, pairs in 1..64) of query and key rows, then the
+ * keys and values of any number of tokens, less their centres, written in 4
+ * bits at slots[t] = physical page * 16 + token.  A negative slot skips its
+ * token: nothing of it is read or written.  Every other slot may occur once
+ * per call (with two tokens at one slot the slot's contents are undefined).
+ * A slot outside the pool, a centre row outside the centres
+ * (PG_DEV_BAD_PAGE_ID) or a position outside the table
+ * (PG_DEV_BAD_POSITION) skips the token and is reported.                  */
+typedef struct pg_int4_append_args {
+  const void* query; /* [tokens, query_heads, 128], last dim contiguous */
+  const void* key;   /* [tokens, kv_heads, 128] */
+  const void* value;
+  void* rotated_query; /* [tokens, query_heads, 128]; may be query */
+  void* rotated_key;   /* [tokens, kv_heads, 128] or NULL; may be key */
+  int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+  int64_t rq_stride_t, rq_stride_h, rk_stride_t, rk_stride_h; /* elements */
+  const float* cosine; /* [table_rows, pairs], rows table_stride apart */
+  const float* sine;
+  int64_t table_stride, table_rows;
+  const int32_t* positions; /* device [tokens] */
+  const int32_t* slots;     /* device [tokens] */
+  void* records;
+  int64_t num_pages;
+  const void* key_center; /* [num_centers, kv_heads, 128] or NULL */
+  const void* value_center;
+  const int32_t* center_rows; /* device [tokens]; NULL: row 0 */
+  int64_t num_centers, tokens;
+  int32_t query_heads, kv_heads, pairs, interleaved;
+  int32_t dtype; /* PG_DTYPE_F16 or PG_DTYPE_BF16: rows and centres */
+  int32_t reserved;
+} pg_int4_append_args;
+
+int32_t pg_rope_append_int4(const pg_int4_append_args* args, void* stream);
+
+/* The values the cache holds for the tokens at `slots` (device [tokens]):
+ * key and value [tokens, kv_heads, 128] contiguous, of type dtype, centres
+ * not added.  Negative slots give zeros; slots outside the pool give zeros
+ * and are reported (PG_DEV_BAD_PAGE_ID).                                  */
+int32_t pg_int4_read(const void* records, int64_t num_pages, int32_t kv_heads,
+                     const int32_t* slots, int64_t tokens, void* key, void* value,
+                     int32_t dtype, void* stream);
+
+/* Decode attention over the 4-bit cache: per request and query head
+ *   out = softmax(sm_scale q K^T) V (+ value_center), lse_out = base-2
+ * log-sum-exp of the scores.  The page table and its plan are those of
+ * pg_decode_plan with one segment (indptr0); last_page_len counts the valid
+ * tokens of a request's last page.  Requests without pages give zeros (no
+ * centre) and -inf.  Pages may have been written by the kernel just before
+ * in the stream: they are read after it completes.  A page id outside the
+ * pool is left out and reported (PG_DEV_BAD_PAGE_ID).                      */
+typedef struct pg_int4_decode_args {
+  const void* q; /* [B, Hq, 128] of dtype, last dim contiguous */
+  int64_t q_stride_b, q_stride_h;
+  void* out; /* [B, Hq, 128] of dtype */
+  int64_t out_stride_b, out_stride_h;
+  float* lse_out;           /* [B, Hq] or NULL */
+  const void* value_center; /* [B, Hkv, 128] of dtype or NULL */
+  int64_t vc_stride_b;
+  const void* records;
+  int64_t num_pages;
+  const int32_t* indices;       /* device page ids */
+  const int32_t* last_page_len; /* device [B] */
+  const pg_decode_item* items;  /* device, from pg_decode_plan */
+  const int32_t* item_off;      /* device [B*Hkv+1] */
+  float* part_o;                /* device workspace [num_items*group*128] */
+  float* part_lse;              /* device workspace [num_items*group] */
+  int32_t num_items, batch, kv_heads, group;
+  int32_t final_mode; /* 1: one item per (request, head): no merge launch */
+  int32_t dtype;      /* PG_DTYPE_F16 or PG_DTYPE_BF16 */
+  float sm_scale;
+  int32_t reserved;
+} pg_int4_decode_args;
+
+int32_t pg_decode_int4_run(const pg_int4_decode_args* args, void* stream);
 
 /* ---------------------------------------------------------------------- */
 /* Decoder-layer element-wise steps around the attention path (the Mistral   */

@@ -65,6 +65,48 @@ class PgGemmArgs(ctypes.Structure):
     ]
 
 
+class PgRotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", c_vp * 2), ("y", c_vp * 2),
+        ("x_stride_t", c_i64 * 2), ("x_stride_h", c_i64 * 2),
+        ("y_stride_t", c_i64 * 2), ("y_stride_h", c_i64 * 2),
+        ("tokens", c_i64), ("table_stride", c_i64), ("table_rows", c_i64),
+        ("cosine", c_vp), ("sine", c_vp), ("positions", c_vp),
+        ("heads", c_i32 * 2), ("head_dim", c_i32), ("pairs", c_i32), ("interleaved", c_i32),
+        ("adjoint", c_i32), ("dtype", c_i32),
+    ]
+
+
+class PgInt4AppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("query", c_vp), ("key", c_vp), ("value", c_vp), ("rotated_query", c_vp),
+        ("rotated_key", c_vp),
+        ("q_stride_t", c_i64), ("q_stride_h", c_i64), ("k_stride_t", c_i64),
+        ("k_stride_h", c_i64), ("v_stride_t", c_i64), ("v_stride_h", c_i64),
+        ("rq_stride_t", c_i64), ("rq_stride_h", c_i64), ("rk_stride_t", c_i64),
+        ("rk_stride_h", c_i64),
+        ("cosine", c_vp), ("sine", c_vp), ("table_stride", c_i64), ("table_rows", c_i64),
+        ("positions", c_vp), ("slots", c_vp), ("records", c_vp), ("num_pages", c_i64),
+        ("key_center", c_vp), ("value_center", c_vp), ("center_rows", c_vp),
+        ("num_centers", c_i64), ("tokens", c_i64),
+        ("query_heads", c_i32), ("kv_heads", c_i32), ("pairs", c_i32), ("interleaved", c_i32),
+        ("dtype", c_i32), ("reserved", c_i32),
+    ]
+
+
+class PgInt4DecodeArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", c_vp), ("q_stride_b", c_i64), ("q_stride_h", c_i64),
+        ("out", c_vp), ("out_stride_b", c_i64), ("out_stride_h", c_i64),
+        ("lse_out", c_vp), ("value_center", c_vp), ("vc_stride_b", c_i64),
+        ("records", c_vp), ("num_pages", c_i64), ("indices", c_vp), ("last_page_len", c_vp),
+        ("items", c_vp), ("item_off", c_vp), ("part_o", c_vp), ("part_lse", c_vp),
+        ("num_items", c_i32), ("batch", c_i32), ("kv_heads", c_i32), ("group", c_i32),
+        ("final_mode", c_i32), ("dtype", c_i32), ("sm_scale", ctypes.c_float),
+        ("reserved", c_i32),
+    ]
+
+
 # name -> (restype, argtypes); every entry point returns int32 status.
 _SIGNATURES = {
     "pg_last_error": (ctypes.c_char_p, []),
@@ -119,6 +161,10 @@ _SIGNATURES = {
                                          ctypes.POINTER(c_i64), c_i32p]),
     "pg_skinny_gemm": (c_i32, [ctypes.POINTER(PgGemmArgs), c_vp]),
     "pg_quantize_pages": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_i32, c_i32, c_vp]),
+    "pg_rotary": (c_i32, [ctypes.POINTER(PgRotaryArgs), c_vp]),
+    "pg_rope_append_int4": (c_i32, [ctypes.POINTER(PgInt4AppendArgs), c_vp]),
+    "pg_int4_read": (c_i32, [c_vp, c_i64, c_i32, c_vp, c_i64, c_vp, c_vp, c_i32, c_vp]),
+    "pg_decode_int4_run": (c_i32, [ctypes.POINTER(PgInt4DecodeArgs), c_vp]),
     "pg_quantize_affine_group16": (c_i32, [c_vp, c_i64, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp]),
 }
 
@@ -150,11 +196,12 @@ def load() -> ctypes.CDLL:
         fn.argtypes = argtypes
     # The argument blocks cross the boundary by pointer: their layouts must
     # match the library's exactly.
-    sizes = (c_i64 * 5)()
-    if lib.pg_struct_sizes(sizes, 5) != 0:
+    sizes = (c_i64 * 8)()
+    if lib.pg_struct_sizes(sizes, 8) != 0:
         raise RuntimeError("pg_struct_sizes failed")
     mine = (ctypes.sizeof(PgDecodeArgs), ctypes.sizeof(PgGemmArgs), ctypes.sizeof(PgSegment),
-            ctypes.sizeof(PgPlanInfo), ctypes.sizeof(PgDecodeItem))
+            ctypes.sizeof(PgPlanInfo), ctypes.sizeof(PgDecodeItem), ctypes.sizeof(PgRotaryArgs),
+            ctypes.sizeof(PgInt4AppendArgs), ctypes.sizeof(PgInt4DecodeArgs))
     if tuple(sizes) != mine:
         raise RuntimeError(f"C ABI structure sizes {tuple(sizes)} differ from the binding's {mine}")
     _lib = lib

@@ -17,8 +17,11 @@
 #include "pg_affine.cuh"
 #include "pg_append.cuh"
 #include "pg_decode.cuh"
+#include "pg_decode_int4.cuh"
 #include "pg_decoder.cuh"
 #include "pg_gemm.cuh"
+#include "pg_int4.cuh"
+#include "pg_rotary.cuh"
 
 namespace {
 
@@ -306,6 +309,11 @@ int32_t pg_struct_sizes(int64_t* out, int32_t n) {
   out[2] = sizeof(pg_segment);
   out[3] = sizeof(pg_plan_info);
   out[4] = sizeof(pg_decode_item);
+  if (n >= 8) {
+    out[5] = sizeof(pg_rotary_args);
+    out[6] = sizeof(pg_int4_append_args);
+    out[7] = sizeof(pg_int4_decode_args);
+  }
   return PG_OK;
 }
 
@@ -1037,6 +1045,242 @@ int32_t pg_quantize_affine_group16(const void* values, int64_t num_pages, int32_
   pg::pg_quantize_affine_kernel<<<blocks, pg::kAffineQuantWarps * 32, 0,
                                   static_cast<cudaStream_t>(stream)>>>(p);
   return cuda_check(cudaGetLastError(), "affine quantize launch");
+}
+
+// ---------------------------------------- rotary positions and 4-bit cache
+int32_t pg_rotary(const pg_rotary_args* a, void* stream) {
+  PG_REQUIRE(a != nullptr, "null arguments");
+  PG_REQUIRE(a->dtype >= PG_DTYPE_F16 && a->dtype <= PG_DTYPE_F32, "unknown dtype %d", a->dtype);
+  PG_REQUIRE(a->tokens >= 0 && a->heads[0] >= 0 && a->heads[1] >= 0,
+             "token and head counts must be non-negative");
+  PG_REQUIRE(a->head_dim > 0 && a->head_dim <= 4096 && a->pairs > 0 &&
+                 2 * a->pairs <= a->head_dim,
+             "the rotated dims must be 2..head_dim, and head_dim at most 4096");
+  PG_REQUIRE(a->table_rows > 0 && a->table_stride >= a->pairs,
+             "cosine and sine must be [positions, pairs] tables");
+  pg::RotaryParams p{};
+  int64_t rows = 0;
+  for (int i = 0; i < 2; ++i) {
+    p.heads[i] = a->x[i] == nullptr ? 0 : a->heads[i];
+    if (p.heads[i] > 0) PG_REQUIRE(a->y[i] != nullptr, "rotated rows need an output");
+    p.x[i] = a->x[i];
+    p.y[i] = a->y[i];
+    p.x_stride_t[i] = a->x_stride_t[i];
+    p.x_stride_h[i] = a->x_stride_h[i];
+    p.y_stride_t[i] = a->y_stride_t[i];
+    p.y_stride_h[i] = a->y_stride_h[i];
+    rows += p.heads[i];
+  }
+  if (a->tokens == 0 || rows == 0) return PG_OK;
+  PG_REQUIRE(rows < (int64_t(1) << 20) && a->tokens < (int64_t(1) << 31),
+             "too many rows or tokens");
+  PG_REQUIRE(a->cosine != nullptr && a->sine != nullptr && a->positions != nullptr,
+             "rotary tables and device positions are required");
+  p.tokens = a->tokens;
+  p.head_dim = a->head_dim;
+  p.pairs = a->pairs;
+  p.interleaved = a->interleaved != 0;
+  p.sign = a->adjoint ? -1.f : 1.f;
+  p.cos = a->cosine;
+  p.sin = a->sine;
+  p.table_stride = a->table_stride;
+  p.table_rows = a->table_rows;
+  p.positions = a->positions;
+  p.error_flag = device_error_ptr();
+  const int64_t total = a->tokens * rows * (a->head_dim - a->pairs);
+  const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((total + 255) / 256, 148 * 64));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a->dtype == PG_DTYPE_F16)
+    return launch_pdl(pg::pg_rotary_kernel<__half>, dim3(blocks), dim3(256), 0, st,
+                      "rotary launch", p);
+  if (a->dtype == PG_DTYPE_BF16)
+    return launch_pdl(pg::pg_rotary_kernel<__nv_bfloat16>, dim3(blocks), dim3(256), 0, st,
+                      "rotary launch", p);
+  return launch_pdl(pg::pg_rotary_kernel<float>, dim3(blocks), dim3(256), 0, st,
+                    "rotary launch", p);
+}
+
+int32_t pg_rope_append_int4(const pg_int4_append_args* a, void* stream) {
+  PG_REQUIRE(a != nullptr, "null arguments");
+  PG_REQUIRE(a->dtype == PG_DTYPE_F16 || a->dtype == PG_DTYPE_BF16,
+             "rows must be float16 or bfloat16");
+  PG_REQUIRE(a->tokens >= 0, "the token count must be non-negative");
+  PG_REQUIRE(a->query_heads > 0 && a->kv_heads > 0 && a->query_heads <= 65536 &&
+                 a->kv_heads <= 65536,
+             "head counts must be positive");
+  PG_REQUIRE(a->pairs >= 1 && a->pairs <= pg::kHeadDim / 2, "the rotated dims must be 2..128");
+  PG_REQUIRE(a->table_rows > 0 && a->table_stride >= a->pairs,
+             "cosine and sine must be [positions, pairs] tables");
+  PG_REQUIRE(a->num_pages > 0 && a->num_pages < (int64_t(1) << 27), "pool page count out of range");
+  PG_REQUIRE((a->key_center == nullptr) == (a->value_center == nullptr),
+             "key and value centres are both given or both NULL");
+  PG_REQUIRE(a->key_center == nullptr || a->num_centers > 0, "no centre rows");
+  if (a->tokens == 0) return PG_OK;
+  PG_REQUIRE(a->tokens < (int64_t(1) << 31), "too many tokens");
+  PG_REQUIRE(a->query != nullptr && a->key != nullptr && a->value != nullptr &&
+                 a->rotated_query != nullptr && a->cosine != nullptr && a->sine != nullptr &&
+                 a->positions != nullptr && a->slots != nullptr && a->records != nullptr,
+             "rows, tables, positions, slots and records are required");
+  PG_REQUIRE(aligned(a->records, 16) && aligned(a->key_center, 16) && aligned(a->value_center, 16),
+             "records and centres must be 16-byte aligned");
+  pg::Int4AppendParams p{};
+  p.q = a->query;
+  p.k = a->key;
+  p.v = a->value;
+  p.q_stride_t = a->q_stride_t;
+  p.q_stride_h = a->q_stride_h;
+  p.k_stride_t = a->k_stride_t;
+  p.k_stride_h = a->k_stride_h;
+  p.v_stride_t = a->v_stride_t;
+  p.v_stride_h = a->v_stride_h;
+  p.rotated_q = a->rotated_query;
+  p.rotated_k = a->rotated_key;
+  p.rq_stride_t = a->rq_stride_t;
+  p.rq_stride_h = a->rq_stride_h;
+  p.rk_stride_t = a->rk_stride_t;
+  p.rk_stride_h = a->rk_stride_h;
+  p.cos = a->cosine;
+  p.sin = a->sine;
+  p.table_stride = a->table_stride;
+  p.table_rows = a->table_rows;
+  p.positions = a->positions;
+  p.slots = a->slots;
+  p.records = static_cast<uint8_t*>(a->records);
+  p.num_pages = a->num_pages;
+  p.key_center = a->key_center;
+  p.value_center = a->value_center;
+  p.center_rows = a->key_center != nullptr ? a->center_rows : nullptr;
+  p.num_centers = a->num_centers;
+  p.tokens = a->tokens;
+  p.hq = a->query_heads;
+  p.hkv = a->kv_heads;
+  p.pairs = a->pairs;
+  p.interleaved = a->interleaved != 0;
+  p.error_flag = device_error_ptr();
+  const bool rows16 =
+      aligned(a->query, 16) && aligned(a->key, 16) && aligned(a->value, 16) &&
+      aligned(a->rotated_query, 16) && aligned(a->rotated_key, 16) &&
+      (a->q_stride_t | a->q_stride_h | a->k_stride_t | a->k_stride_h | a->v_stride_t |
+       a->v_stride_h | a->rq_stride_t | a->rq_stride_h) % 8 == 0 &&
+      (a->rotated_key == nullptr || (a->rk_stride_t | a->rk_stride_h) % 8 == 0);
+  const bool table16 = aligned(a->cosine, 16) && aligned(a->sine, 16) &&
+                       a->table_stride % 4 == 0 && a->pairs % (p.interleaved ? 4 : 8) == 0;
+  const bool fast = rows16 && table16;
+  // Row pairs of one token: all in one warp when the tokens alone fill the
+  // GPU, spread over as many warps as it takes otherwise.
+  const int units = (p.hq + 1) / 2 + 2 * ((p.hkv + 1) / 2);
+  const int64_t want = 148 * 64;
+  p.split = static_cast<int32_t>(
+      std::min<int64_t>(units, std::max<int64_t>(1, want / a->tokens)));
+  const int64_t warps = a->tokens * p.split;
+  PG_REQUIRE((warps + 7) / 8 < (int64_t(1) << 31), "too many tokens");
+  const dim3 grid(static_cast<unsigned>((warps + 7) / 8));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a->dtype == PG_DTYPE_F16)
+    return launch_pdl(fast ? pg::pg_rope_append_int4_kernel<__half, true>
+                           : pg::pg_rope_append_int4_kernel<__half, false>,
+                      grid, dim3(256), 0, st, "rope_append_int4 launch", p);
+  return launch_pdl(fast ? pg::pg_rope_append_int4_kernel<__nv_bfloat16, true>
+                         : pg::pg_rope_append_int4_kernel<__nv_bfloat16, false>,
+                    grid, dim3(256), 0, st, "rope_append_int4 launch", p);
+}
+
+int32_t pg_int4_read(const void* records, int64_t num_pages, int32_t kv_heads,
+                     const int32_t* slots, int64_t tokens, void* key, void* value,
+                     int32_t dtype, void* stream) {
+  PG_REQUIRE(dtype >= PG_DTYPE_F16 && dtype <= PG_DTYPE_F32, "unknown dtype %d", dtype);
+  PG_REQUIRE(kv_heads > 0 && kv_heads <= 65536, "head counts must be positive");
+  PG_REQUIRE(num_pages > 0 && num_pages < (int64_t(1) << 27), "pool page count out of range");
+  PG_REQUIRE(tokens >= 0 && tokens < (int64_t(1) << 31), "token count out of range");
+  if (tokens == 0) return PG_OK;
+  PG_REQUIRE(records != nullptr && slots != nullptr && key != nullptr && value != nullptr,
+             "records, slots and outputs are required");
+  PG_REQUIRE(aligned(records, 16) && aligned(key, 16) && aligned(value, 16),
+             "records and outputs must be 16-byte aligned");
+  pg::Int4ReadParams p{};
+  p.records = static_cast<const uint8_t*>(records);
+  p.num_pages = num_pages;
+  p.slots = slots;
+  p.tokens = tokens;
+  p.hkv = kv_heads;
+  p.key = key;
+  p.value = value;
+  p.error_flag = device_error_ptr();
+  const int64_t rows = tokens * kv_heads * 2;
+  PG_REQUIRE((rows + 15) / 16 < (int64_t(1) << 31), "too many tokens");
+  const dim3 grid(static_cast<unsigned>((rows + 15) / 16));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == PG_DTYPE_F16)
+    return launch_pdl(pg::pg_int4_read_kernel<__half>, grid, dim3(256), 0, st, "int4 read launch",
+                      p);
+  if (dtype == PG_DTYPE_BF16)
+    return launch_pdl(pg::pg_int4_read_kernel<__nv_bfloat16>, grid, dim3(256), 0, st,
+                      "int4 read launch", p);
+  return launch_pdl(pg::pg_int4_read_kernel<float>, grid, dim3(256), 0, st, "int4 read launch", p);
+}
+
+int32_t pg_decode_int4_run(const pg_int4_decode_args* a, void* stream) {
+  PG_REQUIRE(a != nullptr, "null arguments");
+  PG_REQUIRE(a->batch > 0 && a->kv_heads > 0, "batch and kv heads must be positive");
+  PG_REQUIRE(a->group >= 1 && a->group <= 8, "GQA group size must be in 1..8");
+  PG_REQUIRE(a->sm_scale > 0.f && std::isfinite(a->sm_scale),
+             "sm_scale must be positive and finite");
+  PG_REQUIRE(a->dtype == PG_DTYPE_F16 || a->dtype == PG_DTYPE_BF16,
+             "rows must be float16 or bfloat16");
+  PG_REQUIRE(a->q != nullptr && aligned(a->q, 4) && a->q_stride_b % 2 == 0 &&
+                 a->q_stride_h % 2 == 0,
+             "query must be 4-byte aligned with even strides");
+  PG_REQUIRE(a->out != nullptr, "output is required");
+  PG_REQUIRE(a->num_items >= 0, "negative item count");
+  PG_REQUIRE(a->num_pages > 0 && a->num_pages < (int64_t(1) << 27),
+             "pool page count out of range");
+  PG_REQUIRE(a->records != nullptr && aligned(a->records, 16),
+             "records must be 16-byte aligned");
+  PG_REQUIRE(a->num_items == 0 || (a->indices != nullptr && a->last_page_len != nullptr),
+             "page table is incomplete");
+  PG_REQUIRE(a->num_items == 0 || a->items != nullptr, "work items are required");
+  const bool final_mode = a->final_mode != 0 && a->num_items > 0;
+  PG_REQUIRE(final_mode || a->item_off != nullptr, "item offsets are required for the merge");
+  PG_REQUIRE(final_mode || a->num_items == 0 || (a->part_o != nullptr && a->part_lse != nullptr),
+             "split decode needs a partial-state workspace");
+  pg::Int4DecodeParams p{};
+  p.q = a->q;
+  p.q_stride_b = a->q_stride_b;
+  p.q_stride_h = a->q_stride_h;
+  p.records = static_cast<const uint8_t*>(a->records);
+  p.num_pages = static_cast<int32_t>(a->num_pages);
+  p.indices = a->indices;
+  p.last_len = a->last_page_len;
+  p.items = reinterpret_cast<const pg::DecodeItem*>(a->items);
+  p.item_off = a->item_off;
+  p.num_items = a->num_items;
+  p.batch = a->batch;
+  p.hkv = a->kv_heads;
+  p.group = a->group;
+  p.sm_scale_log2 = a->sm_scale * 1.4426950408889634f;
+  p.part_o = a->part_o;
+  p.part_lse = a->part_lse;
+  p.final_mode = final_mode;
+  p.out = a->out;
+  p.out_stride_b = a->out_stride_b;
+  p.out_stride_h = a->out_stride_h;
+  p.lse_out = a->lse_out;
+  p.value_center = a->value_center;
+  p.vc_stride_b = a->vc_stride_b;
+  p.error_flag = device_error_ptr();
+  const bool half = a->dtype == PG_DTYPE_F16;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a->num_items > 0) {
+    int32_t rc = launch_pdl(half ? pg::pg_decode_int4_kernel<__half>
+                                 : pg::pg_decode_int4_kernel<__nv_bfloat16>,
+                            dim3(a->num_items), dim3(pg::kInt4Warps * 32), 0, st,
+                            "int4 decode launch", p);
+    if (rc != PG_OK || final_mode) return rc;
+  }
+  return launch_pdl(half ? pg::pg_int4_merge_kernel<__half>
+                         : pg::pg_int4_merge_kernel<__nv_bfloat16>,
+                    dim3(a->batch * a->kv_heads * a->group), dim3(pg::kHeadDim), 0, st,
+                    "int4 merge launch", p);
 }
 
 // ------------------------------------------------ decoder layer element-wise

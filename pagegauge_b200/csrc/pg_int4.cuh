@@ -1,0 +1,369 @@
+// The 4-bit paged cache: record layout, the fused rotation + append of any
+// number of tokens, and the read-back of stored tokens.
+//
+// One record of 2560 bytes per (page of 16 tokens, KV head), [pages, Hkv,
+// 2560] bytes in all, so a page of one head is one contiguous copy:
+//   [0, 1024)     key codes, 64 bytes per token
+//   [1024, 2048)  value codes, 64 bytes per token
+//   [2048, 2304)  key scales and midpoints, 16 bytes per token
+//   [2304, 2560)  value scales and midpoints
+// A token's key (or value) x of 128 dims is held in four groups of 32 dims:
+//   s = f16((max x - min x) / 15),  m = f16(min x + 8 s)
+//   z = clamp(rint((x - m) / s), -8, 7) + 8,   x ~ (z - 8) s + m
+// with all arithmetic in FP32 (the division by s is a product with the
+// rounded reciprocal, which differs only at exact ties of a code).  16 bytes
+// of scales per 64 bytes of codes: a group of 32 halves the error's power of
+// one scale per head row for 8 bytes more.
+//
+// Every byte of a record belongs to one token, so tokens of one page may be
+// written by different warps or launches in any order.  The order of the
+// codes within a token's 64 bytes is the decode kernel's tensor-core operand
+// order: see key_code_byte / value_code_byte.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "pg_common.cuh"
+
+namespace pg {
+
+constexpr int kInt4Record = 2560;
+constexpr int kInt4Value = 1024;    // value codes
+constexpr int kInt4KeyMeta = 2048;  // key scales and midpoints
+constexpr int kInt4ValueMeta = 2304;
+constexpr int kInt4Group = 32;  // dims that share a scale and a midpoint
+
+// Element types of q/k/v rows (the C ABI's PG_DTYPE_*).
+constexpr int kDtypeF16 = 0;
+constexpr int kDtypeBf16 = 1;
+constexpr int kDtypeF32 = 2;
+
+template <typename T>
+__device__ __forceinline__ float to_float(T x);
+template <>
+__device__ __forceinline__ float to_float<__half>(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 x) {
+  return __bfloat162float(x);
+}
+template <>
+__device__ __forceinline__ float to_float<float>(float x) { return x; }
+
+template <typename T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) {
+  return __float2bfloat16_rn(x);
+}
+template <>
+__device__ __forceinline__ float from_float<float>(float x) { return x; }
+
+// 8 consecutive 16-bit elements at p: one 16-byte access, or one by one
+// when rows are not 16-byte aligned.
+template <typename T, bool FAST>
+__device__ __forceinline__ void load8(const T* p, float* x) {
+  if constexpr (FAST) {
+    const uint4 w = *reinterpret_cast<const uint4*>(p);
+    const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_float<T>(e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_float<T>(p[i]);
+  }
+}
+
+template <typename T, bool FAST>
+__device__ __forceinline__ void store8(T* p, const float* x) {
+  if constexpr (FAST) {
+    uint4 w;
+    T* e = reinterpret_cast<T*>(&w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = from_float<T>(x[i]);
+    *reinterpret_cast<uint4*>(p) = w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = from_float<T>(x[i]);
+  }
+}
+
+// Minimum and maximum that keep a NaN, so that one shows in what is read.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Token tok's row of value codes: tokens 8p + 2u + e lie at row 8p + 4e + u,
+// so that the decode's reads of tokens {0, 2, 4, 6} (and {1, 3, 5, 7}) of a
+// half page are contiguous in shared memory.
+__host__ __device__ constexpr int value_code_row(int tok) {
+  return (tok & 8) + 4 * (tok & 1) + ((tok >> 1) & 3);
+}
+
+// Quantise lane m's 8 dims 8m .. 8m+7 of one row (16 lanes per row; lanes
+// 4j .. 4j+3 hold group j).  Returns the 8 codes, dim 8m + i in nibble i.
+__device__ __forceinline__ uint32_t int4_quantize8(float* x, __half& scale, __half& mid) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = min_nan(max_nan(x[i], -65504.f), 65504.f);
+  float lo = x[0], hi = x[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    lo = min_nan(lo, x[i]);
+    hi = max_nan(hi, x[i]);
+  }
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  scale = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
+  const float s = __half2float(scale);
+  mid = __float2half_rn(__fadd_rn(lo, 8.f * s));
+  const float m = __half2float(mid);
+  const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    // A NaN keeps code 0; its group's scale and midpoint are NaN.
+    const float z = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[i], m), inv)), -8.f), 7.f);
+    w |= (static_cast<uint32_t>(static_cast<int>(z) + 8) & 15u) << (4 * i);
+  }
+  return w;
+}
+
+struct Int4AppendParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+  void* rotated_q;  // [T, Hq, 128]
+  void* rotated_k;  // [T, Hkv, 128] or null
+  int64_t rq_stride_t, rq_stride_h, rk_stride_t, rk_stride_h;
+  const float* cos;  // [table_rows, pairs]
+  const float* sin;
+  int64_t table_stride, table_rows;
+  const int32_t* positions;  // [T]
+  const int32_t* slots;      // [T]: page * 16 + token, negative: skipped
+  uint8_t* records;
+  int64_t num_pages;
+  const void* key_center;  // [centers, Hkv, 128] or null
+  const void* value_center;
+  const int32_t* center_rows;  // [T] or null (row 0)
+  int64_t num_centers;
+  int64_t tokens;
+  int32_t hq, hkv, pairs, interleaved;
+  int32_t split;  // warps that share one token's rows
+  int* error_flag;
+};
+
+// Rotate lane m's 8 dims of a row (base = the row's element 0).  Half
+// layout: dims (d, d + pairs) turn together; interleaved: (2j, 2j + 1).
+// c, s: this lane's table entries (load_table8), or read here if !FAST.
+template <typename T, bool FAST>
+__device__ __forceinline__ void rotate8(float* x, const T* base, int m, int pairs,
+                                        bool interleaved, const float* c, const float* s,
+                                        const float* cos_row, const float* sin_row) {
+  if (interleaved) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const int j = 4 * m + (i >> 1);
+      if (j >= pairs) continue;
+      const float cj = FAST ? c[i >> 1] : cos_row[j], sj = FAST ? s[i >> 1] : sin_row[j];
+      const float a = x[i], b = x[i + 1];
+      x[i] = __fsub_rn(__fmul_rn(a, cj), __fmul_rn(b, sj));
+      x[i + 1] = __fadd_rn(__fmul_rn(b, cj), __fmul_rn(a, sj));
+    }
+    return;
+  }
+  if constexpr (FAST) {
+    // pairs is a multiple of 8: a lane's partner dims are one lane's.
+    const int step = pairs >> 3;
+    const int peer = m < step ? m + step : m - step;
+    const bool turns = m < 2 * step;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float o = __shfl_sync(0xffffffffu, x[i], turns ? peer : m, 16);
+      const float a = __fmul_rn(x[i], c[i]), b = __fmul_rn(o, s[i]);
+      if (turns) x[i] = m < step ? __fsub_rn(a, b) : __fadd_rn(a, b);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int d = 8 * m + i;
+      if (d >= 2 * pairs) continue;
+      const int j = d < pairs ? d : d - pairs;
+      const float o = to_float<T>(base[d < pairs ? d + pairs : j]);
+      const float a = __fmul_rn(x[i], cos_row[j]), b = __fmul_rn(o, sin_row[j]);
+      x[i] = d < pairs ? __fsub_rn(a, b) : __fadd_rn(a, b);
+    }
+  }
+}
+
+// One warp takes two rows at a time (16 lanes of 8 dims each) of one token:
+// its query rows, its key rows and its value rows; `split` warps share a
+// token.  The table entries of the token's position stay in registers.
+template <typename T, bool FAST>
+__global__ void __launch_bounds__(256)
+    pg_rope_append_int4_kernel(const __grid_constant__ Int4AppendParams p) {
+  pdl_launch_dependents();
+  pdl_wait_primary();
+  const int lane = threadIdx.x & 31, half = lane >> 4, m = lane & 15;
+  const int64_t w = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+  const int64_t token = w / p.split;
+  const int part = static_cast<int>(w - token * p.split);
+  if (token >= p.tokens) return;
+  const int slot = p.slots[token];
+  if (slot < 0) return;
+  const int64_t page = slot >> 4;
+  const int tok = slot & 15;
+  const int pos = p.positions[token];
+  const int64_t center = p.center_rows != nullptr ? p.center_rows[token] : 0;
+  if (page >= p.num_pages || (p.key_center != nullptr && (center < 0 || center >= p.num_centers))) {
+    record_error(p.error_flag, kDevBadPageId);
+    return;
+  }
+  if (pos < 0 || pos >= p.table_rows) {
+    record_error(p.error_flag, kDevBadPosition);
+    return;
+  }
+  const float* cos_row = p.cos + pos * p.table_stride;
+  const float* sin_row = p.sin + pos * p.table_stride;
+  float c[8], s[8];
+  if constexpr (FAST) {
+    // The lane's entries: half layout 8 of them, interleaved 4.
+    const int step = p.pairs >> 3;
+    const int j = p.interleaved ? 4 * m : 8 * (m < step ? m : m - step);
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      const bool in = (p.interleaved ? i == 0 : m < 2 * step) && j + i < p.pairs;
+      const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4 a = in ? __ldg(reinterpret_cast<const float4*>(cos_row + j + i)) : z;
+      const float4 b = in ? __ldg(reinterpret_cast<const float4*>(sin_row + j + i)) : z;
+      c[i] = a.x; c[i + 1] = a.y; c[i + 2] = a.z; c[i + 3] = a.w;
+      s[i] = b.x; s[i + 1] = b.y; s[i + 2] = b.z; s[i + 3] = b.w;
+    }
+  }
+  const int qu = (p.hq + 1) >> 1, ku = (p.hkv + 1) >> 1;  // row pairs
+  for (int u = part; u < qu + 2 * ku; u += p.split) {
+    if (u < qu) {
+      const int h = 2 * u + half;
+      const int hc = h < p.hq ? h : p.hq - 1;  // an odd last row: both halves load it
+      const T* row = static_cast<const T*>(p.q) + token * p.q_stride_t + hc * p.q_stride_h;
+      float x[8];
+      load8<T, FAST>(row + 8 * m, x);
+      rotate8<T, FAST>(x, row, m, p.pairs, p.interleaved, c, s, cos_row, sin_row);
+      // In place, other lanes' partner dims are this lane's.
+      if constexpr (!FAST) __syncwarp();
+      if (h < p.hq)
+        store8<T, FAST>(static_cast<T*>(p.rotated_q) + token * p.rq_stride_t +
+                            h * p.rq_stride_h + 8 * m, x);
+      continue;
+    }
+    const bool is_key = u < qu + ku;
+    const int h = 2 * (u - qu - (is_key ? 0 : ku)) + half;
+    const int hc = h < p.hkv ? h : p.hkv - 1;
+    const T* row = is_key ? static_cast<const T*>(p.k) + token * p.k_stride_t + hc * p.k_stride_h
+                          : static_cast<const T*>(p.v) + token * p.v_stride_t + hc * p.v_stride_h;
+    float x[8];
+    load8<T, FAST>(row + 8 * m, x);
+    if (is_key) {
+      rotate8<T, FAST>(x, row, m, p.pairs, p.interleaved, c, s, cos_row, sin_row);
+      if constexpr (!FAST) __syncwarp();
+      if (p.rotated_k != nullptr && h < p.hkv)
+        store8<T, FAST>(static_cast<T*>(p.rotated_k) + token * p.rk_stride_t +
+                            h * p.rk_stride_h + 8 * m, x);
+    }
+    const void* cen = is_key ? p.key_center : p.value_center;
+    if (cen != nullptr) {
+      float y[8];
+      load8<T, true>(static_cast<const T*>(cen) + (center * p.hkv + hc) * kHeadDim + 8 * m, y);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = __fsub_rn(x[i], y[i]);
+    }
+    __half scale, mid;
+    const uint32_t codes = int4_quantize8(x, scale, mid);
+    if (h >= p.hkv) continue;
+    uint8_t* rec = p.records + (page * p.hkv + h) * kInt4Record;
+    const int grp = m >> 2;
+    if (is_key) {
+      *reinterpret_cast<uint32_t*>(rec + tok * 64 + (m & 3) * 16 + grp * 4) = codes;
+    } else {
+      uint8_t* vr = rec + kInt4Value + value_code_row(tok) * 64 + (m & 3) * 16 + grp * 2;
+      *reinterpret_cast<uint16_t*>(vr) = static_cast<uint16_t>(codes);
+      *reinterpret_cast<uint16_t*>(vr + 8) = static_cast<uint16_t>(codes >> 16);
+    }
+    if ((m & 3) == 0) {
+      __half* meta =
+          reinterpret_cast<__half*>(rec + (is_key ? kInt4KeyMeta : kInt4ValueMeta) + tok * 16);
+      meta[grp] = scale;
+      meta[4 + grp] = mid;
+    }
+  }
+}
+
+struct Int4ReadParams {
+  const uint8_t* records;
+  int64_t num_pages;
+  const int32_t* slots;
+  int64_t tokens;
+  int32_t hkv;
+  void* key;    // [T, Hkv, 128]
+  void* value;  // [T, Hkv, 128]
+  int* error_flag;
+};
+
+// 16 lanes per (token, head, key or value); skipped slots read as zeros.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    pg_int4_read_kernel(const __grid_constant__ Int4ReadParams p) {
+  pdl_launch_dependents();
+  pdl_wait_primary();
+  const int m = threadIdx.x & 15;
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 4;
+  const int64_t th = row >> 1;
+  const int64_t token = th / p.hkv;
+  if (token >= p.tokens) return;
+  const int h = static_cast<int>(th - token * p.hkv);
+  const bool is_key = (row & 1) == 0;
+  T* out = static_cast<T*>(is_key ? p.key : p.value) + th * kHeadDim + 8 * m;
+  const int slot = p.slots[token];
+  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (slot >= 0 && (slot >> 4) >= p.num_pages) {
+    record_error(p.error_flag, kDevBadPageId);
+  } else if (slot >= 0) {
+    const int tok = slot & 15, grp = m >> 2;
+    const uint8_t* rec = p.records + (static_cast<int64_t>(slot >> 4) * p.hkv + h) * kInt4Record;
+    uint32_t w;
+    if (is_key) {
+      w = *reinterpret_cast<const uint32_t*>(rec + tok * 64 + (m & 3) * 16 + grp * 4);
+    } else {
+      const uint8_t* vr = rec + kInt4Value + value_code_row(tok) * 64 + (m & 3) * 16 + grp * 2;
+      w = *reinterpret_cast<const uint16_t*>(vr) |
+          (static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(vr + 8)) << 16);
+    }
+    const __half* meta = reinterpret_cast<const __half*>(
+        rec + (is_key ? kInt4KeyMeta : kInt4ValueMeta) + tok * 16);
+    const float s = __half2float(meta[grp]), mid = __half2float(meta[4 + grp]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float z = static_cast<float>(static_cast<int>((w >> (4 * i)) & 15u) - 8);
+      x[i] = __fadd_rn(__fmul_rn(z, s), mid);
+    }
+  }
+  if constexpr (sizeof(T) == 2) {
+    store8<T, true>(out, x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = from_float<T>(x[i]);
+  }
+}
+
+}  // namespace pg

@@ -1,0 +1,178 @@
+"""Rotary positions: tables scaled for long contexts, and the rotation of
+query and key rows in either pair layout over part or all of a head.
+
+The reference rotates inside its append, in one form (half layout, the whole
+128-dim head, FP16 arithmetic: tests/page_gauge_append_extension.cu); that
+form stays in ``runtime.AppendExtension`` and ``cache.rope_tables``.  Here
+the arithmetic is FP32 from FP32 tables, rounded once.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+
+DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+@dataclass(frozen=True)
+class RotaryScaling:
+    """How the frequencies of a model trained on ``trained_positions`` are
+    stretched by ``factor`` for longer contexts:
+
+    * ``linear``: every position is divided by the factor;
+    * ``ntk``: the base grows by ``factor ** (d / (d - 2))``, which divides the
+      lowest frequency by the factor and leaves the highest;
+    * ``parts``: frequencies that turn more than ``fast_turns`` times within the
+      trained positions stay, those that turn less than ``slow_turns`` times
+      are divided by the factor, those between are blended linearly over the
+      pair index, and both tables are multiplied by ``attention_factor``
+      (default ``0.1 ln(factor) + 1``).
+    """
+
+    kind: str
+    factor: float
+    trained_positions: int = 8192
+    fast_turns: float = 32.0
+    slow_turns: float = 1.0
+    attention_factor: float | None = None
+
+    def __post_init__(self):
+        if self.kind not in ("linear", "ntk", "parts"):
+            raise ValueError("rotary scaling must be 'linear', 'ntk' or 'parts'")
+        if not (math.isfinite(self.factor) and self.factor >= 1.0):
+            raise ValueError("the rotary scaling factor must be finite and at least 1")
+        if self.trained_positions <= 0 or not self.fast_turns > self.slow_turns > 0:
+            raise ValueError("trained positions must be positive and fast_turns > slow_turns > 0")
+
+
+def rotary_frequencies(rotary_dim: int, theta: float = 1.0e6,
+                       scaling: RotaryScaling | None = None) -> tuple[torch.Tensor, float]:
+    """Angle per position of each of the ``rotary_dim / 2`` pairs (float64)
+    and the factor on both tables."""
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be positive and even")
+    if not (math.isfinite(theta) and theta > 1.0):
+        raise ValueError("theta must be finite and above 1")
+    pairs = rotary_dim // 2
+    if scaling is not None and scaling.kind == "ntk" and rotary_dim > 2:
+        theta = theta * scaling.factor ** (rotary_dim / (rotary_dim - 2))
+    inv = theta ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+    if scaling is None or scaling.kind == "ntk":
+        return inv, 1.0
+    if scaling.kind == "linear":
+        return inv / scaling.factor, 1.0
+
+    def pair_of(turns: float) -> float:
+        return (rotary_dim * math.log(scaling.trained_positions / (turns * 2 * math.pi))
+                / (2 * math.log(theta)))
+
+    low = max(math.floor(pair_of(scaling.fast_turns)), 0)
+    high = min(math.ceil(pair_of(scaling.slow_turns)), rotary_dim - 1)
+    ramp = ((torch.arange(pairs, dtype=torch.float64) - low) / max(high - low, 1e-3)).clamp(0, 1)
+    scale = scaling.attention_factor
+    if scale is None:
+        scale = 0.1 * math.log(scaling.factor) + 1.0
+    return inv / scaling.factor * ramp + inv * (1 - ramp), float(scale)
+
+
+def rotary_tables(positions: int, rotary_dim: int = 128, theta: float = 1.0e6,
+                  scaling: RotaryScaling | None = None,
+                  device: torch.device | str = "cpu") -> tuple[torch.Tensor, torch.Tensor]:
+    """Cosine and sine tables [positions, rotary_dim / 2] in FP32.  The angles
+    are 64-bit products: at position 2^17 an FP32 angle would be off by 2^-7."""
+    if positions <= 0:
+        raise ValueError("positions must be positive")
+    inv, scale = rotary_frequencies(rotary_dim, theta, scaling)
+    t = torch.arange(positions, dtype=torch.float64, device=device)
+    angle = t[:, None] * inv.to(device)
+    return (angle.cos() * scale).float(), (angle.sin() * scale).float()
+
+
+def check_tables(cosine: torch.Tensor, sine: torch.Tensor, device: torch.device,
+                 head_dim: int) -> int:
+    """The number of rotated pairs of a table pair [positions, pairs]."""
+    if (cosine.dtype != torch.float32 or sine.dtype != torch.float32 or cosine.dim() != 2
+            or cosine.shape != sine.shape or cosine.size(0) == 0):
+        raise ValueError("cosine and sine must be matching float32 [positions, pairs] tables")
+    if cosine.device != device or sine.device != device:
+        raise ValueError("rotary tables must be on the rows' device")
+    pairs = cosine.size(1)
+    if cosine.stride() != sine.stride() or cosine.stride(1) != 1 or cosine.stride(0) < pairs:
+        raise ValueError("rotary tables must have equal strides and contiguous rows")
+    if not 1 <= pairs <= head_dim // 2:
+        raise ValueError("the tables rotate more dims than a head has")
+    return pairs
+
+
+def check_token_index(t: torch.Tensor, name: str, tokens: int, device: torch.device) -> None:
+    if (t.dtype != torch.int32 or t.dim() != 1 or t.numel() != tokens or t.device != device
+            or not t.is_contiguous()):
+        raise ValueError(f"{name} must be contiguous int32 [{tokens}] on the rows' device")
+
+
+def check_output(out: torch.Tensor, like: torch.Tensor, name: str) -> None:
+    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
+        raise ValueError(f"{name} must have its input's shape, dtype and device")
+    if out.stride(-1) != 1:
+        raise ValueError(f"{name} must have a contiguous last dimension")
+    if any(size > 1 and stride <= 0 for size, stride in zip(out.shape, out.stride())):
+        raise ValueError(f"{name} must not be expanded")
+
+
+def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, cosine: torch.Tensor,
+                 sine: torch.Tensor, positions: torch.Tensor, *, interleaved: bool = False,
+                 adjoint: bool = False, query_out: torch.Tensor | None = None,
+                 key_out: torch.Tensor | None = None):
+    """Rotate ``query`` [T, Hq, D] and ``key`` [T, Hkv, D] (or None) by
+    ``positions`` (device int32 [T]); returns (query_out, key_out).
+
+    ``cosine``/``sine`` are FP32 [positions, pairs] (``rotary_tables``); the
+    first ``2 * pairs`` dims turn, the others are copied.  Half layout pairs
+    dim j with j + pairs, ``interleaved`` 2j with 2j + 1.  ``adjoint`` turns
+    back (the gradient of the rotation with respect to its rows).  Rows are
+    float16, bfloat16 or float32 with a contiguous last dimension and any
+    other strides.  The outputs may be the inputs (in place); they must not
+    overlap them in any other way.  Rows of a token whose position is outside
+    the tables are not written (``runtime.read_device_error`` reports it)."""
+    if query.dtype not in DTYPES:
+        raise ValueError("rows must be float16, bfloat16 or float32")
+    tensors = [(query, query_out, "query")]
+    if key is not None:
+        tensors.append((key, key_out, "key"))
+    elif key_out is not None:
+        raise ValueError("key_out without key")
+    a = _lib.PgRotaryArgs()
+    outs: list = [None, None]
+    device, tokens, head_dim = query.device, query.size(0), query.size(-1)
+    for i, (x, y, name) in enumerate(tensors):
+        if not x.is_cuda or x.device != device or x.dtype != query.dtype:
+            raise ValueError(f"{name} must be a CUDA tensor of the query's device and dtype")
+        if x.dim() != 3 or x.size(0) != tokens or x.size(2) != head_dim:
+            raise ValueError(f"{name} must be [{tokens}, heads, {head_dim}]")
+        if x.stride(2) != 1 and x.numel():
+            raise ValueError(f"{name} must have a contiguous last dimension")
+        if y is None:
+            y = torch.empty(x.shape, dtype=x.dtype, device=device)
+        else:
+            check_output(y, x, f"{name}_out")
+        outs[i] = y
+        a.x[i], a.y[i] = x.data_ptr(), y.data_ptr()
+        a.x_stride_t[i], a.x_stride_h[i] = x.stride(0), x.stride(1)
+        a.y_stride_t[i], a.y_stride_h[i] = y.stride(0), y.stride(1)
+        a.heads[i] = x.size(1)
+    a.pairs = check_tables(cosine, sine, device, head_dim)
+    check_token_index(positions, "positions", tokens, device)
+    a.tokens, a.head_dim = tokens, head_dim
+    a.cosine, a.sine, a.positions = cosine.data_ptr(), sine.data_ptr(), positions.data_ptr()
+    a.table_rows, a.table_stride = cosine.size(0), cosine.stride(0)
+    a.interleaved, a.adjoint = int(interleaved), int(adjoint)
+    a.dtype = DTYPES[query.dtype]
+    with torch.cuda.device(device):
+        _lib.call("pg_rotary", ctypes.byref(a), torch.cuda.current_stream().cuda_stream)
+    return outs[0], outs[1]

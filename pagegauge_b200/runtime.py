@@ -11,9 +11,13 @@ CUDA stream; nothing is allocated on the device.
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
+from .int4 import check_records
+from .rotary import DTYPES, check_output, check_tables, check_token_index
 
 HEAD_DIM = 128
 PAGE = 16
@@ -289,6 +293,82 @@ class AppendExtension:
             key.stride(0), value.stride(0), cstride, query.size(0), query.size(1), key.size(1),
             exact_k.size(0), codes_k.size(0), int(sink), position, device_position,
             rope_stride, rope_rows, _stream(query))
+
+    def rope_append_int4(self, query, key, value, cosine, sine, positions, token_slots,
+                         rotated_query, records, key_center=None, value_center=None,
+                         center_rows=None, rotated_key=None, interleaved: bool = False) -> None:
+        """Rotate the query and key rows of any number of tokens and append
+        their keys and values to a 4-bit pool (no counterpart in the
+        reference, whose appends take one token per request).
+
+        ``query`` [T,Hq,128], ``key``/``value`` [T,Hkv,128] are float16 or
+        bfloat16 with a contiguous last dimension (views of a packed
+        projection are fine); ``cosine``/``sine`` FP32 [positions,pairs] from
+        ``rotary.rotary_tables`` (``pairs`` < 64 rotates part of the head);
+        ``positions`` and ``token_slots`` (physical page * 16 + token) device
+        int32 [T].  A negative slot skips its token (padding): none of its
+        rows is read or written.  Every other slot may occur once per call.
+        ``records`` is the pool's [pages,Hkv,2560] uint8.  With
+        ``key_center``/``value_center`` [C,Hkv,128] the rows' centres (row
+        ``center_rows[t]``, or row 0) are subtracted before quantising; the
+        decode adds the value centre back.  ``rotated_query`` and the optional
+        ``rotated_key`` take the rotated rows and may be the inputs."""
+        _require(query.is_cuda and query.dim() == 3, "query must be CUDA of rank three")
+        _require(query.dtype in (torch.float16, torch.bfloat16),
+                 "query must be float16 or bfloat16")
+        tokens, device = query.size(0), query.device
+        for name, t in (("query", query), ("key", key), ("value", value)):
+            _require(t.device == device and t.dtype == query.dtype,
+                     f"{name} must have the query's device and dtype")
+            _require(t.dim() == 3 and t.size(0) == tokens and t.size(1) > 0
+                     and t.size(2) == HEAD_DIM, f"{name} must be [{tokens},heads,{HEAD_DIM}]")
+            _require(t.stride(2) == 1 or tokens == 0,
+                     f"{name} must have a contiguous last dimension")
+        _require(key.shape == value.shape, "K/V input shapes must match")
+        kv_heads = key.size(1)
+        check_output(rotated_query, query, "rotated_query")
+        pairs = check_tables(cosine, sine, device, HEAD_DIM)
+        check_token_index(positions, "positions", tokens, device)
+        check_token_index(token_slots, "token_slots", tokens, device)
+        check_records(records)
+        _require(records.device == device and records.size(1) == kv_heads,
+                 "records must be [pages,Hkv,2560] on the rows' device")
+        a = _lib.PgInt4AppendArgs()
+        if rotated_key is not None:
+            check_output(rotated_key, key, "rotated_key")
+            a.rotated_key = rotated_key.data_ptr()
+            a.rk_stride_t, a.rk_stride_h = rotated_key.stride(0), rotated_key.stride(1)
+        _require((key_center is None) == (value_center is None),
+                 "key and value centers are both given or both None")
+        if key_center is not None:
+            for name, t in (("key_center", key_center), ("value_center", value_center)):
+                _require(t.device == device and t.dtype == query.dtype and t.is_contiguous()
+                         and t.dim() == 3 and t.size(0) > 0
+                         and tuple(t.shape[1:]) == (kv_heads, HEAD_DIM),
+                         f"{name} must be contiguous [rows,{kv_heads},{HEAD_DIM}] of the "
+                         "query's dtype")
+            _require(key_center.size(0) == value_center.size(0), "center row counts must match")
+            a.key_center, a.value_center = key_center.data_ptr(), value_center.data_ptr()
+            a.num_centers = key_center.size(0)
+            if center_rows is not None:
+                check_token_index(center_rows, "center_rows", tokens, device)
+                a.center_rows = center_rows.data_ptr()
+        else:
+            _require(center_rows is None, "center_rows without centers")
+        a.query, a.key, a.value = query.data_ptr(), key.data_ptr(), value.data_ptr()
+        a.rotated_query = rotated_query.data_ptr()
+        a.q_stride_t, a.q_stride_h = query.stride(0), query.stride(1)
+        a.k_stride_t, a.k_stride_h = key.stride(0), key.stride(1)
+        a.v_stride_t, a.v_stride_h = value.stride(0), value.stride(1)
+        a.rq_stride_t, a.rq_stride_h = rotated_query.stride(0), rotated_query.stride(1)
+        a.cosine, a.sine = cosine.data_ptr(), sine.data_ptr()
+        a.table_stride, a.table_rows = cosine.stride(0), cosine.size(0)
+        a.positions, a.slots = positions.data_ptr(), token_slots.data_ptr()
+        a.records, a.num_pages = records.data_ptr(), records.size(0)
+        a.tokens, a.query_heads, a.kv_heads = tokens, query.size(1), kv_heads
+        a.pairs, a.interleaved, a.dtype = pairs, int(interleaved), DTYPES[query.dtype]
+        with torch.cuda.device(device):
+            _lib.call("pg_rope_append_int4", ctypes.byref(a), _stream(query))
 
     def exact_tail_merge_center(self, query, exact_key_pages, exact_value_pages,
                                 exact_page_indices, exact_last_page_len, old_output, old_lse,

@@ -11,6 +11,8 @@ PageGauge reference drives, backed by the sm_100a split-KV kernels.
   "affine_group16" representation: INT8 codes with an FP16 scale and bias
   per (page, KV head, 16-dim group); ``run(q, (k_codes, v_codes), k_bias,
   k_scale, v_bias, v_scale, sm_scale, out=, lse=, return_lse=)``.
+* ``make_int4_wrapper(workspace=...)`` decodes a 4-bit pool (``int4``), without
+  a counterpart in the reference.
 * ``BatchDecodeWithPagedKVCacheWrapper(workspace, "NHD", ...)`` is the FP16
   paged decode used for the exact tail segment and the FP16 baseline.
 * ``plan(wrapper, indptr, indices, last_page_len, kv_dtype, fixed_split_pages)``
@@ -31,6 +33,8 @@ import numpy as np
 import torch
 
 from . import _lib
+from .int4 import check_records
+from .rotary import DTYPES, check_output
 
 HEAD_DIM = 128
 PAGE = 16
@@ -236,6 +240,7 @@ class BatchDecodeWithPagedKVCacheWrapper:
         self._last_len: torch.Tensor | None = None
         self._sm_scale = 1.0 / math.sqrt(HEAD_DIM)
         self._kv_dtype = torch.int8 if self.page_gauge else torch.float16
+        self._first_segment = self.page_gauge  # quantised pages are segment 0
         self.plan_invocations = 0
 
     @property
@@ -260,7 +265,7 @@ class BatchDecodeWithPagedKVCacheWrapper:
             raise ValueError("num_qo_heads must be a multiple (1..8) of num_kv_heads")
         kvd = kv_data_type if kv_data_type is not None else data_type
         if kvd is not None:
-            want = torch.int8 if self.page_gauge else torch.float16
+            want = self._kv_dtype
             if kvd != want:
                 raise ValueError(f"this wrapper decodes {want} pages, got {kvd}")
         for name, t in (("indptr", indptr), ("indices", indices), ("last_page_len", last_page_len)):
@@ -289,8 +294,8 @@ class BatchDecodeWithPagedKVCacheWrapper:
         if disable_split_kv:
             split = 1 << 30
         sms = num_sms(self._ws.buffer.device)
-        seg0 = ind if self.page_gauge else None
-        seg1 = None if self.page_gauge else ind
+        seg0 = ind if self._first_segment else None
+        seg1 = None if self._first_segment else ind
         items, off, info = plan_items(batch, num_kv_heads, seg0, seg1,
                                       min(split, 1 << 30), min(split, 1 << 30), sms)
         self._plan = PagedDecodePlan(self._ws, items, off, info, batch, num_kv_heads,
@@ -306,7 +311,7 @@ class BatchDecodeWithPagedKVCacheWrapper:
     def split_pages(self) -> int:
         if self._plan is None:
             raise RuntimeError("plan() has not been called")
-        return self._plan.split_pages[0 if self.page_gauge else 1]
+        return self._plan.split_pages[0 if self._first_segment else 1]
 
     def run(self, q: torch.Tensor, paged_kv_cache, *args, q_scale=None, k_scale=None,
             v_scale=None, out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
@@ -359,6 +364,100 @@ class BatchDecodeWithPagedKVCacheWrapper:
         return (out, lse) if return_lse else out
 
     forward = run
+
+
+class Int4DecodeWrapper(BatchDecodeWithPagedKVCacheWrapper):
+    """Decode over a 4-bit pool (``int4.Int4PagePool``): ``plan`` as the other
+    wrappers' (``kv_data_type`` torch.uint8), ``run(q, records, sm_scale,
+    value_center=, out=, lse=, return_lse=)`` with ``q`` and ``out`` float16
+    or bfloat16 [B,Hq,128].  Requests without pages give zeros and -inf.  One
+    wrapper's workspace serves one run at a time: concurrent streams (or
+    graphs replayed concurrently) need a wrapper each."""
+
+    def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD", **kwargs):
+        super().__init__(float_workspace_buffer, kv_layout, **kwargs)
+        if self.page_gauge:
+            raise ValueError("choose one representation")
+        self._kv_dtype = torch.uint8
+        self._first_segment = True
+
+    def plan(self, indptr: torch.Tensor, indices: torch.Tensor, last_page_len: torch.Tensor,
+             *args, **kwargs) -> None:
+        device = self._ws.buffer.device
+        for name, t in (("indices", indices), ("last_page_len", last_page_len)):
+            if t.is_cuda and (t.device != device or not t.is_contiguous()):
+                raise ValueError(f"{name} must be contiguous on the workspace's device")
+        if indices.numel() < int(indptr[-1]):
+            raise ValueError("indptr counts more pages than indices has")
+        with torch.cuda.device(device):
+            super().plan(indptr, indices, last_page_len, *args, **kwargs)
+
+    begin_forward = plan
+
+    def run(self, q: torch.Tensor, records, sm_scale: float | None = None, *,
+            value_center: torch.Tensor | None = None, out: torch.Tensor | None = None,
+            lse: torch.Tensor | None = None, return_lse: bool = False):
+        plan = self._plan
+        if plan is None:
+            raise RuntimeError("plan() must be called before run()")
+        records = getattr(records, "records", records)
+        check_records(records)
+        device = self._ws.buffer.device
+        if records.device != device or records.size(1) != self._num_kv_heads:
+            raise ValueError(f"records must be [pages,{self._num_kv_heads},2560] on the "
+                             "workspace's device")
+        if (q.dtype not in (torch.float16, torch.bfloat16) or q.device != device
+                or tuple(q.shape) != (plan.batch, self._num_qo_heads, HEAD_DIM)):
+            raise ValueError(f"q must be float16 or bfloat16 "
+                             f"[{plan.batch},{self._num_qo_heads},{HEAD_DIM}] on the "
+                             "workspace's device")
+        if q.stride(2) != 1:
+            raise ValueError("q must have a contiguous last dimension")
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        else:
+            check_output(out, q, "out")
+        if lse is None and return_lse:
+            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=device)
+        if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2]
+                                or lse.device != device or not lse.is_contiguous()):
+            raise ValueError(f"lse must be contiguous float32 [{plan.batch},"
+                             f"{self._num_qo_heads}] on the workspace's device")
+        a = _lib.PgInt4DecodeArgs()
+        if value_center is not None:
+            if (value_center.dtype != q.dtype or value_center.device != device
+                    or not value_center.is_contiguous()
+                    or tuple(value_center.shape) != (plan.batch, self._num_kv_heads, HEAD_DIM)):
+                raise ValueError(f"value_center must be contiguous [{plan.batch},"
+                                 f"{self._num_kv_heads},{HEAD_DIM}] of q's dtype")
+            a.value_center, a.vc_stride_b = value_center.data_ptr(), value_center.stride(0)
+        a.q, a.q_stride_b, a.q_stride_h = q.data_ptr(), q.stride(0), q.stride(1)
+        a.out, a.out_stride_b, a.out_stride_h = out.data_ptr(), out.stride(0), out.stride(1)
+        a.lse_out = None if lse is None else lse.data_ptr()
+        a.records, a.num_pages = records.data_ptr(), records.size(0)
+        a.indices, a.last_page_len = self._indices.data_ptr(), self._last_len.data_ptr()
+        a.items, a.item_off = plan.items_ptr, plan.off_ptr
+        a.part_o, a.part_lse = plan.o_ptr, plan.lse_ptr
+        a.num_items, a.batch = plan.num_items, plan.batch
+        a.kv_heads, a.group = plan.kv_heads, plan.group
+        a.final_mode = int(plan.single and plan.num_items > 0)
+        a.dtype = DTYPES[q.dtype]
+        a.sm_scale = self._sm_scale if sm_scale is None else float(sm_scale)
+        with torch.cuda.device(device):
+            _lib.call("pg_decode_int4_run", ctypes.byref(a), _stream(q))
+        return (out, lse) if return_lse else out
+
+    forward = run
+
+
+def make_int4_wrapper(flashinfer=None, workspace: torch.Tensor | None = None,
+                      **wrapper_kwargs) -> Int4DecodeWrapper:
+    """The decode over a 4-bit pool, made as the INT8 wrappers are (the
+    ``flashinfer`` argument is ignored; the reference has no 4-bit cache)."""
+    if workspace is None:
+        raise ValueError("a CUDA uint8 workspace is required")
+    wrapper_kwargs.pop("jit_args", None)
+    return Int4DecodeWrapper(workspace, "NHD", **wrapper_kwargs)
 
 
 def make_page_gauge_wrapper(flashinfer=None, workspace: torch.Tensor | None = None,

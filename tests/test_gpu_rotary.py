@@ -1,0 +1,166 @@
+"""GPU parity of apply_rotary with the float64 oracle.
+
+Bound per element: the result is rounded once (half a step of its type), and
+before that each of the two products and their sum are rounded in FP32, so
+the sum is off by at most 2 * 2^-24 (|a c| + |b s|) to first order (3 * is
+used)."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import int4_oracle as I
+from pagegauge_b200.rotary import RotaryScaling, apply_rotary, rotary_tables
+from pagegauge_b200.runtime import read_device_error
+
+pytestmark = pytest.mark.gpu
+
+
+def rows(tokens, heads, dim, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(tokens, heads, dim, generator=g) * 2).to(dtype)
+
+
+def check(got, x, cos, sin, interleaved=False, adjoint=False):
+    x64, c, s = (t.double().cpu().numpy() for t in (x, cos, sin))
+    exp = I.rotate(x64, c, s, interleaved, adjoint)
+    size = I.rotate(np.abs(x64), np.abs(c), -np.abs(s), interleaved)  # |a c| + |b s| at a
+    other = I.rotate(np.abs(x64), np.abs(c), np.abs(s), interleaved)  # and at b
+    size = np.maximum(np.abs(size), np.abs(other))
+    eps = torch.finfo(got.dtype).eps / 2
+    tiny = float(torch.finfo(got.dtype).smallest_normal) * 2 * eps
+    bound = eps * (np.abs(exp) + 1e-6 * size) + 3 * 2.0 ** -24 * size + tiny
+    err = np.abs(got.double().cpu().numpy() - exp)
+    assert (err <= bound).all(), float((err / bound).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim,rotary_dim", [(128, 128), (128, 64), (80, 80), (80, 34), (64, 62),
+                                            (256, 256), (6, 2), (96, 96), (31, 30), (128, 8)])
+def test_layouts_and_parts_of_the_head(cuda_lib, dtype, interleaved, dim, rotary_dim):
+    tokens, hq, hkv = 37, 5, 2
+    q, k = rows(tokens, hq, dim, dtype, 1).cuda(), rows(tokens, hkv, dim, dtype, 2).cuda()
+    cos, sin = rotary_tables(4096, rotary_dim, device="cuda")
+    g = torch.Generator().manual_seed(3)
+    pos = torch.randint(0, 4096, (tokens,), generator=g).int().cuda()
+    for adjoint in (False, True):
+        qo, ko = apply_rotary(q, k, cos, sin, pos, interleaved=interleaved, adjoint=adjoint)
+        at = pos.long()
+        check(qo, q, cos[at], sin[at], interleaved, adjoint)
+        check(ko, k, cos[at], sin[at], interleaved, adjoint)
+    assert read_device_error() == 0
+
+
+@pytest.mark.parametrize("tokens", [0, 1, 2, 3, 129, 4097])
+def test_token_counts(cuda_lib, tokens):
+    q, k = rows(tokens, 8, 128, torch.float16, 4).cuda(), rows(tokens, 2, 128, torch.float16,
+                                                               5).cuda()
+    cos, sin = rotary_tables(70000, 128, scaling=RotaryScaling("parts", 8.0), device="cuda")
+    pos = torch.arange(60000, 60000 + tokens, dtype=torch.int32, device="cuda")
+    qo, ko = apply_rotary(q, k, cos, sin, pos)
+    assert qo.shape == q.shape and ko.shape == k.shape
+    if tokens:
+        check(qo, q, cos[pos.long()], sin[pos.long()])
+        check(ko, k, cos[pos.long()], sin[pos.long()])
+
+
+@pytest.mark.parametrize("offset", [0, 1, 4, 8])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_strided_views_in_place_and_out_of_place(cuda_lib, offset, interleaved, dtype):
+    """Packed projection rows at odd offsets and strides; the dims and rows
+    around the views stay as they were."""
+    tokens, hq, hkv, dim = 19, 6, 2, 64
+    width = (hq + 2 * hkv) * dim + 2 * offset
+    flat = rows(tokens, 1, width, dtype, 6).cuda().view(tokens, width)
+    body = flat[:, offset:offset + (hq + 2 * hkv) * dim].unflatten(1, (hq + 2 * hkv, dim))
+    q, k = body[:, :hq], body[:, hq:hq + hkv]
+    cos, sin = rotary_tables(64, 48, device="cuda")
+    pos = torch.arange(tokens, dtype=torch.int32, device="cuda").flip(0).contiguous()
+    before = flat.clone()
+    qo, ko = apply_rotary(q, k, cos, sin, pos, interleaved=interleaved)
+    assert torch.equal(flat, before)
+    at = pos.long()
+    check(qo, q, cos[at], sin[at], interleaved)
+    heads_first = torch.zeros(hkv, tokens, dim, dtype=dtype, device="cuda").transpose(0, 1)
+    apply_rotary(q, k, cos, sin, pos, interleaved=interleaved, query_out=q, key_out=heads_first)
+    assert torch.equal(q, qo) and torch.equal(heads_first, ko)
+    assert torch.equal(flat[:, :offset], before[:, :offset])
+    assert torch.equal(flat[:, offset + hq * dim:], before[:, offset + hq * dim:])
+
+
+def test_query_alone_and_bad_positions_leave_rows(cuda_lib):
+    q = rows(5, 3, 128, torch.float16, 7).cuda()
+    cos, sin = rotary_tables(16, 128, device="cuda")
+    pos = torch.tensor([3, -1, 15, 16, 0], dtype=torch.int32, device="cuda")
+    out = torch.full_like(q, 7.0)
+    got, none = apply_rotary(q, None, cos, sin, pos, query_out=out)
+    assert none is None and got is out
+    assert read_device_error() == 2
+    assert (out[[1, 3]] == 7).all()
+    keep = torch.tensor([0, 2, 4], device="cuda")
+    check(out[keep], q[keep], cos[pos[keep].long()], sin[pos[keep].long()])
+
+
+def test_adjoint_is_the_gradient(cuda_lib):
+    """<R x, y> = <x, R^T y>, and central differences of <R x, y> in FP32."""
+    x, y = rows(4, 2, 32, torch.float32, 8).cuda(), rows(4, 2, 32, torch.float32, 9).cuda()
+    cos, sin = rotary_tables(128, 24, scaling=RotaryScaling("parts", 4.0), device="cuda")
+    pos = torch.tensor([0, 5, 77, 127], dtype=torch.int32, device="cuda")
+    for interleaved in (False, True):
+        grad, _ = apply_rotary(y, None, cos, sin, pos, interleaved=interleaved, adjoint=True)
+        f = lambda v: float((apply_rotary(v, None, cos, sin, pos,  # noqa: E731
+                                          interleaved=interleaved)[0].double() * y).sum())
+        for i in ((0, 0, 0), (2, 1, 13), (3, 0, 23), (3, 1, 24), (1, 1, 31)):
+            up, down = x.clone(), x.clone()
+            up[i] += 1.0
+            down[i] -= 1.0
+            # The map is linear; each f is off by FP32 rounding of 256 products.
+            assert abs((f(up) - f(down)) / 2 - float(grad[i])) < 256 * 2.0 ** -22 * 40
+
+
+def test_capture_and_another_stream(cuda_lib):
+    q, k = rows(33, 4, 128, torch.bfloat16, 10).cuda(), rows(33, 2, 128, torch.bfloat16,
+                                                             11).cuda()
+    cos, sin = rotary_tables(256, 128, device="cuda")
+    pos = torch.arange(33, dtype=torch.int32, device="cuda")
+    qo, ko = torch.empty_like(q), torch.empty_like(k)
+    exp = [t.clone() for t in apply_rotary(q, k, cos, sin, pos)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        apply_rotary(q, k, cos, sin, pos, query_out=qo, key_out=ko)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(qo, exp[0]) and torch.equal(ko, exp[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        apply_rotary(q, k, cos, sin, pos, query_out=qo, key_out=ko)
+    pos += 100
+    graph.replay()
+    exp = apply_rotary(q, k, cos, sin, pos)
+    assert torch.equal(qo, exp[0]) and torch.equal(ko, exp[1])
+
+
+def test_refusals(cuda_lib):
+    q, k = rows(4, 2, 64, torch.float16, 12).cuda(), rows(4, 1, 64, torch.float16, 13).cuda()
+    cos, sin = rotary_tables(8, 64, device="cuda")
+    pos = torch.zeros(4, dtype=torch.int32, device="cuda")
+    wide = rotary_tables(8, 128, device="cuda")
+    for args, kw in (((q, k, *wide, pos), {}), ((q, k, cos.half(), sin.half(), pos), {}),
+                     ((q, k, cos, sin[:4], pos), {}), ((q, k, cos, sin, pos.long()), {}),
+                     ((q, k, cos, sin, pos[:3]), {}), ((q, k, cos, sin, pos.cpu()), {}),
+                     ((q, k, cos.cpu(), sin.cpu(), pos), {}), ((q, k[:3], cos, sin, pos), {}),
+                     ((q, k.bfloat16(), cos, sin, pos), {}),
+                     ((q.transpose(1, 2), None, cos, sin, pos), {}),
+                     ((q, None, cos, sin, pos), dict(key_out=k)),
+                     ((q, k, cos, sin, pos), dict(query_out=q[:, :1].expand(4, 2, 64))),
+                     ((q, k, cos, sin, pos), dict(query_out=torch.empty_like(q).float())),
+                     ((q, k, cos, sin, pos), dict(key_out=torch.empty(4, 2, 64).cuda().half()))):
+        with pytest.raises(ValueError):
+            apply_rotary(*args, **kw)
+    assert math.isfinite(float(q.float().sum()))

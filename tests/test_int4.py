@@ -1,0 +1,125 @@
+"""The 4-bit cache on the CPU: the record layout and the quantiser's bounds in
+the oracle, and the refusals of the C entries and the Python classes."""
+
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import int4_oracle as I
+from pagegauge_b200 import _lib
+from pagegauge_b200.int4 import Int4PagePool
+
+
+def test_codes_fill_a_record_once():
+    seen = np.zeros((I.RECORD, 2), int)
+    for t in range(16):
+        for d in range(128):
+            seen[I.key_byte(t, d)] += 1
+            seen[I.value_byte(t, d)] += 1
+    assert (seen[:2048] == 1).all() and (seen[2048:] == 0).all()
+
+
+def test_store_and_load_round_trip():
+    rng = np.random.default_rng(1)
+    records = rng.integers(0, 256, (3, 2, I.RECORD), np.uint8)
+    x = rng.standard_normal((2, 128)).astype(np.float32)
+    k, v = (I.quantise(row) for row in x)
+    other = records.copy()
+    I.store_token(records, 1, 1, 5, k, v)
+    (ka, km), (va, vm) = I.load(records[1, 1])
+    for (z, s, m), got in ((k, ka[5] + km[5]), (v, va[5] + vm[5])):
+        exp = (z.astype(float) - 8) * np.repeat(s.astype(float), 32) + np.repeat(m.astype(float), 32)
+        assert np.array_equal(got, exp)
+    touched = np.argwhere(records[1, 1] != other[1, 1])
+    assert len(touched) <= 160 and np.array_equal(records[0], other[0])
+
+
+@pytest.mark.parametrize("scale", [1e-6, 1e-3, 1.0, 300.0, 4e4])
+@pytest.mark.parametrize("offset", [0.0, 50.0])
+def test_quantiser_error_is_half_a_step(scale, offset):
+    """|x - x'| <= s/2 inside the codes' range; beyond it the scale's and the
+    midpoint's roundings (2^-11 relative, or half a subnormal step) add."""
+    rng = np.random.default_rng(2)
+    x = (rng.standard_normal((64, 128)) * scale + offset).astype(np.float32)
+    x = np.clip(x, -65504, 65504)
+    z, s, m = (t.astype(np.float64) for t in I.quantise(x))
+    s, m = np.repeat(s, 32, -1), np.repeat(m, 32, -1)
+    err = np.abs((z - 8) * s + m - x)
+    slack = 15 * np.maximum(s * 2.0 ** -11, 2.0 ** -25) + np.maximum(np.abs(m) * 2.0 ** -11,
+                                                                     2.0 ** -25)
+    assert (err <= s * (0.5 + 2.0 ** -20) + slack).all()
+
+
+def test_constant_groups_are_held_to_one_rounding():
+    x = np.repeat(np.float32([3.0, -7.5, 0.0, 1000.25]), 32)[None]
+    z, s, m = I.quantise(x)
+    assert (s == 0).all() and (z == 8).all()
+    assert np.array_equal(np.repeat(m, 32, -1), x.astype(np.float16))
+
+
+def append_args(**kw):
+    a = _lib.PgInt4AppendArgs()
+    a.query = a.key = a.value = a.rotated_query = a.records = 0x1000
+    a.cosine = a.sine = a.positions = a.slots = 0x1000
+    a.table_rows, a.table_stride, a.pairs = 8, 64, 64
+    a.num_pages, a.tokens, a.query_heads, a.kv_heads = 4, 1, 4, 1
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def decode_args(**kw):
+    a = _lib.PgInt4DecodeArgs()
+    a.q = a.out = a.records = a.indices = a.last_page_len = a.items = a.item_off = 0x1000
+    a.part_o = a.part_lse = 0x1000
+    a.num_items, a.batch, a.kv_heads, a.group, a.num_pages, a.sm_scale = 2, 1, 1, 4, 4, 0.1
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("entry,make,bad", [
+    ("pg_rope_append_int4", append_args,
+     [dict(dtype=2), dict(tokens=-1), dict(query_heads=0), dict(kv_heads=0), dict(pairs=65),
+      dict(pairs=0), dict(table_rows=0), dict(table_stride=63), dict(num_pages=0),
+      dict(num_pages=1 << 27), dict(key_center=0x1000), dict(records=0x1008),
+      dict(records=None), dict(slots=None), dict(rotated_query=None),
+      dict(key_center=0x1000, value_center=0x1000, num_centers=0)]),
+    ("pg_decode_int4_run", decode_args,
+     [dict(batch=0), dict(group=9), dict(group=0), dict(sm_scale=0.0),
+      dict(sm_scale=float("nan")), dict(dtype=2), dict(q=0x1002), dict(q_stride_h=3),
+      dict(out=None), dict(num_items=-1), dict(num_pages=0), dict(records=0x1004),
+      dict(indices=None), dict(items=None), dict(item_off=None), dict(part_o=None)]),
+])
+def test_c_entries_refuse(entry, make, bad):
+    fn = getattr(_lib.load(), entry)
+    assert fn(None, None) == 1
+    for kw in bad:
+        assert fn(ctypes.byref(make(**kw)), None) == 1, kw
+        assert _lib.load().pg_last_error()
+    if entry == "pg_rope_append_int4":
+        assert fn(ctypes.byref(make(tokens=0)), None) == 0
+
+
+def test_read_refuses():
+    fn = _lib.load().pg_int4_read
+    good = [0x1000, 4, 1, 0x1000, 1, 0x1000, 0x1000, 0, None]
+    for i, v in ((0, None), (0, 0x1004), (1, 0), (2, 0), (3, None), (4, -1), (5, 0x1008), (7, 3)):
+        bad = list(good)
+        bad[i] = v
+        assert fn(*bad) == 1, (i, v)
+    good[4] = 0
+    assert fn(*good) == 0
+
+
+def test_pool_refuses():
+    with pytest.raises(ValueError):
+        Int4PagePool(0, 8, device="cpu")
+    with pytest.raises(ValueError, match="CUDA"):
+        Int4PagePool(2, 8, device="cpu")
+    with pytest.raises(ValueError):
+        Int4PagePool(2, 8, records=torch.zeros(2, 8, 2559, dtype=torch.uint8))
