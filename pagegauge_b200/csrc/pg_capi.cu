@@ -166,6 +166,27 @@ int32_t ensure_decode_smem() {
   return PG_OK;
 }
 
+int32_t ensure_int4_smem() {
+  static std::mutex mu;
+  static bool done[64] = {false};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
+    return fail(PG_ERR_CUDA, "cudaGetDevice failed");
+  std::lock_guard<std::mutex> lock(mu);
+  if (done[dev]) return PG_OK;
+  int32_t rc = cuda_check(cudaFuncSetAttribute(pg::pg_decode_int4_kernel<__half>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               pg::kInt4SmemBytes),
+                          "cudaFuncSetAttribute(int4 decode smem)");
+  if (rc != PG_OK) return rc;
+  rc = cuda_check(cudaFuncSetAttribute(pg::pg_decode_int4_kernel<__nv_bfloat16>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       pg::kInt4SmemBytes),
+                  "cudaFuncSetAttribute(int4 decode smem)");
+  if (rc == PG_OK) done[dev] = true;
+  return rc;
+}
+
 int32_t launch_decode(const pg::DecodeParams& p, const CUtensorMap& k8,
                       const CUtensorMap& v8, const CUtensorMap& k16,
                       const CUtensorMap& v16, int num_ctas, int warps,
@@ -1271,15 +1292,17 @@ int32_t pg_decode_int4_run(const pg_int4_decode_args* a, void* stream) {
   const bool half = a->dtype == PG_DTYPE_F16;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (a->num_items > 0) {
-    int32_t rc = launch_pdl(half ? pg::pg_decode_int4_kernel<__half>
-                                 : pg::pg_decode_int4_kernel<__nv_bfloat16>,
-                            dim3(a->num_items), dim3(pg::kInt4Warps * 32), 0, st,
-                            "int4 decode launch", p);
+    int32_t rc = ensure_int4_smem();
+    if (rc != PG_OK) return rc;
+    rc = launch_pdl(half ? pg::pg_decode_int4_kernel<__half>
+                         : pg::pg_decode_int4_kernel<__nv_bfloat16>,
+                    dim3(a->num_items), dim3(pg::kInt4Warps * 32), pg::kInt4SmemBytes, st,
+                    "int4 decode launch", p);
     if (rc != PG_OK || final_mode) return rc;
   }
   return launch_pdl(half ? pg::pg_int4_merge_kernel<__half>
                          : pg::pg_int4_merge_kernel<__nv_bfloat16>,
-                    dim3(a->batch * a->kv_heads * a->group), dim3(pg::kHeadDim), 0, st,
+                    dim3(a->batch * a->kv_heads * a->group), dim3(256), 0, st,
                     "int4 merge launch", p);
 }
 

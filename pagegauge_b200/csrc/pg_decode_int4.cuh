@@ -1,6 +1,29 @@
 // Decode attention over the 4-bit paged cache (record layout: pg_int4.cuh):
-// one query token per request, GQA group of up to 8 query heads per KV head,
-// split over the planner's work items (request, KV head, run of pages).
+// one query token per request, a GQA group of up to 8 query heads per KV
+// head, split over the planner's work items (request, KV head, run of pages).
+//
+// Every warp owns a ring of records in shared memory (one 2560-byte bulk copy
+// per page) and computes, per page of 16 tokens,
+//   S^T = K (16 tok x 128) . Q^T (128 x 8 rows)
+//   O^T += V^T (128 x 16 tok) . P^T (16 tok x 8 rows)
+// on the FP16 tensor path with FP32 accumulators.  The codes need no
+// conversion: a code z in the low bits of a half is the subnormal z 2^-24
+// (z 2^-20 one nibble higher), exact in the product, so one AND makes two
+// operands.  A word of key codes holds 8 dims of one token and its nibble i
+// and i + 4 are one operand register; the query's odd dims are divided by 16
+// to match.  The rows are first scaled by a power of two that brings their
+// largest element to [512, 1024), so that this division loses nothing.
+//
+// The scales and midpoints come after the products.  With qs_g = the sum of
+// q over group g's 32 dims,
+//   score = sum_g s_g (sum_d q_d z_d - 8 qs_g) + m_g qs_g
+// -8 qs_g is the initial accumulator of group g's products, and the last
+// term one TF32 product with qs split in two (22 bits).  For the values
+//   O_d = sum_t (P_t s_tg) z_td - 8 sum_t (P_t s_tg) + sum_t P_t m_tg
+// where P s is formed in FP32 and rounded once to FP16, and the two last sums
+// come from tensor-core products of the same rounded operands, so that a
+// rounding of P s weighs (z - 8) s and not z s.  P <= 4 (the running maximum
+// is raised when a score passes it by 2 in log2), so P s <= 4 * 8734.
 #pragma once
 
 #include "pg_decode_core.cuh"
@@ -31,6 +54,240 @@ struct Int4DecodeParams {
 };
 
 constexpr int kInt4Warps = 4;
+constexpr int kInt4Stages = 5;
+constexpr int kInt4CtasPerSm = 4;
+constexpr int kInt4RingBytes = kInt4Stages * kInt4Record;
+// The warps' rings, then their barriers; the epilogue reuses the rings.
+constexpr int kInt4SmemBytes = kInt4Warps * (kInt4RingBytes + kInt4Stages * 8);
+static_assert(kInt4Warps * (16 + 8 * kCoStride) * 4 <= kInt4Warps * kInt4RingBytes,
+              "the combine buffer lies in the rings");
+// The running maximum is raised when a score passes it by this (log2).
+constexpr float kInt4Slack = 2.f;
+
+// D = A(16x16 f16) * B(16x8 f16) + C.
+__device__ __forceinline__ void mma_16816_c(float* d, uint32_t a0, uint32_t a1, uint32_t a2,
+                                            uint32_t a3, uint32_t b0, uint32_t b1, float c0,
+                                            float c1, float c2, float c3) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2),
+        "f"(c3));
+}
+__device__ __forceinline__ void mma_16816_acc(float* d, uint32_t a0, uint32_t a1, uint32_t a2,
+                                              uint32_t a3, uint32_t b0, uint32_t b1) {
+  mma_16816_c(d, a0, a1, a2, a3, b0, b1, d[0], d[1], d[2], d[3]);
+}
+// D = A(16x8 tf32) * B(8x8 tf32).
+__device__ __forceinline__ void mma_1688_tf32(float* d, float a0, float a1, float a2, float a3,
+                                              float b0, float b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(__float_as_uint(a0)), "r"(__float_as_uint(a1)), "r"(__float_as_uint(a2)),
+        "r"(__float_as_uint(a3)), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)), "f"(0.f));
+}
+// The 8x8 matrix of halves whose row g lane (g, t) holds columns 2t, 2t+1
+// of, transposed.
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ float2 half2_float2(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+constexpr uint32_t kNibble0 = 0x000f000fu;  // z 2^-24 as a subnormal half
+constexpr uint32_t kNibble1 = 0x00f000f0u;  // z 2^-20
+
+// One warp's query operands (row g) and constants.
+struct Int4Query {
+  uint32_t b[16];     // B operands of the 8 key steps
+  float c0[4][2];     // -8 qs_g 2^-24 of rows 2t, 2t+1
+  float qs_hi, qs_lo; // qs_t 2^-24 of row g in two TF32 parts
+  float cr[2];        // score factor of rows 2t, 2t+1 (log2 units)
+};
+
+struct Int4State {
+  float m[2], l[2];  // running max and sum of rows 2t, 2t+1 (this lane's tokens)
+  float o[8][4];     // tile 2j + e: dims 32j + 4g + 2e (rows g), + 1 (rows g+8)
+  float sums[4];     // rows 0-3: sum P s_g, rows 4-7: sum P m_g
+};
+
+template <typename T>
+__device__ __forceinline__ void load_query_int4(const Int4DecodeParams& p, int r, int h, int g,
+                                                int t, Int4Query& iq) {
+  float x[4][8];
+  float big = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[j][i] = 0.f;
+    if (g < p.group) {
+      const T* row = static_cast<const T*>(p.q) + r * p.q_stride_b +
+                     static_cast<int64_t>(h * p.group + g) * p.q_stride_h + 32 * j + 8 * t;
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = *(reinterpret_cast<const uint32_t*>(row) + i);
+      const T* e = reinterpret_cast<const T*>(w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[j][i] = to_float<T>(e[i]);
+        big = fmaxf(big, fabsf(x[j][i]));
+      }
+    }
+  }
+  big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+  big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+  // big = a 2^e with a in [1, 2): scale by 2^(9 - e).  Rows of zeros and
+  // rows with an infinity (whose results are NaN) keep their scale; below
+  // 2^-90 a row's scores are nothing.
+  int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;
+  e = (big == 0.f || e > 127) ? 9 : max(e, -90);
+  const float up = __uint_as_float(static_cast<uint32_t>(127 + 9 - e) << 23);
+  float qs[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[j][i] *= up;
+      sum += x[j][i];
+    }
+    iq.b[4 * j + 0] = pack_half2(x[j][0], x[j][4]);
+    iq.b[4 * j + 1] = pack_half2(x[j][1] * 0.0625f, x[j][5] * 0.0625f);
+    iq.b[4 * j + 2] = pack_half2(x[j][2], x[j][6]);
+    iq.b[4 * j + 3] = pack_half2(x[j][3] * 0.0625f, x[j][7] * 0.0625f);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    qs[j] = sum * 0x1p-24f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      iq.c0[j][i] = -8.f * __shfl_sync(0xffffffffu, qs[j], 4 * (2 * t + i));
+  }
+  const float mine = t == 0 ? qs[0] : t == 1 ? qs[1] : t == 2 ? qs[2] : qs[3];
+  iq.qs_hi = __uint_as_float(__float_as_uint(mine) & 0xffffe000u);
+  iq.qs_lo = mine - iq.qs_hi;
+  // 2^24 undoes the subnormal codes.
+  const float down = p.sm_scale_log2 * 0x1p24f / up;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) iq.cr[i] = __shfl_sync(0xffffffffu, down, 4 * (2 * t + i));
+}
+
+// One page: rec in shared memory, its first `valid` tokens count (MASKED:
+// valid < 16; the other tokens' scales may hold anything).
+template <bool MASKED>
+__device__ __forceinline__ void page_int4(const uint8_t* rec, const Int4Query& iq, Int4State& st,
+                                          int valid, int g, int t) {
+  const int lane = 4 * g + t;
+  // Scores of tokens g (s[0], s[1]: rows 2t, 2t+1) and g + 8 (s[2], s[3]).
+  float s[4];
+  {
+    const __half* mid = reinterpret_cast<const __half*>(rec + kInt4KeyMeta + 8) + t;
+    const float m0 = __half2float(mid[8 * g]), m1 = __half2float(mid[8 * g + 64]);
+    mma_1688_tf32(s, m0, m1, m0, m1, iq.qs_hi, iq.qs_lo);
+  }
+  {
+    const uint4 ka = lds128(rec, 16 * lane), kb = lds128(rec, 512 + 16 * lane);
+    const uint2 sa = *reinterpret_cast<const uint2*>(rec + kInt4KeyMeta + 16 * g);
+    const uint2 sb = *reinterpret_cast<const uint2*>(rec + kInt4KeyMeta + 128 + 16 * g);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t a = j == 0 ? ka.x : j == 1 ? ka.y : j == 2 ? ka.z : ka.w;
+      const uint32_t b = j == 0 ? kb.x : j == 1 ? kb.y : j == 2 ? kb.z : kb.w;
+      float acc[4];
+      mma_16816_c(acc, a & kNibble0, b & kNibble0, a & kNibble1, b & kNibble1, iq.b[4 * j],
+                  iq.b[4 * j + 1], iq.c0[j][0], iq.c0[j][1], iq.c0[j][0], iq.c0[j][1]);
+      mma_16816_acc(acc, (a >> 8) & kNibble0, (b >> 8) & kNibble0, (a >> 8) & kNibble1,
+                    (b >> 8) & kNibble1, iq.b[4 * j + 2], iq.b[4 * j + 3]);
+      const float2 fa = half2_float2(j < 2 ? sa.x : sa.y);
+      const float2 fb = half2_float2(j < 2 ? sb.x : sb.y);
+      const float wa = (j & 1) ? fa.y : fa.x, wb = (j & 1) ? fb.y : fb.x;
+      s[0] = fmaf(wa, acc[0], s[0]);
+      s[1] = fmaf(wa, acc[1], s[1]);
+      s[2] = fmaf(wb, acc[2], s[2]);
+      s[3] = fmaf(wb, acc[3], s[3]);
+    }
+  }
+  const bool in_a = !MASKED || g < valid, in_b = !MASKED || g + 8 < valid;
+  if (MASKED) {
+    if (!in_a) s[0] = s[1] = kNegInf;
+    if (!in_b) s[2] = s[3] = kNegInf;
+  }
+  const float lm0 = fmaxf(s[0], s[2]) * iq.cr[0], lm1 = fmaxf(s[1], s[3]) * iq.cr[1];
+  if (__any_sync(0xffffffffu, lm0 > st.m[0] + kInt4Slack || lm1 > st.m[1] + kInt4Slack)) {
+    const float lm[2] = {warp_max_xor_g(lm0), warp_max_xor_g(lm1)};
+    float a[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float mn = fmaxf(st.m[i], lm[i]);
+      a[i] = mn == kNegInf ? 1.f : fast_exp2(st.m[i] - mn);  // -inf -> 0
+      st.m[i] = mn;
+      st.l[i] *= a[i];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) st.o[j][i] *= a[i & 1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) st.sums[i] *= a[i & 1];
+  }
+  const float ref0 = st.m[0] == kNegInf ? 0.f : st.m[0];
+  const float ref1 = st.m[1] == kNegInf ? 0.f : st.m[1];
+  const float p0 = fast_exp2(fmaf(s[0], iq.cr[0], -ref0));
+  const float p1 = fast_exp2(fmaf(s[1], iq.cr[1], -ref1));
+  const float p2 = fast_exp2(fmaf(s[2], iq.cr[0], -ref0));
+  const float p3 = fast_exp2(fmaf(s[3], iq.cr[1], -ref1));
+  st.l[0] += p0 + p2;
+  st.l[1] += p1 + p3;
+  {
+    // Row 4 + j of the sums: P m_j.
+    const __half* mid = reinterpret_cast<const __half*>(rec + kInt4ValueMeta + 8) + (g & 3);
+    uint32_t a0 = 0, a2 = 0;
+    if (g >= 4) {
+      const unsigned short* m16 = reinterpret_cast<const unsigned short*>(mid);
+      const uint32_t x0 = m16[16 * t], x1 = m16[16 * t + 8];
+      const uint32_t y0 = m16[16 * t + 64], y1 = m16[16 * t + 72];
+      a0 = x0 | (x1 << 16);
+      a2 = y0 | (y1 << 16);
+      if (MASKED) {
+        if (2 * t + 1 >= valid) a0 = 2 * t < valid ? a0 & 0xffffu : 0u;
+        if (2 * t + 9 >= valid) a2 = 2 * t + 8 < valid ? a2 & 0xffffu : 0u;
+      }
+    }
+    mma_16816_acc(st.sums, a0, 0u, a2, 0u, transpose_8x8(pack_half2(p0, p1)),
+                  transpose_8x8(pack_half2(p2, p3)));
+  }
+  const uint2 va = *reinterpret_cast<const uint2*>(rec + kInt4ValueMeta + 16 * g);
+  const uint2 vb = *reinterpret_cast<const uint2*>(rec + kInt4ValueMeta + 128 + 16 * g);
+  // Codes of tokens 2t, 2t+1 and 2t+8, 2t+9.
+  const uint8_t* codes = rec + kInt4Value + 64 * t + 8 * g;
+  const uint2 c00 = *reinterpret_cast<const uint2*>(codes);
+  const uint2 c01 = *reinterpret_cast<const uint2*>(codes + 256);
+  const uint2 c10 = *reinterpret_cast<const uint2*>(codes + 512);
+  const uint2 c11 = *reinterpret_cast<const uint2*>(codes + 768);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 fa = half2_float2(j < 2 ? va.x : va.y);
+    const float2 fb = half2_float2(j < 2 ? vb.x : vb.y);
+    float wa = (j & 1) ? fa.y : fa.x, wb = (j & 1) ? fb.y : fb.x;
+    if (MASKED) {
+      if (!in_a) wa = 0.f;
+      if (!in_b) wb = 0.f;
+    }
+    const uint32_t b0 = transpose_8x8(pack_half2(p0 * wa, p1 * wa));
+    const uint32_t b1 = transpose_8x8(pack_half2(p2 * wb, p3 * wb));
+    const uint32_t one = g == j ? 0x3c003c00u : 0u;
+    mma_16816_acc(st.sums, one, 0u, one, 0u, b0, b1);
+    const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
+    const uint32_t x = j < 2 ? prmt(c00.x, c01.x, sel) : prmt(c00.y, c01.y, sel);
+    const uint32_t y = j < 2 ? prmt(c10.x, c11.x, sel) : prmt(c10.y, c11.y, sel);
+    mma_16816_acc(st.o[2 * j], x & kNibble0, x & kNibble1, y & kNibble0, y & kNibble1, b0, b1);
+    mma_16816_acc(st.o[2 * j + 1], (x >> 8) & kNibble0, (x >> 8) & kNibble1,
+                  (y >> 8) & kNibble0, (y >> 8) & kNibble1, b0, b1);
+  }
+}
 
 // Output row element (v, base-2 lse): the value centre is added where the
 // row attended to anything.
@@ -45,130 +302,212 @@ __device__ __forceinline__ void int4_store_out(const Int4DecodeParams& p, int r,
     p.lse_out[static_cast<int64_t>(r) * (p.hkv * p.group) + qh] = lse;
 }
 
-// One CTA per work item; warps take every fourth page, lane l holds dims
-// 4l .. 4l+3 of every row.
 template <typename T>
-__global__ void __launch_bounds__(kInt4Warps * 32)
+__global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
     pg_decode_int4_kernel(const __grid_constant__ Int4DecodeParams p) {
-  __shared__ float sm_m[kInt4Warps][8], sm_l[kInt4Warps][8], sm_o[kInt4Warps][8][kHeadDim];
+  extern __shared__ __align__(128) uint8_t smem_int4[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  uint8_t* ring = smem_int4 + warp * kInt4RingBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_int4 + kInt4Warps * kInt4RingBytes) +
+                   warp * kInt4Stages;
+  if (lane == 0) {
+    for (int i = 0; i < kInt4Stages; ++i) mbar_init(bars + i, 1);
+    fence_barrier_init();
+  }
+  __syncwarp();
   pdl_launch_dependents();
-  const DecodeItem item = p.items[blockIdx.x];
+  const DecodeItem item = p.items[blockIdx.x];  // plan data
   const int r = item.request, h = item.head_seg & 0xffff;
   const int n_pages = item.count & 0x7fffffff;
+  const int n_w = n_pages > warp ? (n_pages - warp + kInt4Warps - 1) / kInt4Warps : 0;
+  // Pages may be the append's just before: nothing is read ahead of the wait.
   pdl_wait_primary();
+  // Lane u holds the id of the warp's page u (at most 32 per warp).
+  int id = 0;
+  bool bad = false;
+  if (lane < n_w) {
+    id = __ldg(p.indices + item.idx_begin + warp + kInt4Warps * lane);
+    bad = id < 0 || id >= p.num_pages;
+    if (bad) {
+      record_error(p.error_flag, kDevBadPageId);
+      id = 0;
+    }
+  }
+  const uint32_t bad_pages = __ballot_sync(0xffffffffu, bad);
+  const uint64_t policy = l2_evict_first_policy();
+  auto issue = [&](int u) {
+    const int64_t page = __shfl_sync(0xffffffffu, id, u);
+    if (lane == 0) {
+      uint64_t* bar = bars + u % kInt4Stages;
+      mbar_arrive_expect_tx(bar, kInt4Record);
+      bulk_load_hint(ring + (u % kInt4Stages) * kInt4Record,
+                     p.records + (page * p.hkv + h) * kInt4Record, kInt4Record, bar, policy);
+    }
+  };
+  for (int u = 0; u < kInt4Stages && u < n_w; ++u) issue(u);
   int last = kPage;
   if (item.count < 0) {
-    const int lv = p.last_len[r];
+    const int lv = __ldg(p.last_len + r);
     last = lv < 1 ? 1 : (lv > kPage ? kPage : lv);
   }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float q[8][4], o[8][4], m[8], l[8];
+  Int4Query iq;
+  load_query_int4<T>(p, r, h, g, t, iq);
+  Int4State st;
+  st.m[0] = st.m[1] = kNegInf;
+  st.l[0] = st.l[1] = 0.f;
 #pragma unroll
-  for (int g = 0; g < 8; ++g) {
-    m[g] = kNegInf;
-    l[g] = 0.f;
+  for (int j = 0; j < 8; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      o[g][i] = 0.f;
-      q[g][i] = g < p.group ? to_float<T>(static_cast<const T*>(
-                                  p.q)[r * p.q_stride_b + (h * p.group + g) * p.q_stride_h +
-                                       4 * lane + i]) * p.sm_scale_log2
-                            : 0.f;
+    for (int i = 0; i < 4; ++i) st.o[j][i] = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) st.sums[i] = 0.f;
+
+  bool ok = true;
+  int stage = 0;
+  uint32_t phase = 0;
+  for (int u = 0; u < n_w; ++u) {
+    const bool waited = mbar_wait_bounded(bars + stage, phase);
+    if (!__all_sync(0xffffffffu, waited)) {
+      // Let the copies in flight land before the block ends.
+      record_error(p.error_flag, kDevWaitTimeout);
+      const int end = u + kInt4Stages < n_w ? u + kInt4Stages : n_w;
+      for (int v = u; v < end; ++v)
+        mbar_wait_bounded(bars + v % kInt4Stages, static_cast<uint32_t>(v / kInt4Stages) & 1u);
+      ok = false;
+      break;
+    }
+    const uint8_t* rec = ring + stage * kInt4Record;
+    const bool is_last = warp + kInt4Warps * u == n_pages - 1;
+    const int valid = ((bad_pages >> u) & 1u) ? 0 : is_last ? last : kPage;
+    if (valid == kPage)
+      page_int4<false>(rec, iq, st, kPage, g, t);
+    else
+      page_int4<true>(rec, iq, st, valid, g, t);
+    __syncwarp();
+    if (u + kInt4Stages < n_w) issue(u + kInt4Stages);
+    if (++stage == kInt4Stages) {
+      stage = 0;
+      phase ^= 1u;
     }
   }
-  for (int u = warp; u < n_pages; u += kInt4Warps) {
-    int id = p.indices[item.idx_begin + u];
-    if (id < 0 || id >= p.num_pages) {
-      record_error(p.error_flag, kDevBadPageId);
-      continue;
-    }
-    const uint8_t* rec = p.records + (static_cast<int64_t>(id) * p.hkv + h) * kInt4Record;
-    const int valid = u == n_pages - 1 ? last : kPage;
-    for (int t = 0; t < valid; ++t) {
-      const int grp = lane >> 3;
-      const uint32_t kw = *reinterpret_cast<const uint16_t*>(
-          rec + t * 64 + ((lane >> 1) & 3) * 16 + grp * 4 + (lane & 1) * 2);
-      const uint32_t vw = *reinterpret_cast<const uint16_t*>(
-          rec + kInt4Value + value_code_row(t) * 64 + (lane & 7) * 8 + grp * 2);
-      const __half* km = reinterpret_cast<const __half*>(rec + kInt4KeyMeta + t * 16);
-      const __half* vm = reinterpret_cast<const __half*>(rec + kInt4ValueMeta + t * 16);
-      const float ks = __half2float(km[grp]), kmid = __half2float(km[4 + grp]);
-      const float vs = __half2float(vm[grp]), vmid = __half2float(vm[4 + grp]);
-      float k[4], v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        k[i] = fmaf(static_cast<float>(static_cast<int>((kw >> (4 * i)) & 15u) - 8), ks, kmid);
-        v[i] = fmaf(static_cast<float>(static_cast<int>((vw >> (4 * i)) & 15u) - 8), vs, vmid);
-      }
-#pragma unroll
-      for (int g = 0; g < 8; ++g) {
-        if (g >= p.group) break;
-        float s = q[g][0] * k[0] + q[g][1] * k[1] + q[g][2] * k[2] + q[g][3] * k[3];
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        const float mn = fmaxf(m[g], s);
-        const float a = fast_exp2(m[g] - mn), e = fast_exp2(s - mn);
-        m[g] = mn;
-        l[g] = l[g] * a + e;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[g][i] = o[g][i] * a + e * v[i];
-      }
-    }
+
+  // Warp totals: l over the 8 token lanes, then the output rows.
+  const float l0 = warp_sum_xor_g(st.l[0]), l1 = warp_sum_xor_g(st.l[1]);
+  __syncthreads();  // every warp has drained its ring
+  float* cm = reinterpret_cast<float*>(smem_int4);  // [W][8]
+  float* cl = cm + kInt4Warps * 8;                  // [W][8]
+  float* co = cl + kInt4Warps * 8;                  // [W][8][kCoStride]
+  if (g == 0) {
+    cm[warp * 8 + 2 * t] = ok ? st.m[0] : kNegInf;
+    cm[warp * 8 + 2 * t + 1] = ok ? st.m[1] : kNegInf;
+    cl[warp * 8 + 2 * t] = ok ? l0 : 0.f;
+    cl[warp * 8 + 2 * t + 1] = ok ? l1 : 0.f;
   }
 #pragma unroll
-  for (int g = 0; g < 8; ++g) {
-    if (g >= p.group) break;
-    if (lane == 0) {
-      sm_m[warp][g] = m[g];
-      sm_l[warp][g] = l[g];
-    }
+  for (int i = 0; i < 2; ++i) {
+    float* row = co + (warp * 8 + 2 * t + i) * kCoStride;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sm_o[warp][g][4 * lane + i] = o[g][i];
+    for (int j = 0; j < 4; ++j) {
+      const float add = __shfl_sync(0xffffffffu, st.sums[i], 16 + 4 * j + t) -
+                        8.f * __shfl_sync(0xffffffffu, st.sums[i], 4 * j + t);
+      if (2 * t + i < p.group)
+        *reinterpret_cast<float4*>(row + 32 * j + 4 * g) =
+            make_float4(fmaf(st.o[2 * j][i], 0x1p24f, add),
+                        fmaf(st.o[2 * j][2 + i], 0x1p20f, add),
+                        fmaf(st.o[2 * j + 1][i], 0x1p24f, add),
+                        fmaf(st.o[2 * j + 1][2 + i], 0x1p20f, add));
+    }
   }
   __syncthreads();
   for (int idx = threadIdx.x; idx < p.group * kHeadDim; idx += blockDim.x) {
-    const int g = idx >> 7, d = idx & 127;
+    const int q = idx >> 7, d = idx & 127;
     float M = kNegInf, L = 0.f, O = 0.f;
-    for (int w = 0; w < kInt4Warps; ++w) M = fmaxf(M, sm_m[w][g]);
+#pragma unroll
+    for (int w = 0; w < kInt4Warps; ++w) M = fmaxf(M, cm[w * 8 + q]);
+#pragma unroll
     for (int w = 0; w < kInt4Warps; ++w) {
-      const float e = sm_l[w][g] == 0.f ? 0.f : fast_exp2(sm_m[w][g] - M);
-      L += sm_l[w][g] * e;
-      O += sm_o[w][g][d] * e;
+      if (cl[w * 8 + q] == 0.f) continue;
+      const float e = fast_exp2(cm[w * 8 + q] - M);
+      L += cl[w * 8 + q] * e;
+      O += co[(w * 8 + q) * kCoStride + d] * e;
     }
     const float v = L == 0.f ? 0.f : O / L, lse = L == 0.f ? kNegInf : M + fast_log2(L);
     if (p.final_mode) {
-      int4_store_out<T>(p, r, h, g, d, v, lse);
+      int4_store_out<T>(p, r, h, q, d, v, lse);
     } else {
-      const int64_t base = static_cast<int64_t>(blockIdx.x) * p.group + g;
+      const int64_t base = static_cast<int64_t>(blockIdx.x) * p.group + q;
       p.part_o[base * kHeadDim + d] = v;
       if (d == 0) p.part_lse[base] = lse;
     }
   }
 }
 
-// Joins the work items of each (request, query head): one CTA of 128 threads
-// per row, thread = dim.
+// Joins the work items of each (request, query head): one CTA per row, warp w
+// folds partials w, w + 8, ... with four dims per lane and up to eight loads
+// in flight, then the warps' states are combined.
 template <typename T>
-__global__ void __launch_bounds__(kHeadDim)
+__global__ void __launch_bounds__(256)
     pg_int4_merge_kernel(const __grid_constant__ Int4DecodeParams p) {
+  constexpr int W = 8, U = 8;
+  __shared__ float s_m[W], s_l[W];
+  __shared__ float4 s_o[W][32];
   const int hq = p.hkv * p.group;
   const int r = blockIdx.x / hq, qh = blockIdx.x % hq;
-  const int h = qh / p.group, q = qh % p.group, d = threadIdx.x;
+  const int h = qh / p.group, q = qh % p.group;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int begin = p.item_off[r * p.hkv + h], end = p.item_off[r * p.hkv + h + 1];
   pdl_launch_dependents();
   pdl_wait_primary();
-  float M = kNegInf, L = 0.f, O = 0.f;
-  for (int i = begin; i < end; ++i) {
-    const int64_t b = static_cast<int64_t>(i) * p.group + q;
-    const float lse = __ldcg(p.part_lse + b);
-    if (lse == kNegInf) continue;
-    const float mn = fmaxf(M, lse);
-    const float a = fast_exp2(M - mn), e = fast_exp2(lse - mn);
-    M = mn;
-    L = L * a + e;
-    O = O * a + e * __ldcg(p.part_o + b * kHeadDim + d);
+  float m = kNegInf, den = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = begin + warp; i0 < end; i0 += W * U) {
+    float l[U];
+    float4 v[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int i = i0 + W * k;
+      l[k] = kNegInf;
+      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i < end) {
+        const int64_t b = static_cast<int64_t>(i) * p.group + q;
+        l[k] = __ldcg(p.part_lse + b);
+        v[k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + b * kHeadDim) + lane);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      if (l[k] == kNegInf) continue;
+      const float mn = fmaxf(m, l[k]);
+      const float a = fast_exp2(m - mn), e = fast_exp2(l[k] - mn);
+      acc.x = acc.x * a + e * v[k].x;
+      acc.y = acc.y * a + e * v[k].y;
+      acc.z = acc.z * a + e * v[k].z;
+      acc.w = acc.w * a + e * v[k].w;
+      den = den * a + e;
+      m = mn;
+    }
   }
-  int4_store_out<T>(p, r, h, q, d, L == 0.f ? 0.f : O / L, L == 0.f ? kNegInf : M + fast_log2(L));
+  if (lane == 0) {
+    s_m[warp] = m;
+    s_l[warp] = den;
+  }
+  s_o[warp][lane] = acc;
+  __syncthreads();
+  if (threadIdx.x >= kHeadDim) return;
+  const int d = threadIdx.x;
+  float M = kNegInf, L = 0.f, O = 0.f;
+#pragma unroll
+  for (int w = 0; w < W; ++w) M = fmaxf(M, s_m[w]);
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    if (s_l[w] == 0.f) continue;
+    const float e = fast_exp2(s_m[w] - M);
+    L += s_l[w] * e;
+    O += reinterpret_cast<const float*>(s_o[w])[d] * e;
+  }
+  int4_store_out<T>(p, r, h, q, d, L == 0.f ? 0.f : O / L,
+                    L == 0.f ? kNegInf : M + fast_log2(L));
 }
 
 }  // namespace pg
