@@ -54,11 +54,11 @@ struct Int4DecodeParams {
 };
 
 constexpr int kInt4Warps = 4;
-constexpr int kInt4Stages = 5;
-constexpr int kInt4CtasPerSm = 4;
-constexpr int kInt4RingBytes = kInt4Stages * kInt4Record;
+constexpr int kInt4Slots = 3;  // pairs of pages in a warp's ring
+constexpr int kInt4CtasPerSm = 3;
+constexpr int kInt4RingBytes = kInt4Slots * 2 * kInt4Record;
 // The warps' rings, then their barriers; the epilogue reuses the rings.
-constexpr int kInt4SmemBytes = kInt4Warps * (kInt4RingBytes + kInt4Stages * 8);
+constexpr int kInt4SmemBytes = kInt4Warps * (kInt4RingBytes + kInt4Slots * 8);
 static_assert(kInt4Warps * (16 + 8 * kCoStride) * 4 <= kInt4Warps * kInt4RingBytes,
               "the combine buffer lies in the rings");
 // The running maximum is raised when a score passes it by this (log2).
@@ -111,6 +111,7 @@ struct Int4Query {
 
 struct Int4State {
   float m[2], l[2];  // running max and sum of rows 2t, 2t+1 (this lane's tokens)
+  float ref[2];      // m, or 0 while m is -inf
   float o[8][4];     // tile 2j + e: dims 32j + 4g + 2e (rows g), + 1 (rows g+8)
   float sums[4];     // rows 0-3: sum P s_g, rows 4-7: sum P m_g
 };
@@ -175,23 +176,24 @@ __device__ __forceinline__ void load_query_int4(const Int4DecodeParams& p, int r
   for (int i = 0; i < 2; ++i) iq.cr[i] = __shfl_sync(0xffffffffu, down, 4 * (2 * t + i));
 }
 
-// One page: rec in shared memory, its first `valid` tokens count (MASKED:
-// valid < 16; the other tokens' scales may hold anything).
-template <bool MASKED>
-__device__ __forceinline__ void page_int4(const uint8_t* rec, const Int4Query& iq, Int4State& st,
-                                          int valid, int g, int t) {
+// Two pages at rec and rec + kInt4Record in shared memory, of which the first
+// valid[i] tokens count (the others' scales may hold anything).
+__device__ __forceinline__ void pages_int4(const uint8_t* rec, const Int4Query& iq, Int4State& st,
+                                           const int* valid, int g, int t) {
   const int lane = 4 * g + t;
-  // Scores of tokens g (s[0], s[1]: rows 2t, 2t+1) and g + 8 (s[2], s[3]).
-  float s[4];
-  {
-    const __half* mid = reinterpret_cast<const __half*>(rec + kInt4KeyMeta + 8) + t;
-    const float m0 = __half2float(mid[8 * g]), m1 = __half2float(mid[8 * g + 64]);
-    mma_1688_tf32(s, m0, m1, m0, m1, iq.qs_hi, iq.qs_lo);
-  }
-  {
-    const uint4 ka = lds128(rec, 16 * lane), kb = lds128(rec, 512 + 16 * lane);
-    const uint2 sa = *reinterpret_cast<const uint2*>(rec + kInt4KeyMeta + 16 * g);
-    const uint2 sb = *reinterpret_cast<const uint2*>(rec + kInt4KeyMeta + 128 + 16 * g);
+  // Scores of tokens g (s[i][0], s[i][1]: rows 2t, 2t+1) and g + 8.
+  float s[2][4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint8_t* page = rec + i * kInt4Record;
+    {
+      const __half* mid = reinterpret_cast<const __half*>(page + kInt4KeyMeta + 8) + t;
+      const float m0 = __half2float(mid[8 * g]), m1 = __half2float(mid[8 * g + 64]);
+      mma_1688_tf32(s[i], m0, m1, m0, m1, iq.qs_hi, iq.qs_lo);
+    }
+    const uint4 ka = lds128(page, 16 * lane), kb = lds128(page, 512 + 16 * lane);
+    const uint2 sa = *reinterpret_cast<const uint2*>(page + kInt4KeyMeta + 16 * g);
+    const uint2 sb = *reinterpret_cast<const uint2*>(page + kInt4KeyMeta + 128 + 16 * g);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint32_t a = j == 0 ? ka.x : j == 1 ? ka.y : j == 2 ? ka.z : ka.w;
@@ -204,18 +206,22 @@ __device__ __forceinline__ void page_int4(const uint8_t* rec, const Int4Query& i
       const float2 fa = half2_float2(j < 2 ? sa.x : sa.y);
       const float2 fb = half2_float2(j < 2 ? sb.x : sb.y);
       const float wa = (j & 1) ? fa.y : fa.x, wb = (j & 1) ? fb.y : fb.x;
-      s[0] = fmaf(wa, acc[0], s[0]);
-      s[1] = fmaf(wa, acc[1], s[1]);
-      s[2] = fmaf(wb, acc[2], s[2]);
-      s[3] = fmaf(wb, acc[3], s[3]);
+      s[i][0] = fmaf(wa, acc[0], s[i][0]);
+      s[i][1] = fmaf(wa, acc[1], s[i][1]);
+      s[i][2] = fmaf(wb, acc[2], s[i][2]);
+      s[i][3] = fmaf(wb, acc[3], s[i][3]);
     }
   }
-  const bool in_a = !MASKED || g < valid, in_b = !MASKED || g + 8 < valid;
-  if (MASKED) {
-    if (!in_a) s[0] = s[1] = kNegInf;
-    if (!in_b) s[2] = s[3] = kNegInf;
+  const bool masked = valid[0] + valid[1] != 2 * kPage;
+  if (masked) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (g >= valid[i]) s[i][0] = s[i][1] = kNegInf;
+      if (g + 8 >= valid[i]) s[i][2] = s[i][3] = kNegInf;
+    }
   }
-  const float lm0 = fmaxf(s[0], s[2]) * iq.cr[0], lm1 = fmaxf(s[1], s[3]) * iq.cr[1];
+  const float lm0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2])) * iq.cr[0];
+  const float lm1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3])) * iq.cr[1];
   if (__any_sync(0xffffffffu, lm0 > st.m[0] + kInt4Slack || lm1 > st.m[1] + kInt4Slack)) {
     const float lm[2] = {warp_max_xor_g(lm0), warp_max_xor_g(lm1)};
     float a[2];
@@ -224,6 +230,7 @@ __device__ __forceinline__ void page_int4(const uint8_t* rec, const Int4Query& i
       const float mn = fmaxf(st.m[i], lm[i]);
       a[i] = mn == kNegInf ? 1.f : fast_exp2(st.m[i] - mn);  // -inf -> 0
       st.m[i] = mn;
+      st.ref[i] = mn == kNegInf ? 0.f : mn;
       st.l[i] *= a[i];
     }
 #pragma unroll
@@ -233,59 +240,54 @@ __device__ __forceinline__ void page_int4(const uint8_t* rec, const Int4Query& i
 #pragma unroll
     for (int i = 0; i < 4; ++i) st.sums[i] *= a[i & 1];
   }
-  const float ref0 = st.m[0] == kNegInf ? 0.f : st.m[0];
-  const float ref1 = st.m[1] == kNegInf ? 0.f : st.m[1];
-  const float p0 = fast_exp2(fmaf(s[0], iq.cr[0], -ref0));
-  const float p1 = fast_exp2(fmaf(s[1], iq.cr[1], -ref1));
-  const float p2 = fast_exp2(fmaf(s[2], iq.cr[0], -ref0));
-  const float p3 = fast_exp2(fmaf(s[3], iq.cr[1], -ref1));
-  st.l[0] += p0 + p2;
-  st.l[1] += p1 + p3;
-  {
-    // Row 4 + j of the sums: P m_j.
-    const __half* mid = reinterpret_cast<const __half*>(rec + kInt4ValueMeta + 8) + (g & 3);
-    uint32_t a0 = 0, a2 = 0;
-    if (g >= 4) {
-      const unsigned short* m16 = reinterpret_cast<const unsigned short*>(mid);
-      const uint32_t x0 = m16[16 * t], x1 = m16[16 * t + 8];
-      const uint32_t y0 = m16[16 * t + 64], y1 = m16[16 * t + 72];
-      a0 = x0 | (x1 << 16);
-      a2 = y0 | (y1 << 16);
-      if (MASKED) {
-        if (2 * t + 1 >= valid) a0 = 2 * t < valid ? a0 & 0xffffu : 0u;
-        if (2 * t + 9 >= valid) a2 = 2 * t + 8 < valid ? a2 & 0xffffu : 0u;
-      }
-    }
-    mma_16816_acc(st.sums, a0, 0u, a2, 0u, transpose_8x8(pack_half2(p0, p1)),
-                  transpose_8x8(pack_half2(p2, p3)));
-  }
-  const uint2 va = *reinterpret_cast<const uint2*>(rec + kInt4ValueMeta + 16 * g);
-  const uint2 vb = *reinterpret_cast<const uint2*>(rec + kInt4ValueMeta + 128 + 16 * g);
-  // Codes of tokens 2t, 2t+1 and 2t+8, 2t+9.
-  const uint8_t* codes = rec + kInt4Value + 64 * t + 8 * g;
-  const uint2 c00 = *reinterpret_cast<const uint2*>(codes);
-  const uint2 c01 = *reinterpret_cast<const uint2*>(codes + 256);
-  const uint2 c10 = *reinterpret_cast<const uint2*>(codes + 512);
-  const uint2 c11 = *reinterpret_cast<const uint2*>(codes + 768);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 fa = half2_float2(j < 2 ? va.x : va.y);
-    const float2 fb = half2_float2(j < 2 ? vb.x : vb.y);
-    float wa = (j & 1) ? fa.y : fa.x, wb = (j & 1) ? fb.y : fb.x;
-    if (MASKED) {
-      if (!in_a) wa = 0.f;
-      if (!in_b) wb = 0.f;
+  for (int i = 0; i < 2; ++i) {
+    const uint8_t* page = rec + i * kInt4Record;
+    const float p0 = fast_exp2(fmaf(s[i][0], iq.cr[0], -st.ref[0]));
+    const float p1 = fast_exp2(fmaf(s[i][1], iq.cr[1], -st.ref[1]));
+    const float p2 = fast_exp2(fmaf(s[i][2], iq.cr[0], -st.ref[0]));
+    const float p3 = fast_exp2(fmaf(s[i][3], iq.cr[1], -st.ref[1]));
+    st.l[0] += p0 + p2;
+    st.l[1] += p1 + p3;
+    // Rows 4 + j of the sums: P m_j of tokens 2t, 2t+1 and 2t+8, 2t+9.
+    const unsigned short* mid =
+        reinterpret_cast<const unsigned short*>(page + kInt4ValueMeta + 8) + (g & 3) + 16 * t;
+    uint32_t ma = mid[0] | (static_cast<uint32_t>(mid[8]) << 16);
+    uint32_t mb = mid[64] | (static_cast<uint32_t>(mid[72]) << 16);
+    if (g < 4) ma = mb = 0u;
+    uint2 va = *reinterpret_cast<const uint2*>(page + kInt4ValueMeta + 16 * g);
+    uint2 vb = *reinterpret_cast<const uint2*>(page + kInt4ValueMeta + 128 + 16 * g);
+    if (masked) {
+      const int n = valid[i];
+      if (2 * t + 1 >= n) ma = 2 * t < n ? ma & 0xffffu : 0u;
+      if (2 * t + 9 >= n) mb = 2 * t + 8 < n ? mb & 0xffffu : 0u;
+      if (g >= n) va = make_uint2(0u, 0u);
+      if (g + 8 >= n) vb = make_uint2(0u, 0u);
     }
-    const uint32_t b0 = transpose_8x8(pack_half2(p0 * wa, p1 * wa));
-    const uint32_t b1 = transpose_8x8(pack_half2(p2 * wb, p3 * wb));
-    const uint32_t one = g == j ? 0x3c003c00u : 0u;
-    mma_16816_acc(st.sums, one, 0u, one, 0u, b0, b1);
-    const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
-    const uint32_t x = j < 2 ? prmt(c00.x, c01.x, sel) : prmt(c00.y, c01.y, sel);
-    const uint32_t y = j < 2 ? prmt(c10.x, c11.x, sel) : prmt(c10.y, c11.y, sel);
-    mma_16816_acc(st.o[2 * j], x & kNibble0, x & kNibble1, y & kNibble0, y & kNibble1, b0, b1);
-    mma_16816_acc(st.o[2 * j + 1], (x >> 8) & kNibble0, (x >> 8) & kNibble1,
-                  (y >> 8) & kNibble0, (y >> 8) & kNibble1, b0, b1);
+    mma_16816_acc(st.sums, ma, 0u, mb, 0u, transpose_8x8(pack_half2(p0, p1)),
+                  transpose_8x8(pack_half2(p2, p3)));
+    // Codes of tokens 2t, 2t+1 and 2t+8, 2t+9.
+    const uint8_t* codes = page + kInt4Value + 64 * t + 8 * g;
+    const uint2 c00 = *reinterpret_cast<const uint2*>(codes);
+    const uint2 c01 = *reinterpret_cast<const uint2*>(codes + 256);
+    const uint2 c10 = *reinterpret_cast<const uint2*>(codes + 512);
+    const uint2 c11 = *reinterpret_cast<const uint2*>(codes + 768);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 fa = half2_float2(j < 2 ? va.x : va.y);
+      const float2 fb = half2_float2(j < 2 ? vb.x : vb.y);
+      const float wa = (j & 1) ? fa.y : fa.x, wb = (j & 1) ? fb.y : fb.x;
+      const uint32_t b0 = transpose_8x8(pack_half2(p0 * wa, p1 * wa));
+      const uint32_t b1 = transpose_8x8(pack_half2(p2 * wb, p3 * wb));
+      const uint32_t one = g == j ? 0x3c003c00u : 0u;
+      mma_16816_acc(st.sums, one, 0u, one, 0u, b0, b1);
+      const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
+      const uint32_t x = j < 2 ? prmt(c00.x, c01.x, sel) : prmt(c00.y, c01.y, sel);
+      const uint32_t y = j < 2 ? prmt(c10.x, c11.x, sel) : prmt(c10.y, c11.y, sel);
+      mma_16816_acc(st.o[2 * j], x & kNibble0, x & kNibble1, y & kNibble0, y & kNibble1, b0, b1);
+      mma_16816_acc(st.o[2 * j + 1], (x >> 8) & kNibble0, (x >> 8) & kNibble1,
+                    (y >> 8) & kNibble0, (y >> 8) & kNibble1, b0, b1);
+    }
   }
 }
 
@@ -310,9 +312,9 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
   const int g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem_int4 + warp * kInt4RingBytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem_int4 + kInt4Warps * kInt4RingBytes) +
-                   warp * kInt4Stages;
+                   warp * kInt4Slots;
   if (lane == 0) {
-    for (int i = 0; i < kInt4Stages; ++i) mbar_init(bars + i, 1);
+    for (int i = 0; i < kInt4Slots; ++i) mbar_init(bars + i, 1);
     fence_barrier_init();
   }
   __syncwarp();
@@ -321,31 +323,35 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
   const int r = item.request, h = item.head_seg & 0xffff;
   const int n_pages = item.count & 0x7fffffff;
   const int n_w = n_pages > warp ? (n_pages - warp + kInt4Warps - 1) / kInt4Warps : 0;
+  const int n_pairs = (n_w + 1) >> 1;
   // Pages may be the append's just before: nothing is read ahead of the wait.
   pdl_wait_primary();
-  // Lane u holds the id of the warp's page u (at most 32 per warp).
-  int id = 0;
+  // Lane u holds the record of the warp's page u (at most 32 per warp) and
+  // copies it itself.
+  const uint8_t* mine = nullptr;
   bool bad = false;
   if (lane < n_w) {
-    id = __ldg(p.indices + item.idx_begin + warp + kInt4Warps * lane);
+    int id = __ldg(p.indices + item.idx_begin + warp + kInt4Warps * lane);
     bad = id < 0 || id >= p.num_pages;
     if (bad) {
       record_error(p.error_flag, kDevBadPageId);
       id = 0;
     }
+    mine = p.records + (static_cast<int64_t>(id) * p.hkv + h) * kInt4Record;
   }
   const uint32_t bad_pages = __ballot_sync(0xffffffffu, bad);
   const uint64_t policy = l2_evict_first_policy();
-  auto issue = [&](int u) {
-    const int64_t page = __shfl_sync(0xffffffffu, id, u);
-    if (lane == 0) {
-      uint64_t* bar = bars + u % kInt4Stages;
-      mbar_arrive_expect_tx(bar, kInt4Record);
-      bulk_load_hint(ring + (u % kInt4Stages) * kInt4Record,
-                     p.records + (page * p.hkv + h) * kInt4Record, kInt4Record, bar, policy);
-    }
+  // Pair u's copies into slot `slot`: its first lane announces the bytes.
+  auto issue = [&](int u, int slot) {
+    const int first = 2 * u;
+    if (lane == first)
+      mbar_arrive_expect_tx(bars + slot, first + 1 < n_w ? 2 * kInt4Record : kInt4Record);
+    __syncwarp();
+    if ((lane >> 1) == u && mine != nullptr)
+      bulk_load_hint(ring + (2 * slot + (lane & 1)) * kInt4Record, mine, kInt4Record, bars + slot,
+                     policy);
   };
-  for (int u = 0; u < kInt4Stages && u < n_w; ++u) issue(u);
+  for (int u = 0; u < kInt4Slots && u < n_pairs; ++u) issue(u, u);
   int last = kPage;
   if (item.count < 0) {
     const int lv = __ldg(p.last_len + r);
@@ -356,38 +362,45 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
   Int4State st;
   st.m[0] = st.m[1] = kNegInf;
   st.l[0] = st.l[1] = 0.f;
+  st.ref[0] = st.ref[1] = 0.f;
 #pragma unroll
   for (int j = 0; j < 8; ++j)
 #pragma unroll
     for (int i = 0; i < 4; ++i) st.o[j][i] = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) st.sums[i] = 0.f;
+  // Tokens that count in the warp's last page, if it is the request's last.
+  const int tail = n_w > 0 && warp + kInt4Warps * (n_w - 1) == n_pages - 1 ? last : kPage;
 
   bool ok = true;
-  int stage = 0;
+  int slot = 0;
   uint32_t phase = 0;
-  for (int u = 0; u < n_w; ++u) {
-    const bool waited = mbar_wait_bounded(bars + stage, phase);
+  for (int u = 0; u < n_pairs; ++u) {
+    const bool waited = mbar_wait_bounded(bars + slot, phase);
     if (!__all_sync(0xffffffffu, waited)) {
       // Let the copies in flight land before the block ends.
       record_error(p.error_flag, kDevWaitTimeout);
-      const int end = u + kInt4Stages < n_w ? u + kInt4Stages : n_w;
+      const int end = u + kInt4Slots < n_pairs ? u + kInt4Slots : n_pairs;
       for (int v = u; v < end; ++v)
-        mbar_wait_bounded(bars + v % kInt4Stages, static_cast<uint32_t>(v / kInt4Stages) & 1u);
+        mbar_wait_bounded(bars + v % kInt4Slots, static_cast<uint32_t>(v / kInt4Slots) & 1u);
       ok = false;
       break;
     }
-    const uint8_t* rec = ring + stage * kInt4Record;
-    const bool is_last = warp + kInt4Warps * u == n_pages - 1;
-    const int valid = ((bad_pages >> u) & 1u) ? 0 : is_last ? last : kPage;
-    if (valid == kPage)
-      page_int4<false>(rec, iq, st, kPage, g, t);
-    else
-      page_int4<true>(rec, iq, st, valid, g, t);
+    int valid[2] = {kPage, kPage};
+    if (u == n_pairs - 1) {
+      const bool two = (n_w & 1) == 0;
+      valid[0] = two ? kPage : tail;
+      valid[1] = two ? tail : 0;
+    }
+    if (bad_pages != 0u) {
+      if ((bad_pages >> (2 * u)) & 1u) valid[0] = 0;
+      if ((bad_pages >> (2 * u)) & 2u) valid[1] = 0;
+    }
+    pages_int4(ring + 2 * slot * kInt4Record, iq, st, valid, g, t);
     __syncwarp();
-    if (u + kInt4Stages < n_w) issue(u + kInt4Stages);
-    if (++stage == kInt4Stages) {
-      stage = 0;
+    if (u + kInt4Slots < n_pairs) issue(u + kInt4Slots, slot);
+    if (++slot == kInt4Slots) {
+      slot = 0;
       phase ^= 1u;
     }
   }
