@@ -174,15 +174,16 @@ int32_t ensure_int4_smem() {
     return fail(PG_ERR_CUDA, "cudaGetDevice failed");
   std::lock_guard<std::mutex> lock(mu);
   if (done[dev]) return PG_OK;
-  int32_t rc = cuda_check(cudaFuncSetAttribute(pg::pg_decode_int4_kernel<__half>,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               pg::kInt4SmemBytes),
-                          "cudaFuncSetAttribute(int4 decode smem)");
-  if (rc != PG_OK) return rc;
-  rc = cuda_check(cudaFuncSetAttribute(pg::pg_decode_int4_kernel<__nv_bfloat16>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       pg::kInt4SmemBytes),
-                  "cudaFuncSetAttribute(int4 decode smem)");
+  using Kernel = void (*)(pg::Int4DecodeParams);
+  const Kernel kernels[4] = {pg::pg_decode_int4_kernel<__half, true>,
+                             pg::pg_decode_int4_kernel<__half, false>,
+                             pg::pg_decode_int4_kernel<__nv_bfloat16, true>,
+                             pg::pg_decode_int4_kernel<__nv_bfloat16, false>};
+  int32_t rc = PG_OK;
+  for (int i = 0; i < 4 && rc == PG_OK; ++i)
+    rc = cuda_check(cudaFuncSetAttribute(kernels[i], cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         pg::kInt4SmemBytes),
+                    "cudaFuncSetAttribute(int4 decode smem)");
   if (rc == PG_OK) done[dev] = true;
   return rc;
 }
@@ -1294,8 +1295,11 @@ int32_t pg_decode_int4_run(const pg_int4_decode_args* a, void* stream) {
   if (a->num_items > 0) {
     int32_t rc = ensure_int4_smem();
     if (rc != PG_OK) return rc;
-    rc = launch_pdl(half ? pg::pg_decode_int4_kernel<__half>
-                         : pg::pg_decode_int4_kernel<__nv_bfloat16>,
+    const bool narrow = a->group <= 4;
+    rc = launch_pdl(half ? (narrow ? pg::pg_decode_int4_kernel<__half, true>
+                                   : pg::pg_decode_int4_kernel<__half, false>)
+                         : (narrow ? pg::pg_decode_int4_kernel<__nv_bfloat16, true>
+                                   : pg::pg_decode_int4_kernel<__nv_bfloat16, false>),
                     dim3(a->num_items), dim3(pg::kInt4Warps * 32), pg::kInt4SmemBytes, st,
                     "int4 decode launch", p);
     if (rc != PG_OK || final_mode) return rc;

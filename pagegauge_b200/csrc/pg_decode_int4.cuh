@@ -54,7 +54,7 @@ struct Int4DecodeParams {
 };
 
 constexpr int kInt4Warps = 4;
-constexpr int kInt4Slots = 3;  // pairs of pages in a warp's ring
+constexpr int kInt4Slots = 2;  // pairs of pages in a warp's ring
 constexpr int kInt4CtasPerSm = 3;
 constexpr int kInt4RingBytes = kInt4Slots * 2 * kInt4Record;
 // The warps' rings, then their barriers; the epilogue reuses the rings.
@@ -100,6 +100,7 @@ __device__ __forceinline__ float2 half2_float2(uint32_t w) {
 
 constexpr uint32_t kNibble0 = 0x000f000fu;  // z 2^-24 as a subnormal half
 constexpr uint32_t kNibble1 = 0x00f000f0u;  // z 2^-20
+constexpr uint32_t kNibbles = 0x00ff00ffu;  // (z0 + 16 z1) 2^-24
 
 // One warp's query operands (row g) and constants.
 struct Int4Query {
@@ -112,11 +113,18 @@ struct Int4Query {
 struct Int4State {
   float m[2], l[2];  // running max and sum of rows 2t, 2t+1 (this lane's tokens)
   float ref[2];      // m, or 0 while m is -inf
-  float o[8][4];     // tile 2j + e: dims 32j + 4g + 2e (rows g), + 1 (rows g+8)
-  float sums[4];     // rows 0-3: sum P s_g, rows 4-7: sum P m_g
+  // Tile 2j + e, rows g: dims d = 32j + 4g + 2e; rows g + 8: d and d + 1 as
+  // z_d + 16 z_(d+1) (one AND less than the two nibbles apart).
+  float o[8][4];
+  float sums[4];  // sum P s_g (rows 0-3, NARROW: 0-1), sum P m_g (rows 4-7)
 };
 
-template <typename T>
+// NARROW (GQA group <= 4): columns 4-7 of the products repeat the query rows
+// 0-3, so that one B operand of the value products holds two dim groups'
+// weights (columns 0-3 with group 2i's scale, 4-7 with group 2i + 1's): half
+// the multiplies, conversions and transposes, and each value product still
+// reads its own columns.
+template <typename T, bool NARROW>
 __device__ __forceinline__ void load_query_int4(const Int4DecodeParams& p, int r, int h, int g,
                                                 int t, Int4Query& iq) {
   float x[4][8];
@@ -125,9 +133,10 @@ __device__ __forceinline__ void load_query_int4(const Int4DecodeParams& p, int r
   for (int j = 0; j < 4; ++j) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[j][i] = 0.f;
-    if (g < p.group) {
+    const int q = NARROW ? g & 3 : g;
+    if (q < p.group) {
       const T* row = static_cast<const T*>(p.q) + r * p.q_stride_b +
-                     static_cast<int64_t>(h * p.group + g) * p.q_stride_h + 32 * j + 8 * t;
+                     static_cast<int64_t>(h * p.group + q) * p.q_stride_h + 32 * j + 8 * t;
       uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = *(reinterpret_cast<const uint32_t*>(row) + i);
@@ -178,6 +187,7 @@ __device__ __forceinline__ void load_query_int4(const Int4DecodeParams& p, int r
 
 // Two pages at rec and rec + kInt4Record in shared memory, of which the first
 // valid[i] tokens count (the others' scales may hold anything).
+template <bool NARROW>
 __device__ __forceinline__ void pages_int4(const uint8_t* rec, const Int4Query& iq, Int4State& st,
                                            const int* valid, int g, int t) {
   const int lane = 4 * g + t;
@@ -255,14 +265,34 @@ __device__ __forceinline__ void pages_int4(const uint8_t* rec, const Int4Query& 
     uint32_t ma = mid[0] | (static_cast<uint32_t>(mid[8]) << 16);
     uint32_t mb = mid[64] | (static_cast<uint32_t>(mid[72]) << 16);
     if (g < 4) ma = mb = 0u;
-    uint2 va = *reinterpret_cast<const uint2*>(page + kInt4ValueMeta + 16 * g);
-    uint2 vb = *reinterpret_cast<const uint2*>(page + kInt4ValueMeta + 128 + 16 * g);
+    // Value scales of tokens g and g + 8, four groups or (NARROW) the two of
+    // this lane's columns.
+    constexpr int kParts = NARROW ? 2 : 4;
+    float wa[kParts], wb[kParts];
+    if constexpr (NARROW) {
+      const __half* sa = reinterpret_cast<const __half*>(page + kInt4ValueMeta + 16 * g) + (t >> 1);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        wa[k] = __half2float(sa[2 * k]);
+        wb[k] = __half2float(sa[64 + 2 * k]);
+      }
+    } else {
+      const uint2 va = *reinterpret_cast<const uint2*>(page + kInt4ValueMeta + 16 * g);
+      const uint2 vb = *reinterpret_cast<const uint2*>(page + kInt4ValueMeta + 128 + 16 * g);
+      const float2 a0 = half2_float2(va.x), a1 = half2_float2(va.y);
+      const float2 b0 = half2_float2(vb.x), b1 = half2_float2(vb.y);
+      wa[0] = a0.x; wa[1] = a0.y; wa[kParts - 2] = a1.x; wa[kParts - 1] = a1.y;
+      wb[0] = b0.x; wb[1] = b0.y; wb[kParts - 2] = b1.x; wb[kParts - 1] = b1.y;
+    }
     if (masked) {
       const int n = valid[i];
       if (2 * t + 1 >= n) ma = 2 * t < n ? ma & 0xffffu : 0u;
       if (2 * t + 9 >= n) mb = 2 * t + 8 < n ? mb & 0xffffu : 0u;
-      if (g >= n) va = make_uint2(0u, 0u);
-      if (g + 8 >= n) vb = make_uint2(0u, 0u);
+#pragma unroll
+      for (int k = 0; k < kParts; ++k) {
+        if (g >= n) wa[k] = 0.f;
+        if (g + 8 >= n) wb[k] = 0.f;
+      }
     }
     mma_16816_acc(st.sums, ma, 0u, mb, 0u, transpose_8x8(pack_half2(p0, p1)),
                   transpose_8x8(pack_half2(p2, p3)));
@@ -273,20 +303,22 @@ __device__ __forceinline__ void pages_int4(const uint8_t* rec, const Int4Query& 
     const uint2 c10 = *reinterpret_cast<const uint2*>(codes + 512);
     const uint2 c11 = *reinterpret_cast<const uint2*>(codes + 768);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 fa = half2_float2(j < 2 ? va.x : va.y);
-      const float2 fb = half2_float2(j < 2 ? vb.x : vb.y);
-      const float wa = (j & 1) ? fa.y : fa.x, wb = (j & 1) ? fb.y : fb.x;
-      const uint32_t b0 = transpose_8x8(pack_half2(p0 * wa, p1 * wa));
-      const uint32_t b1 = transpose_8x8(pack_half2(p2 * wb, p3 * wb));
-      const uint32_t one = g == j ? 0x3c003c00u : 0u;
+    for (int k = 0; k < kParts; ++k) {
+      const uint32_t b0 = transpose_8x8(pack_half2(p0 * wa[k], p1 * wa[k]));
+      const uint32_t b1 = transpose_8x8(pack_half2(p2 * wb[k], p3 * wb[k]));
+      const uint32_t one = g == k ? 0x3c003c00u : 0u;
       mma_16816_acc(st.sums, one, 0u, one, 0u, b0, b1);
-      const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
-      const uint32_t x = j < 2 ? prmt(c00.x, c01.x, sel) : prmt(c00.y, c01.y, sel);
-      const uint32_t y = j < 2 ? prmt(c10.x, c11.x, sel) : prmt(c10.y, c11.y, sel);
-      mma_16816_acc(st.o[2 * j], x & kNibble0, x & kNibble1, y & kNibble0, y & kNibble1, b0, b1);
-      mma_16816_acc(st.o[2 * j + 1], (x >> 8) & kNibble0, (x >> 8) & kNibble1,
-                    (y >> 8) & kNibble0, (y >> 8) & kNibble1, b0, b1);
+#pragma unroll
+      for (int e = 0; e < 4 / kParts; ++e) {
+        const int j = k * (4 / kParts) + e;
+        const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
+        const uint32_t x = j < 2 ? prmt(c00.x, c01.x, sel) : prmt(c00.y, c01.y, sel);
+        const uint32_t y = j < 2 ? prmt(c10.x, c11.x, sel) : prmt(c10.y, c11.y, sel);
+        mma_16816_acc(st.o[2 * j], x & kNibble0, x & kNibbles, y & kNibble0, y & kNibbles, b0,
+                      b1);
+        const uint32_t xh = prmt(x, 0u, 0x4341u), yh = prmt(y, 0u, 0x4341u);
+        mma_16816_acc(st.o[2 * j + 1], xh & kNibble0, xh, yh & kNibble0, yh, b0, b1);
+      }
     }
   }
 }
@@ -304,7 +336,7 @@ __device__ __forceinline__ void int4_store_out(const Int4DecodeParams& p, int r,
     p.lse_out[static_cast<int64_t>(r) * (p.hkv * p.group) + qh] = lse;
 }
 
-template <typename T>
+template <typename T, bool NARROW>
 __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
     pg_decode_int4_kernel(const __grid_constant__ Int4DecodeParams p) {
   extern __shared__ __align__(128) uint8_t smem_int4[];
@@ -358,7 +390,7 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
     last = lv < 1 ? 1 : (lv > kPage ? kPage : lv);
   }
   Int4Query iq;
-  load_query_int4<T>(p, r, h, g, t, iq);
+  load_query_int4<T, NARROW>(p, r, h, g, t, iq);
   Int4State st;
   st.m[0] = st.m[1] = kNegInf;
   st.l[0] = st.l[1] = 0.f;
@@ -396,7 +428,7 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
       if ((bad_pages >> (2 * u)) & 1u) valid[0] = 0;
       if ((bad_pages >> (2 * u)) & 2u) valid[1] = 0;
     }
-    pages_int4(ring + 2 * slot * kInt4Record, iq, st, valid, g, t);
+    pages_int4<NARROW>(ring + 2 * slot * kInt4Record, iq, st, valid, g, t);
     __syncwarp();
     if (u + kInt4Slots < n_pairs) issue(u + kInt4Slots, slot);
     if (++slot == kInt4Slots) {
@@ -419,17 +451,20 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    float* row = co + (warp * 8 + 2 * t + i) * kCoStride;
+    // The row of this lane's column, and its sums (shuffled by every lane).
+    const int q = NARROW ? (2 * t + i) & 3 : 2 * t + i;
+    float* row = co + (warp * 8 + q) * kCoStride;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float add = __shfl_sync(0xffffffffu, st.sums[i], 16 + 4 * j + t) -
-                        8.f * __shfl_sync(0xffffffffu, st.sums[i], 4 * j + t);
-      if (2 * t + i < p.group)
+                        8.f * __shfl_sync(0xffffffffu, st.sums[i], 4 * (NARROW ? j >> 1 : j) + t);
+      if (q < p.group && (!NARROW || (t >> 1) == (j & 1))) {
+        const float* a = st.o[2 * j];
+        const float* b = st.o[2 * j + 1];
         *reinterpret_cast<float4*>(row + 32 * j + 4 * g) =
-            make_float4(fmaf(st.o[2 * j][i], 0x1p24f, add),
-                        fmaf(st.o[2 * j][2 + i], 0x1p20f, add),
-                        fmaf(st.o[2 * j + 1][i], 0x1p24f, add),
-                        fmaf(st.o[2 * j + 1][2 + i], 0x1p20f, add));
+            make_float4(fmaf(a[i], 0x1p24f, add), fmaf(a[2 + i] - a[i], 0x1p20f, add),
+                        fmaf(b[i], 0x1p24f, add), fmaf(b[2 + i] - b[i], 0x1p20f, add));
+      }
     }
   }
   __syncthreads();
