@@ -8,7 +8,10 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
+
+import torch
 
 LIB_NAME = "libpagegauge_b200.so"
 LIB_PATH = Path(__file__).resolve().parent / LIB_NAME
@@ -161,10 +164,10 @@ _SIGNATURES = {
                                          ctypes.POINTER(c_i64), c_i32p]),
     "pg_skinny_gemm": (c_i32, [ctypes.POINTER(PgGemmArgs), c_vp]),
     "pg_quantize_pages": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_i32, c_i32, c_vp]),
-    "pg_rotary": (c_i32, [ctypes.POINTER(PgRotaryArgs), c_vp]),
-    "pg_rope_append_int4": (c_i32, [ctypes.POINTER(PgInt4AppendArgs), c_vp]),
+    "pg_rotary": (c_i32, [c_vp, c_vp]),
+    "pg_rope_append_int4": (c_i32, [c_vp, c_vp]),
     "pg_int4_read": (c_i32, [c_vp, c_i64, c_i32, c_vp, c_i64, c_vp, c_vp, c_i32, c_vp]),
-    "pg_decode_int4_run": (c_i32, [ctypes.POINTER(PgInt4DecodeArgs), c_vp]),
+    "pg_decode_int4_run": (c_i32, [c_vp, c_vp]),
     "pg_quantize_affine_group16": (c_i32, [c_vp, c_i64, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp]),
 }
 
@@ -217,6 +220,35 @@ def check(rc: int) -> None:
 
 def call(name: str, *args) -> None:
     check(getattr(load(), name)(*args))
+
+
+def packer(structure) -> struct.Struct:
+    """The native packing of an argument structure: packing all fields at once
+    takes a tenth of the time of setting them one by one."""
+    codes = {c_vp: "Q", c_i64: "q", c_i32: "i", ctypes.c_float: "f"}
+    out, at = "", 0
+    for name, kind in structure._fields_:
+        count = 1
+        if issubclass(kind, ctypes.Array):
+            kind, count = kind._type_, kind._length_
+        offset = getattr(structure, name).offset
+        out += "x" * (offset - at) + codes[kind] * count
+        at = offset + ctypes.sizeof(kind) * count
+    return struct.Struct("=" + out + "x" * (ctypes.sizeof(structure) - at))
+
+
+def launch(name: str, device, *args) -> None:
+    """Call entry ``name`` with ``args`` and the current stream of ``device``,
+    which is made the current device for the call."""
+    index = device.index
+    fn = getattr(_lib or load(), name)
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        check(rc)
 
 
 def kernel_pointer(t, name: str) -> int:

@@ -1109,17 +1109,53 @@ int32_t pg_rotary(const pg_rotary_args* a, void* stream) {
   p.table_rows = a->table_rows;
   p.positions = a->positions;
   p.error_flag = device_error_ptr();
-  const int64_t total = a->tokens * rows * (a->head_dim - a->pairs);
-  const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((total + 255) / 256, 148 * 64));
+  // Whole 16-byte chunks: the vector kernel.  (49,152 tokens of 40 FP16 rows:
+  // 168 us against 734 us one pair per thread.)
+  const int size = a->dtype == PG_DTYPE_F32 ? 4 : 2, v = 16 / size;
+  const int table_floats = p.interleaved ? 2 : 4;
+  bool fast = (p.interleaved ? 2 * a->pairs : a->pairs) % v == 0 &&
+              (a->head_dim - 2 * a->pairs) % v == 0 && aligned(a->cosine, 4 * table_floats) &&
+              aligned(a->sine, 4 * table_floats) && a->table_stride % table_floats == 0;
+  for (int i = 0; i < 2 && fast; ++i)
+    fast = p.heads[i] == 0 ||
+           (aligned(p.x[i], 16) && aligned(p.y[i], 16) &&
+            (p.x_stride_t[i] | p.x_stride_h[i] | p.y_stride_t[i] | p.y_stride_h[i]) % v == 0);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (fast) {
+    const int turning = p.interleaved ? 2 * a->pairs / v : a->pairs / v;
+    bool copies = false;
+    for (int i = 0; i < 2; ++i) {
+      p.in_place[i] = p.x[i] == p.y[i] && p.x_stride_t[i] == p.y_stride_t[i] &&
+                      p.x_stride_h[i] == p.y_stride_h[i];
+      copies = copies || (p.heads[i] > 0 && !p.in_place[i]);
+    }
+    p.chunks = turning + (copies ? (a->head_dim - 2 * a->pairs) / v : 0);
+    // Four rows per thread once that still fills the GPU, else one.
+    const int64_t threads = a->tokens * rows * p.chunks;
+    p.row_groups = static_cast<int32_t>(threads >= 148 * 2048 * 4 ? (rows + 3) / 4 : rows);
+    const int64_t per_token = static_cast<int64_t>(p.chunks) * p.row_groups;
+    PG_REQUIRE(per_token < (int64_t(1) << 30), "too many rows");
+    const int64_t units = a->tokens * per_token;
+    const int block = units > 148 * 256 ? 256 : 64;
+    PG_REQUIRE((units + block - 1) / block < (int64_t(1) << 31), "too many rows or tokens");
+    const dim3 grid(static_cast<unsigned>((units + block - 1) / block));
+    if (a->dtype == PG_DTYPE_F16)
+      return launch_pdl(pg::pg_rotary_kernel<__half>, grid, dim3(block), 0, st, "rotary launch",
+                        p);
+    if (a->dtype == PG_DTYPE_BF16)
+      return launch_pdl(pg::pg_rotary_kernel<__nv_bfloat16>, grid, dim3(block), 0, st,
+                        "rotary launch", p);
+    return launch_pdl(pg::pg_rotary_kernel<float>, grid, dim3(block), 0, st, "rotary launch", p);
+  }
+  const int64_t total = a->tokens * rows * (a->head_dim - a->pairs);
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>((total + 255) / 256, 148 * 64)));
   if (a->dtype == PG_DTYPE_F16)
-    return launch_pdl(pg::pg_rotary_kernel<__half>, dim3(blocks), dim3(256), 0, st,
-                      "rotary launch", p);
+    return launch_pdl(pg::pg_rotary_any_kernel<__half>, grid, dim3(256), 0, st, "rotary launch",
+                      p);
   if (a->dtype == PG_DTYPE_BF16)
-    return launch_pdl(pg::pg_rotary_kernel<__nv_bfloat16>, dim3(blocks), dim3(256), 0, st,
+    return launch_pdl(pg::pg_rotary_any_kernel<__nv_bfloat16>, grid, dim3(256), 0, st,
                       "rotary launch", p);
-  return launch_pdl(pg::pg_rotary_kernel<float>, dim3(blocks), dim3(256), 0, st,
-                    "rotary launch", p);
+  return launch_pdl(pg::pg_rotary_any_kernel<float>, grid, dim3(256), 0, st, "rotary launch", p);
 }
 
 int32_t pg_rope_append_int4(const pg_int4_append_args* a, void* stream) {
@@ -1188,23 +1224,31 @@ int32_t pg_rope_append_int4(const pg_int4_append_args* a, void* stream) {
   const bool table16 = aligned(a->cosine, 16) && aligned(a->sine, 16) &&
                        a->table_stride % 4 == 0 && a->pairs % (p.interleaved ? 4 : 8) == 0;
   const bool fast = rows16 && table16;
-  // Row pairs of one token: all in one warp when the tokens alone fill the
-  // GPU, spread over as many warps as it takes otherwise.
-  const int units = (p.hq + 1) / 2 + 2 * ((p.hkv + 1) / 2);
-  const int64_t want = 148 * 64;
+  // Few tokens: a warp per row pair.  Else four query row pairs (or a key and
+  // a value row pair) at a time, a token's groups over as many warps as fill
+  // the GPU.
+  const int64_t pairs_of_rows = (p.hq + 1) / 2 + 2 * ((p.hkv + 1) / 2);
+  const bool wide = a->tokens * pairs_of_rows > 148 * 32;
+  const int64_t units = wide ? (p.hq + 7) / 8 + (p.hkv + 1) / 2 : pairs_of_rows;
   p.split = static_cast<int32_t>(
-      std::min<int64_t>(units, std::max<int64_t>(1, want / a->tokens)));
+      std::min<int64_t>(units, std::max<int64_t>(1, 148 * 64 / a->tokens)));
   const int64_t warps = a->tokens * p.split;
   PG_REQUIRE((warps + 7) / 8 < (int64_t(1) << 31), "too many tokens");
-  const dim3 grid(static_cast<unsigned>((warps + 7) / 8));
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a->dtype == PG_DTYPE_F16)
-    return launch_pdl(fast ? pg::pg_rope_append_int4_kernel<__half, true>
-                           : pg::pg_rope_append_int4_kernel<__half, false>,
-                      grid, dim3(256), 0, st, "rope_append_int4 launch", p);
-  return launch_pdl(fast ? pg::pg_rope_append_int4_kernel<__nv_bfloat16, true>
-                         : pg::pg_rope_append_int4_kernel<__nv_bfloat16, false>,
-                    grid, dim3(256), 0, st, "rope_append_int4 launch", p);
+  // Small blocks spread few warps over the SMs.
+  const int block = wide ? 8 : 2;
+  const dim3 grid(static_cast<unsigned>((warps + block - 1) / block));
+  using Kernel = void (*)(pg::Int4AppendParams);
+  const Kernel kernels[2][2][2] = {
+      {{pg::pg_rope_append_int4_kernel<__half, false, 1>,
+        pg::pg_rope_append_int4_kernel<__half, false, 4>},
+       {pg::pg_rope_append_int4_kernel<__half, true, 1>,
+        pg::pg_rope_append_int4_kernel<__half, true, 4>}},
+      {{pg::pg_rope_append_int4_kernel<__nv_bfloat16, false, 1>,
+        pg::pg_rope_append_int4_kernel<__nv_bfloat16, false, 4>},
+       {pg::pg_rope_append_int4_kernel<__nv_bfloat16, true, 1>,
+        pg::pg_rope_append_int4_kernel<__nv_bfloat16, true, 4>}}};
+  return launch_pdl(kernels[a->dtype == PG_DTYPE_BF16][fast][wide], grid, dim3(block * 32), 0,
+                    static_cast<cudaStream_t>(stream), "rope_append_int4 launch", p);
 }
 
 int32_t pg_int4_read(const void* records, int64_t num_pages, int32_t kv_heads,
@@ -1228,7 +1272,7 @@ int32_t pg_int4_read(const void* records, int64_t num_pages, int32_t kv_heads,
   p.key = key;
   p.value = value;
   p.error_flag = device_error_ptr();
-  const int64_t rows = tokens * kv_heads * 2;
+  const int64_t rows = tokens * kv_heads;
   PG_REQUIRE((rows + 15) / 16 < (int64_t(1) << 31), "too many tokens");
   const dim3 grid(static_cast<unsigned>((rows + 15) / 16));
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -207,26 +207,80 @@ __device__ __forceinline__ void rotate8(float* x, const T* base, int m, int pair
   }
 }
 
-// One warp takes two rows at a time (16 lanes of 8 dims each) of one token:
-// its query rows, its key rows and its value rows; `split` warps share a
-// token.  The table entries of the token's position stay in registers.
-template <typename T, bool FAST>
+// What an append warp knows of its token.
+struct Int4Token {
+  int64_t token, page, center;
+  int tok;
+  const float* cos_row;
+  const float* sin_row;
+};
+
+// Quantise and store lane m's 8 dims of one row of KV head h (the two halves
+// of a warp hold two rows; a row past the last stores nothing).
+__device__ __forceinline__ void store_int4_row(const Int4AppendParams& p, const Int4Token& k,
+                                               bool is_key, int h, int m, float* x) {
+  __half scale, mid;
+  const uint32_t codes = int4_quantize8(x, scale, mid);
+  uint8_t* rec = p.records + (k.page * p.hkv + (h < p.hkv ? h : 0)) * kInt4Record;
+  const int grp = m >> 2;
+  if (is_key) {
+    if (h < p.hkv)
+      *reinterpret_cast<uint32_t*>(rec + k.tok * 64 + (m & 3) * 16 + grp * 4) = codes;
+  } else {
+    // Dims 4a .. 4a+3 of groups 2i and 2i+1 are one word: lanes of an even
+    // group take their first four dims' word, of an odd one the other.
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, codes, 4);
+    const uint32_t word = (grp & 1) ? prmt(other, codes, 0x7632u) : prmt(codes, other, 0x5410u);
+    if (h < p.hkv)
+      *reinterpret_cast<uint32_t*>(rec + kInt4Value + value_code_row(k.tok) * 64 + (m & 3) * 16 +
+                                   (grp & 1) * 8 + (grp >> 1) * 4) = word;
+  }
+  // The token's four scales and midpoints as one 16-byte store.
+  const uint32_t sm = static_cast<uint32_t>(__half_as_ushort(scale)) |
+                      (static_cast<uint32_t>(__half_as_ushort(mid)) << 16);
+  const uint32_t s1 = __shfl_down_sync(0xffffffffu, sm, 4, 16);
+  const uint32_t s2 = __shfl_down_sync(0xffffffffu, sm, 8, 16);
+  const uint32_t s3 = __shfl_down_sync(0xffffffffu, sm, 12, 16);
+  if (m == 0 && h < p.hkv)
+    *reinterpret_cast<uint4*>(rec + (is_key ? kInt4KeyMeta : kInt4ValueMeta) + k.tok * 16) =
+        make_uint4(prmt(sm, s1, 0x5410u), prmt(s2, s3, 0x5410u), prmt(sm, s1, 0x7632u),
+                   prmt(s2, s3, 0x7632u));
+}
+
+template <typename T>
+__device__ __forceinline__ void subtract_center(const Int4AppendParams& p, const Int4Token& k,
+                                                const void* centers, int h, int m, float* x) {
+  if (centers == nullptr) return;
+  float y[8];
+  load8<T, true>(static_cast<const T*>(centers) + (k.center * p.hkv + h) * kHeadDim + 8 * m, y);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = __fsub_rn(x[i], y[i]);
+}
+
+// `split` warps share one token.  A warp takes two rows at a time (16 lanes of
+// 8 dims each) and requests U query row pairs, or a key and a value row pair,
+// before it uses the first.  U = 4 where tokens alone fill the GPU: the
+// table entries, slot and position are then read once per token; U = 1 with
+// a warp per row pair for few tokens, where latency is all.
+template <typename T, bool FAST, int U>
 __global__ void __launch_bounds__(256)
     pg_rope_append_int4_kernel(const __grid_constant__ Int4AppendParams p) {
   pdl_launch_dependents();
-  pdl_wait_primary();
   const int lane = threadIdx.x & 31, half = lane >> 4, m = lane & 15;
   const int64_t w = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-  const int64_t token = w / p.split;
-  const int part = static_cast<int>(w - token * p.split);
-  if (token >= p.tokens) return;
-  const int slot = p.slots[token];
+  Int4Token k;
+  k.token = w / p.split;
+  const int part = static_cast<int>(w - k.token * p.split);
+  if (k.token >= p.tokens) return;
+  pdl_wait_primary();
+  const int slot = p.slots[k.token];
+  const int pos = p.positions[k.token];
+  k.center = p.center_rows != nullptr ? p.center_rows[k.token] : 0;
   if (slot < 0) return;
-  const int64_t page = slot >> 4;
-  const int tok = slot & 15;
-  const int pos = p.positions[token];
-  const int64_t center = p.center_rows != nullptr ? p.center_rows[token] : 0;
-  if (page >= p.num_pages || (p.key_center != nullptr && (center < 0 || center >= p.num_centers))) {
+  k.page = slot >> 4;
+  k.tok = slot & 15;
+  if (k.page >= p.num_pages ||
+      (p.key_center != nullptr && (k.center < 0 || k.center >= p.num_centers))) {
     record_error(p.error_flag, kDevBadPageId);
     return;
   }
@@ -234,8 +288,8 @@ __global__ void __launch_bounds__(256)
     record_error(p.error_flag, kDevBadPosition);
     return;
   }
-  const float* cos_row = p.cos + pos * p.table_stride;
-  const float* sin_row = p.sin + pos * p.table_stride;
+  k.cos_row = p.cos + pos * p.table_stride;
+  k.sin_row = p.sin + pos * p.table_stride;
   float c[8], s[8];
   if constexpr (FAST) {
     // The lane's entries: half layout 8 of them, interleaved 4.
@@ -245,66 +299,75 @@ __global__ void __launch_bounds__(256)
     for (int i = 0; i < 8; i += 4) {
       const bool in = (p.interleaved ? i == 0 : m < 2 * step) && j + i < p.pairs;
       const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-      const float4 a = in ? __ldg(reinterpret_cast<const float4*>(cos_row + j + i)) : z;
-      const float4 b = in ? __ldg(reinterpret_cast<const float4*>(sin_row + j + i)) : z;
+      const float4 a = in ? __ldg(reinterpret_cast<const float4*>(k.cos_row + j + i)) : z;
+      const float4 b = in ? __ldg(reinterpret_cast<const float4*>(k.sin_row + j + i)) : z;
       c[i] = a.x; c[i + 1] = a.y; c[i + 2] = a.z; c[i + 3] = a.w;
       s[i] = b.x; s[i + 1] = b.y; s[i + 2] = b.z; s[i + 3] = b.w;
     }
   }
-  const int qu = (p.hq + 1) >> 1, ku = (p.hkv + 1) >> 1;  // row pairs
-  for (int u = part; u < qu + 2 * ku; u += p.split) {
-    if (u < qu) {
-      const int h = 2 * u + half;
-      const int hc = h < p.hq ? h : p.hq - 1;  // an odd last row: both halves load it
-      const T* row = static_cast<const T*>(p.q) + token * p.q_stride_t + hc * p.q_stride_h;
-      float x[8];
-      load8<T, FAST>(row + 8 * m, x);
-      rotate8<T, FAST>(x, row, m, p.pairs, p.interleaved, c, s, cos_row, sin_row);
-      // In place, other lanes' partner dims are this lane's.
-      if constexpr (!FAST) __syncwarp();
-      if (h < p.hq)
-        store8<T, FAST>(static_cast<T*>(p.rotated_q) + token * p.rq_stride_t +
-                            h * p.rq_stride_h + 8 * m, x);
-      continue;
-    }
-    const bool is_key = u < qu + ku;
-    const int h = 2 * (u - qu - (is_key ? 0 : ku)) + half;
+  const T* q = static_cast<const T*>(p.q) + k.token * p.q_stride_t;
+  const T* kr = static_cast<const T*>(p.k) + k.token * p.k_stride_t;
+  const T* vr = static_cast<const T*>(p.v) + k.token * p.v_stride_t;
+  T* rq = static_cast<T*>(p.rotated_q) + k.token * p.rq_stride_t;
+  // Row h of two halves; an odd last row is loaded by both, stored by one.
+  auto turn_and_store = [&](float* x, const T* row, T* out, bool store) {
+    rotate8<T, FAST>(x, row, m, p.pairs, p.interleaved, c, s, k.cos_row, k.sin_row);
+    // In place, other lanes' partner dims are this lane's.
+    if constexpr (!FAST) __syncwarp();
+    if (store) store8<T, FAST>(out + 8 * m, x);
+  };
+  auto append_row = [&](float* x, bool is_key, int h, const T* row) {
     const int hc = h < p.hkv ? h : p.hkv - 1;
-    const T* row = is_key ? static_cast<const T*>(p.k) + token * p.k_stride_t + hc * p.k_stride_h
-                          : static_cast<const T*>(p.v) + token * p.v_stride_t + hc * p.v_stride_h;
-    float x[8];
-    load8<T, FAST>(row + 8 * m, x);
-    if (is_key) {
-      rotate8<T, FAST>(x, row, m, p.pairs, p.interleaved, c, s, cos_row, sin_row);
-      if constexpr (!FAST) __syncwarp();
-      if (p.rotated_k != nullptr && h < p.hkv)
-        store8<T, FAST>(static_cast<T*>(p.rotated_k) + token * p.rk_stride_t +
-                            h * p.rk_stride_h + 8 * m, x);
-    }
-    const void* cen = is_key ? p.key_center : p.value_center;
-    if (cen != nullptr) {
-      float y[8];
-      load8<T, true>(static_cast<const T*>(cen) + (center * p.hkv + hc) * kHeadDim + 8 * m, y);
+    if (is_key)
+      turn_and_store(x, row,
+                     static_cast<T*>(p.rotated_k) + k.token * p.rk_stride_t + hc * p.rk_stride_h,
+                     p.rotated_k != nullptr && h < p.hkv);
+    subtract_center<T>(p, k, is_key ? p.key_center : p.value_center, hc, m, x);
+    store_int4_row(p, k, is_key, h, m, x);
+  };
+  const int nq = (p.hq + 2 * U - 1) / (2 * U), nk = (p.hkv + 1) >> 1;
+  if constexpr (U > 1) {
+    for (int u = part; u < nq + nk; u += p.split) {
+      if (u < nq) {
+        float x[U][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = __fsub_rn(x[i], y[i]);
+        for (int i = 0; i < U; ++i) {
+          const int h = 2 * (u * U + i) + half;
+          load8<T, FAST>(q + (h < p.hq ? h : p.hq - 1) * p.q_stride_h + 8 * m, x[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          const int h = 2 * (u * U + i) + half;
+          if (2 * (u * U + i) >= p.hq) break;
+          const int hc = h < p.hq ? h : p.hq - 1;
+          turn_and_store(x[i], q + hc * p.q_stride_h, rq + hc * p.rq_stride_h, h < p.hq);
+        }
+      } else {
+        const int h = 2 * (u - nq) + half;
+        const int hc = h < p.hkv ? h : p.hkv - 1;
+        float x[8], y[8];
+        load8<T, FAST>(kr + hc * p.k_stride_h + 8 * m, x);
+        load8<T, FAST>(vr + hc * p.v_stride_h + 8 * m, y);
+        append_row(x, true, h, kr + hc * p.k_stride_h);
+        append_row(y, false, h, nullptr);
+      }
     }
-    __half scale, mid;
-    const uint32_t codes = int4_quantize8(x, scale, mid);
-    if (h >= p.hkv) continue;
-    uint8_t* rec = p.records + (page * p.hkv + h) * kInt4Record;
-    const int grp = m >> 2;
-    if (is_key) {
-      *reinterpret_cast<uint32_t*>(rec + tok * 64 + (m & 3) * 16 + grp * 4) = codes;
-    } else {
-      uint8_t* vr = rec + kInt4Value + value_code_row(tok) * 64 + (m & 3) * 16 + grp * 2;
-      *reinterpret_cast<uint16_t*>(vr) = static_cast<uint16_t>(codes);
-      *reinterpret_cast<uint16_t*>(vr + 8) = static_cast<uint16_t>(codes >> 16);
-    }
-    if ((m & 3) == 0) {
-      __half* meta =
-          reinterpret_cast<__half*>(rec + (is_key ? kInt4KeyMeta : kInt4ValueMeta) + tok * 16);
-      meta[grp] = scale;
-      meta[4 + grp] = mid;
+  } else {
+    for (int u = part; u < nq + 2 * nk; u += p.split) {
+      float x[8];
+      if (u < nq) {
+        const int h = 2 * u + half;
+        const int hc = h < p.hq ? h : p.hq - 1;
+        load8<T, FAST>(q + hc * p.q_stride_h + 8 * m, x);
+        turn_and_store(x, q + hc * p.q_stride_h, rq + hc * p.rq_stride_h, h < p.hq);
+      } else {
+        const bool is_key = u < nq + nk;
+        const int h = 2 * (u - nq - (is_key ? 0 : nk)) + half;
+        const int hc = h < p.hkv ? h : p.hkv - 1;
+        const T* row = is_key ? kr + hc * p.k_stride_h : vr + hc * p.v_stride_h;
+        load8<T, FAST>(row + 8 * m, x);
+        append_row(x, is_key, h, row);
+      }
     }
   }
 }
@@ -320,49 +383,52 @@ struct Int4ReadParams {
   int* error_flag;
 };
 
-// 16 lanes per (token, head, key or value); skipped slots read as zeros.
+// 16 lanes per (token, head): the key row and the value row; skipped slots
+// read as zeros.
 template <typename T>
 __global__ void __launch_bounds__(256)
     pg_int4_read_kernel(const __grid_constant__ Int4ReadParams p) {
   pdl_launch_dependents();
   pdl_wait_primary();
-  const int m = threadIdx.x & 15;
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 4;
-  const int64_t th = row >> 1;
+  const int m = threadIdx.x & 15, grp = m >> 2;
+  const int64_t th = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 4;
   const int64_t token = th / p.hkv;
   if (token >= p.tokens) return;
   const int h = static_cast<int>(th - token * p.hkv);
-  const bool is_key = (row & 1) == 0;
-  T* out = static_cast<T*>(is_key ? p.key : p.value) + th * kHeadDim + 8 * m;
   const int slot = p.slots[token];
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  uint32_t codes[2] = {0x88888888u, 0x88888888u};
+  float s[2] = {0.f, 0.f}, mid[2] = {0.f, 0.f};
   if (slot >= 0 && (slot >> 4) >= p.num_pages) {
     record_error(p.error_flag, kDevBadPageId);
   } else if (slot >= 0) {
-    const int tok = slot & 15, grp = m >> 2;
+    const int tok = slot & 15;
     const uint8_t* rec = p.records + (static_cast<int64_t>(slot >> 4) * p.hkv + h) * kInt4Record;
-    uint32_t w;
-    if (is_key) {
-      w = *reinterpret_cast<const uint32_t*>(rec + tok * 64 + (m & 3) * 16 + grp * 4);
-    } else {
-      const uint8_t* vr = rec + kInt4Value + value_code_row(tok) * 64 + (m & 3) * 16 + grp * 2;
-      w = *reinterpret_cast<const uint16_t*>(vr) |
-          (static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(vr + 8)) << 16);
-    }
-    const __half* meta = reinterpret_cast<const __half*>(
-        rec + (is_key ? kInt4KeyMeta : kInt4ValueMeta) + tok * 16);
-    const float s = __half2float(meta[grp]), mid = __half2float(meta[4 + grp]);
+    codes[0] = *reinterpret_cast<const uint32_t*>(rec + tok * 64 + (m & 3) * 16 + grp * 4);
+    const uint8_t* vr = rec + kInt4Value + value_code_row(tok) * 64 + (m & 3) * 16 + grp * 2;
+    codes[1] = *reinterpret_cast<const uint16_t*>(vr) |
+               (static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(vr + 8)) << 16);
+    const __half* km = reinterpret_cast<const __half*>(rec + kInt4KeyMeta + tok * 16) + grp;
+    const __half* vm = reinterpret_cast<const __half*>(rec + kInt4ValueMeta + tok * 16) + grp;
+    s[0] = __half2float(km[0]);
+    mid[0] = __half2float(km[4]);
+    s[1] = __half2float(vm[0]);
+    mid[1] = __half2float(vm[4]);
+  }
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    T* out = static_cast<T*>(kv == 0 ? p.key : p.value) + th * kHeadDim + 8 * m;
+    float x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float z = static_cast<float>(static_cast<int>((w >> (4 * i)) & 15u) - 8);
-      x[i] = __fadd_rn(__fmul_rn(z, s), mid);
+      const float z = static_cast<float>(static_cast<int>((codes[kv] >> (4 * i)) & 15u) - 8);
+      x[i] = __fadd_rn(__fmul_rn(z, s[kv]), mid[kv]);
     }
-  }
-  if constexpr (sizeof(T) == 2) {
-    store8<T, true>(out, x);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) out[i] = from_float<T>(x[i]);
+    if constexpr (sizeof(T) == 2) {
+      store8<T, true>(out, x);
+    } else {
+      reinterpret_cast<float4*>(out)[0] = make_float4(x[0], x[1], x[2], x[3]);
+      reinterpret_cast<float4*>(out)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    }
   }
 }
 

@@ -23,14 +23,18 @@ GROUP = 32
 RECORD_BYTES = 2560
 
 
-def check_records(records: torch.Tensor) -> None:
-    if (not records.is_cuda or records.dtype != torch.uint8 or records.dim() != 3
-            or records.size(0) == 0 or records.size(1) == 0 or records.size(2) != RECORD_BYTES
-            or not records.is_contiguous() or records.data_ptr() % 16):
+def check_records(records: torch.Tensor) -> tuple[int, int, int]:
+    """(address, pages, KV heads) of a pool's records."""
+    shape = records.shape
+    address = records.data_ptr()
+    if (not records.is_cuda or records.dtype is not torch.uint8 or len(shape) != 3
+            or shape[0] == 0 or shape[1] == 0 or shape[2] != RECORD_BYTES
+            or not records.is_contiguous() or address % 16):
         raise ValueError(f"records must be contiguous 16-byte aligned CUDA uint8 "
                          f"[pages,Hkv,{RECORD_BYTES}]")
-    if records.size(0) >= 1 << 27:
+    if shape[0] >= 1 << 27:
         raise ValueError("a pool holds fewer than 2^27 pages")
+    return address, shape[0], shape[1]
 
 
 class Int4PagePool:
@@ -62,19 +66,19 @@ class Int4PagePool:
         zeros and set the device guard word."""
         if dtype not in DTYPES:
             raise ValueError("values are read as float16, bfloat16 or float32")
-        check_token_index(slots, "slots", slots.numel(), self.records.device)
-        shape = (slots.numel(), self.kv_heads, HEAD_DIM)
-        outs = []
+        records = self.records
+        device, tokens, kv_heads = records.device, slots.numel(), self.kv_heads
+        slot_ptr = check_token_index(slots, "slots", tokens, device)
+        shape = (tokens, kv_heads, HEAD_DIM)
+        if key_out is None:
+            key_out = torch.empty(shape, dtype=dtype, device=device)
+        if value_out is None:
+            value_out = torch.empty(shape, dtype=dtype, device=device)
         for name, t in (("key_out", key_out), ("value_out", value_out)):
-            if t is None:
-                t = torch.empty(shape, dtype=dtype, device=self.records.device)
-            elif (t.shape != shape or t.dtype != dtype or t.device != self.records.device
-                  or not t.is_contiguous() or t.data_ptr() % 16):
+            if (t.shape != shape or t.dtype is not dtype or t.device != device
+                    or not t.is_contiguous() or t.data_ptr() % 16):
                 raise ValueError(f"{name} must be contiguous 16-byte aligned "
-                                 f"[T,{self.kv_heads},{HEAD_DIM}] {dtype}")
-            outs.append(t)
-        with torch.cuda.device(self.records.device):
-            _lib.call("pg_int4_read", self.records.data_ptr(), self.num_pages, self.kv_heads,
-                      slots.data_ptr(), slots.numel(), outs[0].data_ptr(), outs[1].data_ptr(),
-                      DTYPES[dtype], torch.cuda.current_stream().cuda_stream)
-        return outs[0], outs[1]
+                                 f"[T,{kv_heads},{HEAD_DIM}] {dtype}")
+        _lib.launch("pg_int4_read", device, records.data_ptr(), self.num_pages, kv_heads,
+                    slot_ptr, tokens, key_out.data_ptr(), value_out.data_ptr(), DTYPES[dtype])
+        return key_out, value_out

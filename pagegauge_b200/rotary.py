@@ -9,7 +9,6 @@ the arithmetic is FP32 from FP32 tables, rounded once.
 
 from __future__ import annotations
 
-import ctypes
 import math
 from dataclasses import dataclass
 
@@ -94,35 +93,58 @@ def rotary_tables(positions: int, rotary_dim: int = 128, theta: float = 1.0e6,
     return (angle.cos() * scale).float(), (angle.sin() * scale).float()
 
 
+_PACK_ROTARY = _lib.packer(_lib.PgRotaryArgs).pack
+
+
 def check_tables(cosine: torch.Tensor, sine: torch.Tensor, device: torch.device,
-                 head_dim: int) -> int:
-    """The number of rotated pairs of a table pair [positions, pairs]."""
-    if (cosine.dtype != torch.float32 or sine.dtype != torch.float32 or cosine.dim() != 2
-            or cosine.shape != sine.shape or cosine.size(0) == 0):
+                 head_dim: int) -> tuple[int, int, int]:
+    """(rows, row stride, pairs) of a table pair [positions, pairs]."""
+    if (cosine.dtype is not torch.float32 or sine.dtype is not torch.float32
+            or cosine.dim() != 2 or cosine.shape != sine.shape):
         raise ValueError("cosine and sine must be matching float32 [positions, pairs] tables")
     if cosine.device != device or sine.device != device:
         raise ValueError("rotary tables must be on the rows' device")
-    pairs = cosine.size(1)
-    if cosine.stride() != sine.stride() or cosine.stride(1) != 1 or cosine.stride(0) < pairs:
+    rows, pairs = cosine.shape
+    strides = cosine.stride()
+    if strides != sine.stride() or strides[1] != 1 or strides[0] < pairs:
         raise ValueError("rotary tables must have equal strides and contiguous rows")
-    if not 1 <= pairs <= head_dim // 2:
-        raise ValueError("the tables rotate more dims than a head has")
-    return pairs
+    if rows == 0 or not 1 <= pairs <= head_dim // 2:
+        raise ValueError("the tables must have rows and rotate no more dims than a head has")
+    return rows, strides[0], pairs
 
 
-def check_token_index(t: torch.Tensor, name: str, tokens: int, device: torch.device) -> None:
-    if (t.dtype != torch.int32 or t.dim() != 1 or t.numel() != tokens or t.device != device
+def check_token_index(t: torch.Tensor, name: str, tokens: int, device: torch.device) -> int:
+    """The address of an int32 index per token."""
+    if (t.dtype is not torch.int32 or t.shape != (tokens,) or t.device != device
             or not t.is_contiguous()):
         raise ValueError(f"{name} must be contiguous int32 [{tokens}] on the rows' device")
+    return t.data_ptr()
 
 
-def check_output(out: torch.Tensor, like: torch.Tensor, name: str) -> None:
-    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
+def check_output(out: torch.Tensor, like: torch.Tensor, name: str) -> tuple[int, ...]:
+    """The strides of an output that takes ``like``'s rows."""
+    if out.shape != like.shape or out.dtype is not like.dtype or out.device != like.device:
         raise ValueError(f"{name} must have its input's shape, dtype and device")
-    if out.stride(-1) != 1:
+    strides = out.stride()
+    if strides[2] != 1:
         raise ValueError(f"{name} must have a contiguous last dimension")
-    if any(size > 1 and stride <= 0 for size, stride in zip(out.shape, out.stride())):
+    if strides[0] <= 0 < out.size(0) - 1 or strides[1] <= 0 < out.size(1) - 1:
         raise ValueError(f"{name} must not be expanded")
+    return strides
+
+
+def check_rows(x: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device,
+               tokens: int, head_dim: int) -> tuple[int, tuple[int, ...]]:
+    """(heads, strides) of rows [tokens, heads, head_dim]."""
+    if x.dtype is not dtype or x.device != device or not x.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor of the query's device and dtype")
+    shape = x.shape
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != head_dim:
+        raise ValueError(f"{name} must be [{tokens}, heads, {head_dim}]")
+    strides = x.stride()
+    if strides[2] != 1 and x.numel():
+        raise ValueError(f"{name} must have a contiguous last dimension")
+    return shape[1], strides
 
 
 def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, cosine: torch.Tensor,
@@ -140,39 +162,34 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, cosine: torch.Te
     other strides.  The outputs may be the inputs (in place); they must not
     overlap them in any other way.  Rows of a token whose position is outside
     the tables are not written (``runtime.read_device_error`` reports it)."""
-    if query.dtype not in DTYPES:
+    dtype, device = query.dtype, query.device
+    if dtype not in DTYPES:
         raise ValueError("rows must be float16, bfloat16 or float32")
-    tensors = [(query, query_out, "query")]
+    if query.dim() != 3:
+        raise ValueError("query must be [tokens, heads, head_dim]")
+    tokens, _, head_dim = query.shape
+    hq, qs = check_rows(query, "query", dtype, device, tokens, head_dim)
+    if query_out is None:
+        query_out = torch.empty(query.shape, dtype=dtype, device=device)
+        qos = (hq * head_dim, head_dim)
+    else:
+        qos = check_output(query_out, query, "query_out")
+    hkv, ks, kos, k_ptr, ko_ptr = 0, (0, 0), (0, 0), 0, 0
     if key is not None:
-        tensors.append((key, key_out, "key"))
+        hkv, ks = check_rows(key, "key", dtype, device, tokens, head_dim)
+        if key_out is None:
+            key_out = torch.empty(key.shape, dtype=dtype, device=device)
+            kos = (hkv * head_dim, head_dim)
+        else:
+            kos = check_output(key_out, key, "key_out")
+        k_ptr, ko_ptr = key.data_ptr(), key_out.data_ptr()
     elif key_out is not None:
         raise ValueError("key_out without key")
-    a = _lib.PgRotaryArgs()
-    outs: list = [None, None]
-    device, tokens, head_dim = query.device, query.size(0), query.size(-1)
-    for i, (x, y, name) in enumerate(tensors):
-        if not x.is_cuda or x.device != device or x.dtype != query.dtype:
-            raise ValueError(f"{name} must be a CUDA tensor of the query's device and dtype")
-        if x.dim() != 3 or x.size(0) != tokens or x.size(2) != head_dim:
-            raise ValueError(f"{name} must be [{tokens}, heads, {head_dim}]")
-        if x.stride(2) != 1 and x.numel():
-            raise ValueError(f"{name} must have a contiguous last dimension")
-        if y is None:
-            y = torch.empty(x.shape, dtype=x.dtype, device=device)
-        else:
-            check_output(y, x, f"{name}_out")
-        outs[i] = y
-        a.x[i], a.y[i] = x.data_ptr(), y.data_ptr()
-        a.x_stride_t[i], a.x_stride_h[i] = x.stride(0), x.stride(1)
-        a.y_stride_t[i], a.y_stride_h[i] = y.stride(0), y.stride(1)
-        a.heads[i] = x.size(1)
-    a.pairs = check_tables(cosine, sine, device, head_dim)
-    check_token_index(positions, "positions", tokens, device)
-    a.tokens, a.head_dim = tokens, head_dim
-    a.cosine, a.sine, a.positions = cosine.data_ptr(), sine.data_ptr(), positions.data_ptr()
-    a.table_rows, a.table_stride = cosine.size(0), cosine.stride(0)
-    a.interleaved, a.adjoint = int(interleaved), int(adjoint)
-    a.dtype = DTYPES[query.dtype]
-    with torch.cuda.device(device):
-        _lib.call("pg_rotary", ctypes.byref(a), torch.cuda.current_stream().cuda_stream)
-    return outs[0], outs[1]
+    rows, row_stride, pairs = check_tables(cosine, sine, device, head_dim)
+    pos_ptr = check_token_index(positions, "positions", tokens, device)
+    _lib.launch("pg_rotary", device, _PACK_ROTARY(
+        query.data_ptr(), k_ptr, query_out.data_ptr(), ko_ptr, qs[0], ks[0], qs[1], ks[1],
+        qos[0], kos[0], qos[1], kos[1], tokens, row_stride, rows, cosine.data_ptr(),
+        sine.data_ptr(), pos_ptr, hq, hkv, head_dim, pairs, bool(interleaved), bool(adjoint),
+        DTYPES[dtype]))
+    return query_out, key_out

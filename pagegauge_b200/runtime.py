@@ -11,16 +11,15 @@ CUDA stream; nothing is allocated on the device.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
 from .int4 import check_records
-from .rotary import DTYPES, check_output, check_tables, check_token_index
+from .rotary import DTYPES, check_output, check_rows, check_tables, check_token_index
 
 HEAD_DIM = 128
 PAGE = 16
+_PACK_INT4_APPEND = _lib.packer(_lib.PgInt4AppendArgs).pack
 
 
 def _stream(tensor: torch.Tensor) -> int:
@@ -313,62 +312,51 @@ class AppendExtension:
         ``center_rows[t]``, or row 0) are subtracted before quantising; the
         decode adds the value centre back.  ``rotated_query`` and the optional
         ``rotated_key`` take the rotated rows and may be the inputs."""
-        _require(query.is_cuda and query.dim() == 3, "query must be CUDA of rank three")
-        _require(query.dtype in (torch.float16, torch.bfloat16),
+        dtype, device = query.dtype, query.device
+        _require(dtype is torch.float16 or dtype is torch.bfloat16,
                  "query must be float16 or bfloat16")
-        tokens, device = query.size(0), query.device
-        for name, t in (("query", query), ("key", key), ("value", value)):
-            _require(t.device == device and t.dtype == query.dtype,
-                     f"{name} must have the query's device and dtype")
-            _require(t.dim() == 3 and t.size(0) == tokens and t.size(1) > 0
-                     and t.size(2) == HEAD_DIM, f"{name} must be [{tokens},heads,{HEAD_DIM}]")
-            _require(t.stride(2) == 1 or tokens == 0,
-                     f"{name} must have a contiguous last dimension")
-        _require(key.shape == value.shape, "K/V input shapes must match")
-        kv_heads = key.size(1)
-        check_output(rotated_query, query, "rotated_query")
-        pairs = check_tables(cosine, sine, device, HEAD_DIM)
-        check_token_index(positions, "positions", tokens, device)
-        check_token_index(token_slots, "token_slots", tokens, device)
-        check_records(records)
-        _require(records.device == device and records.size(1) == kv_heads,
+        _require(query.dim() == 3, "query must have rank three")
+        tokens = query.size(0)
+        hq, qs = check_rows(query, "query", dtype, device, tokens, HEAD_DIM)
+        kv_heads, ks = check_rows(key, "key", dtype, device, tokens, HEAD_DIM)
+        v_heads, vs = check_rows(value, "value", dtype, device, tokens, HEAD_DIM)
+        _require(kv_heads == v_heads, "K/V input shapes must match")
+        _require(hq > 0 and kv_heads > 0, "head counts must be positive")
+        rqs = check_output(rotated_query, query, "rotated_query")
+        rows, row_stride, pairs = check_tables(cosine, sine, device, HEAD_DIM)
+        pos_ptr = check_token_index(positions, "positions", tokens, device)
+        slot_ptr = check_token_index(token_slots, "token_slots", tokens, device)
+        records_ptr, pages, heads = check_records(records)
+        _require(records.device == device and heads == kv_heads,
                  "records must be [pages,Hkv,2560] on the rows' device")
-        a = _lib.PgInt4AppendArgs()
+        rk_ptr, rks = 0, (0, 0)
         if rotated_key is not None:
-            check_output(rotated_key, key, "rotated_key")
-            a.rotated_key = rotated_key.data_ptr()
-            a.rk_stride_t, a.rk_stride_h = rotated_key.stride(0), rotated_key.stride(1)
-        _require((key_center is None) == (value_center is None),
-                 "key and value centers are both given or both None")
-        if key_center is not None:
+            rks = check_output(rotated_key, key, "rotated_key")
+            rk_ptr = rotated_key.data_ptr()
+        kc_ptr = vc_ptr = row_ptr = centers = 0
+        if key_center is not None and value_center is not None:
             for name, t in (("key_center", key_center), ("value_center", value_center)):
-                _require(t.device == device and t.dtype == query.dtype and t.is_contiguous()
-                         and t.dim() == 3 and t.size(0) > 0
-                         and tuple(t.shape[1:]) == (kv_heads, HEAD_DIM),
+                shape = t.shape
+                _require(t.device == device and t.dtype is dtype and t.is_contiguous()
+                         and len(shape) == 3 and shape[0] > 0 and shape[1] == kv_heads
+                         and shape[2] == HEAD_DIM,
                          f"{name} must be contiguous [rows,{kv_heads},{HEAD_DIM}] of the "
                          "query's dtype")
-            _require(key_center.size(0) == value_center.size(0), "center row counts must match")
-            a.key_center, a.value_center = key_center.data_ptr(), value_center.data_ptr()
-            a.num_centers = key_center.size(0)
+            centers = key_center.size(0)
+            _require(centers == value_center.size(0), "center row counts must match")
+            kc_ptr, vc_ptr = key_center.data_ptr(), value_center.data_ptr()
             if center_rows is not None:
-                check_token_index(center_rows, "center_rows", tokens, device)
-                a.center_rows = center_rows.data_ptr()
+                row_ptr = check_token_index(center_rows, "center_rows", tokens, device)
         else:
+            _require(key_center is None and value_center is None,
+                     "key and value centers are both given or both None")
             _require(center_rows is None, "center_rows without centers")
-        a.query, a.key, a.value = query.data_ptr(), key.data_ptr(), value.data_ptr()
-        a.rotated_query = rotated_query.data_ptr()
-        a.q_stride_t, a.q_stride_h = query.stride(0), query.stride(1)
-        a.k_stride_t, a.k_stride_h = key.stride(0), key.stride(1)
-        a.v_stride_t, a.v_stride_h = value.stride(0), value.stride(1)
-        a.rq_stride_t, a.rq_stride_h = rotated_query.stride(0), rotated_query.stride(1)
-        a.cosine, a.sine = cosine.data_ptr(), sine.data_ptr()
-        a.table_stride, a.table_rows = cosine.stride(0), cosine.size(0)
-        a.positions, a.slots = positions.data_ptr(), token_slots.data_ptr()
-        a.records, a.num_pages = records.data_ptr(), records.size(0)
-        a.tokens, a.query_heads, a.kv_heads = tokens, query.size(1), kv_heads
-        a.pairs, a.interleaved, a.dtype = pairs, int(interleaved), DTYPES[query.dtype]
-        with torch.cuda.device(device):
-            _lib.call("pg_rope_append_int4", ctypes.byref(a), _stream(query))
+        _lib.launch("pg_rope_append_int4", device, _PACK_INT4_APPEND(
+            query.data_ptr(), key.data_ptr(), value.data_ptr(), rotated_query.data_ptr(), rk_ptr,
+            qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], rqs[0], rqs[1], rks[0], rks[1],
+            cosine.data_ptr(), sine.data_ptr(), row_stride, rows, pos_ptr, slot_ptr, records_ptr,
+            pages, kc_ptr, vc_ptr, row_ptr, centers, tokens, hq, kv_heads, pairs,
+            bool(interleaved), DTYPES[dtype], 0))
 
     def exact_tail_merge_center(self, query, exact_key_pages, exact_value_pages,
                                 exact_page_indices, exact_last_page_len, old_output, old_lse,

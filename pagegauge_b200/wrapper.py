@@ -39,6 +39,7 @@ from .rotary import DTYPES, check_output
 HEAD_DIM = 128
 PAGE = 16
 ITEM_BYTES = ctypes.sizeof(_lib.PgDecodeItem)
+_PACK_INT4_DECODE = _lib.packer(_lib.PgInt4DecodeArgs).pack
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -401,50 +402,46 @@ class Int4DecodeWrapper(BatchDecodeWithPagedKVCacheWrapper):
         if plan is None:
             raise RuntimeError("plan() must be called before run()")
         records = getattr(records, "records", records)
-        check_records(records)
         device = self._ws.buffer.device
-        if records.device != device or records.size(1) != self._num_kv_heads:
-            raise ValueError(f"records must be [pages,{self._num_kv_heads},2560] on the "
-                             "workspace's device")
-        if (q.dtype not in (torch.float16, torch.bfloat16) or q.device != device
-                or tuple(q.shape) != (plan.batch, self._num_qo_heads, HEAD_DIM)):
-            raise ValueError(f"q must be float16 or bfloat16 "
-                             f"[{plan.batch},{self._num_qo_heads},{HEAD_DIM}] on the "
-                             "workspace's device")
-        if q.stride(2) != 1:
+        kv_heads, hq = plan.kv_heads, self._num_qo_heads
+        records_ptr, pages, heads = check_records(records)
+        if records.device != device or heads != kv_heads:
+            raise ValueError(f"records must be [pages,{kv_heads},2560] on the workspace's device")
+        dtype = q.dtype
+        if ((dtype is not torch.float16 and dtype is not torch.bfloat16) or q.device != device
+                or q.shape != (plan.batch, hq, HEAD_DIM)):
+            raise ValueError(f"q must be float16 or bfloat16 [{plan.batch},{hq},{HEAD_DIM}] on "
+                             "the workspace's device")
+        qs = q.stride()
+        if qs[2] != 1:
             raise ValueError("q must have a contiguous last dimension")
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=device)
-        else:
-            check_output(out, q, "out")
+            out = torch.empty(q.shape, dtype=dtype, device=device)
+        os = check_output(out, q, "out")
         if lse is None and return_lse:
-            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=device)
-        if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2]
-                                or lse.device != device or not lse.is_contiguous()):
-            raise ValueError(f"lse must be contiguous float32 [{plan.batch},"
-                             f"{self._num_qo_heads}] on the workspace's device")
-        a = _lib.PgInt4DecodeArgs()
+            lse = torch.empty((plan.batch, hq), dtype=torch.float32, device=device)
+        lse_ptr = 0
+        if lse is not None:
+            if (lse.dtype is not torch.float32 or lse.shape != (plan.batch, hq)
+                    or lse.device != device or not lse.is_contiguous()):
+                raise ValueError(f"lse must be contiguous float32 [{plan.batch},{hq}] on the "
+                                 "workspace's device")
+            lse_ptr = lse.data_ptr()
+        vc_ptr = 0
         if value_center is not None:
-            if (value_center.dtype != q.dtype or value_center.device != device
+            if (value_center.dtype is not dtype or value_center.device != device
                     or not value_center.is_contiguous()
-                    or tuple(value_center.shape) != (plan.batch, self._num_kv_heads, HEAD_DIM)):
-                raise ValueError(f"value_center must be contiguous [{plan.batch},"
-                                 f"{self._num_kv_heads},{HEAD_DIM}] of q's dtype")
-            a.value_center, a.vc_stride_b = value_center.data_ptr(), value_center.stride(0)
-        a.q, a.q_stride_b, a.q_stride_h = q.data_ptr(), q.stride(0), q.stride(1)
-        a.out, a.out_stride_b, a.out_stride_h = out.data_ptr(), out.stride(0), out.stride(1)
-        a.lse_out = None if lse is None else lse.data_ptr()
-        a.records, a.num_pages = records.data_ptr(), records.size(0)
-        a.indices, a.last_page_len = self._indices.data_ptr(), self._last_len.data_ptr()
-        a.items, a.item_off = plan.items_ptr, plan.off_ptr
-        a.part_o, a.part_lse = plan.o_ptr, plan.lse_ptr
-        a.num_items, a.batch = plan.num_items, plan.batch
-        a.kv_heads, a.group = plan.kv_heads, plan.group
-        a.final_mode = int(plan.single and plan.num_items > 0)
-        a.dtype = DTYPES[q.dtype]
-        a.sm_scale = self._sm_scale if sm_scale is None else float(sm_scale)
-        with torch.cuda.device(device):
-            _lib.call("pg_decode_int4_run", ctypes.byref(a), _stream(q))
+                    or value_center.shape != (plan.batch, kv_heads, HEAD_DIM)):
+                raise ValueError(f"value_center must be contiguous [{plan.batch},{kv_heads},"
+                                 f"{HEAD_DIM}] of q's dtype")
+            vc_ptr = value_center.data_ptr()
+        _lib.launch("pg_decode_int4_run", device, _PACK_INT4_DECODE(
+            q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], lse_ptr, vc_ptr,
+            kv_heads * HEAD_DIM, records_ptr, pages, self._indices.data_ptr(),
+            self._last_len.data_ptr(), plan.items_ptr, plan.off_ptr, plan.o_ptr, plan.lse_ptr,
+            plan.num_items, plan.batch, kv_heads, plan.group,
+            plan.single and plan.num_items > 0, DTYPES[dtype],
+            self._sm_scale if sm_scale is None else sm_scale, 0))
         return (out, lse) if return_lse else out
 
     forward = run

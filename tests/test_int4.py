@@ -123,3 +123,17 @@ def test_pool_refuses():
         Int4PagePool(2, 8, device="cpu")
     with pytest.raises(ValueError):
         Int4PagePool(2, 8, records=torch.zeros(2, 8, 2559, dtype=torch.uint8))
+
+
+@pytest.mark.parametrize("structure", [_lib.PgRotaryArgs, _lib.PgInt4AppendArgs,
+                                       _lib.PgInt4DecodeArgs])
+def test_packed_arguments_have_the_structure_s_layout(structure):
+    pack = _lib.packer(structure)
+    assert pack.size == ctypes.sizeof(structure)
+    count = len(pack.unpack(bytes(pack.size)))
+    a = structure.from_buffer_copy(pack.pack(*range(1, count + 1)))
+    got = []
+    for name, _ in structure._fields_:
+        value = getattr(a, name)
+        got += list(value) if isinstance(value, ctypes.Array) else [value]
+    assert got == list(range(1, count + 1))
