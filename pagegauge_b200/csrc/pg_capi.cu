@@ -1112,7 +1112,7 @@ int32_t pg_rotary(const pg_rotary_args* a, void* stream) {
   // Whole 16-byte chunks: the vector kernel.  (49,152 tokens of 40 FP16 rows:
   // 168 us against 734 us one pair per thread.)
   const int size = a->dtype == PG_DTYPE_F32 ? 4 : 2, v = 16 / size;
-  const int table_floats = p.interleaved ? 2 : 4;
+  const int table_floats = p.interleaved && v == 4 ? 2 : 4;
   bool fast = (p.interleaved ? 2 * a->pairs : a->pairs) % v == 0 &&
               (a->head_dim - 2 * a->pairs) % v == 0 && aligned(a->cosine, 4 * table_floats) &&
               aligned(a->sine, 4 * table_floats) && a->table_stride % table_floats == 0;
@@ -1122,14 +1122,10 @@ int32_t pg_rotary(const pg_rotary_args* a, void* stream) {
             (p.x_stride_t[i] | p.x_stride_h[i] | p.y_stride_t[i] | p.y_stride_h[i]) % v == 0);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (fast) {
-    const int turning = p.interleaved ? 2 * a->pairs / v : a->pairs / v;
-    bool copies = false;
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 2; ++i)
       p.in_place[i] = p.x[i] == p.y[i] && p.x_stride_t[i] == p.y_stride_t[i] &&
                       p.x_stride_h[i] == p.y_stride_h[i];
-      copies = copies || (p.heads[i] > 0 && !p.in_place[i]);
-    }
-    p.chunks = turning + (copies ? (a->head_dim - 2 * a->pairs) / v : 0);
+    p.chunks = p.interleaved ? 2 * a->pairs / v : a->pairs / v;
     // Four rows per thread once that still fills the GPU, else one.
     const int64_t threads = a->tokens * rows * p.chunks;
     p.row_groups = static_cast<int32_t>(threads >= 148 * 2048 * 4 ? (rows + 3) / 4 : rows);
@@ -1139,13 +1135,13 @@ int32_t pg_rotary(const pg_rotary_args* a, void* stream) {
     const int block = units > 148 * 256 ? 256 : 64;
     PG_REQUIRE((units + block - 1) / block < (int64_t(1) << 31), "too many rows or tokens");
     const dim3 grid(static_cast<unsigned>((units + block - 1) / block));
-    if (a->dtype == PG_DTYPE_F16)
-      return launch_pdl(pg::pg_rotary_kernel<__half>, grid, dim3(block), 0, st, "rotary launch",
-                        p);
-    if (a->dtype == PG_DTYPE_BF16)
-      return launch_pdl(pg::pg_rotary_kernel<__nv_bfloat16>, grid, dim3(block), 0, st,
-                        "rotary launch", p);
-    return launch_pdl(pg::pg_rotary_kernel<float>, grid, dim3(block), 0, st, "rotary launch", p);
+    using Kernel = void (*)(pg::RotaryParams);
+    const Kernel kernels[3][2] = {
+        {pg::pg_rotary_kernel<__half, false>, pg::pg_rotary_kernel<__half, true>},
+        {pg::pg_rotary_kernel<__nv_bfloat16, false>, pg::pg_rotary_kernel<__nv_bfloat16, true>},
+        {pg::pg_rotary_kernel<float, false>, pg::pg_rotary_kernel<float, true>}};
+    return launch_pdl(kernels[a->dtype][p.interleaved], grid, dim3(block), 0, st,
+                      "rotary launch", p);
   }
   const int64_t total = a->tokens * rows * (a->head_dim - a->pairs);
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>((total + 255) / 256, 148 * 64)));

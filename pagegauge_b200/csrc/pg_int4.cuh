@@ -63,16 +63,23 @@ __device__ __forceinline__ float from_float<float>(float x) { return x; }
 // 8 consecutive 16-bit elements at p: one 16-byte access, or one by one
 // when rows are not 16-byte aligned.
 template <typename T, bool FAST>
-__device__ __forceinline__ void load8(const T* p, float* x) {
+__device__ __forceinline__ uint4 load8(const T* p) {
   if constexpr (FAST) {
-    const uint4 w = *reinterpret_cast<const uint4*>(p);
-    const T* e = reinterpret_cast<const T*>(&w);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_float<T>(e[i]);
+    return *reinterpret_cast<const uint4*>(p);
   } else {
+    uint4 w;
+    T* e = reinterpret_cast<T*>(&w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_float<T>(p[i]);
+    for (int i = 0; i < 8; ++i) e[i] = p[i];
+    return w;
   }
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& w, float* x) {
+  const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = to_float<T>(e[i]);
 }
 
 template <typename T, bool FAST>
@@ -100,6 +107,16 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ float min3_nan(float a, float b, float c) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 // Token tok's row of value codes: tokens 8p + 2u + e lie at row 8p + 4e + u,
 // so that the decode's reads of tokens {0, 2, 4, 6} (and {1, 3, 5, 7}) of a
@@ -110,33 +127,52 @@ __host__ __device__ constexpr int value_code_row(int tok) {
 
 // Quantise lane m's 8 dims 8m .. 8m+7 of one row (16 lanes per row; lanes
 // 4j .. 4j+3 hold group j).  Returns the 8 codes, dim 8m + i in nibble i.
+// Bound by the ALU pipe (minima, selections, logic run at half rate), so the
+// clamps are taken only by warps that need them, and rounding and packing are
+// FP32 additions: r + 1.5 2^23 has rint(r) in its low bits, and four codes
+// c0 + 16 c1 + 256 c2 + 4096 c3 are exact.  (57,304 tokens of 32 + 16 rows:
+// 321 us with a clamp, a conversion and a shift per element, 222 us so.)
 __device__ __forceinline__ uint32_t int4_quantize8(float* x, __half& scale, __half& mid) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = min_nan(max_nan(x[i], -65504.f), 65504.f);
-  float lo = x[0], hi = x[0];
-#pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    lo = min_nan(lo, x[i]);
-    hi = max_nan(hi, x[i]);
-  }
+  float lo = min3_nan(x[0], x[1], x[2]), hi = max3_nan(x[0], x[1], x[2]);
+  lo = min3_nan(min3_nan(lo, x[3], x[4]), x[5], min_nan(x[6], x[7]));
+  hi = max3_nan(max3_nan(hi, x[3], x[4]), x[5], max_nan(x[6], x[7]));
 #pragma unroll
   for (int o = 1; o < 4; o <<= 1) {
     lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
     hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  if (__any_sync(0xffffffffu, !(hi <= 65504.f && lo >= -65504.f))) {
+    lo = min_nan(max_nan(lo, -65504.f), 65504.f);
+    hi = min_nan(max_nan(hi, -65504.f), 65504.f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = min_nan(max_nan(x[i], -65504.f), 65504.f);
   }
   scale = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
   const float s = __half2float(scale);
   mid = __float2half_rn(__fadd_rn(lo, 8.f * s));
   const float m = __half2float(mid);
   const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
-  uint32_t w = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    // A NaN keeps code 0; its group's scale and midpoint are NaN.
-    const float z = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[i], m), inv)), -8.f), 7.f);
-    w |= (static_cast<uint32_t>(static_cast<int>(z) + 8) & 15u) << (4 * i);
+  for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fsub_rn(x[i], m), inv);
+  // The map is monotonic, so its extremes say whether any code needs a clamp
+  // (where the midpoint's rounding is a large part of a step, or for a NaN,
+  // which keeps code 0: its group's scale and midpoint are NaN).
+  const bool inside = __fmul_rn(__fsub_rn(lo, m), inv) >= -8.5f &&
+                      __fmul_rn(__fsub_rn(hi, m), inv) < 7.5f;
+  if (__any_sync(0xffffffffu, !inside)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = fminf(fmaxf(x[i], -8.f), 7.f);
   }
-  return w;
+  uint32_t half[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float c[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[j] = __fsub_rn(__fadd_rn(x[4 * i + j], 12582920.f), 12582912.f);
+    const float sum = fmaf(c[3], 4096.f, fmaf(c[2], 256.f, fmaf(c[1], 16.f, c[0])));
+    half[i] = __float_as_uint(__fadd_rn(sum, 8388608.f));
+  }
+  return prmt(half[0], half[1], 0x5410u);
 }
 
 struct Int4AppendParams {
@@ -164,13 +200,16 @@ struct Int4AppendParams {
   int* error_flag;
 };
 
-// Rotate lane m's 8 dims of a row (base = the row's element 0).  Half
-// layout: dims (d, d + pairs) turn together; interleaved: (2j, 2j + 1).
-// c, s: this lane's table entries (load_table8), or read here if !FAST.
+// Lane m's 8 dims of a row, rotated (raw: the row's elements 8m .. 8m + 7,
+// base: its element 0).  Half layout: dims (d, d + pairs) turn together;
+// interleaved: (2j, 2j + 1).  c, s: this lane's table entries, or read from
+// the rows here if !FAST.
 template <typename T, bool FAST>
-__device__ __forceinline__ void rotate8(float* x, const T* base, int m, int pairs,
-                                        bool interleaved, const float* c, const float* s,
-                                        const float* cos_row, const float* sin_row) {
+__device__ __forceinline__ void rotate8(float* x, const uint4& raw, const T* base, int m,
+                                        int pairs, bool interleaved, const float* c,
+                                        const float* s, const float* cos_row,
+                                        const float* sin_row) {
+  unpack8<T>(raw, x);
   if (interleaved) {
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
@@ -184,15 +223,22 @@ __device__ __forceinline__ void rotate8(float* x, const T* base, int m, int pair
     return;
   }
   if constexpr (FAST) {
-    // pairs is a multiple of 8: a lane's partner dims are one lane's.
+    // pairs is a multiple of 8: a lane's partner dims are one lane's.  The
+    // first half's lanes hold -s, so both halves add.
     const int step = pairs >> 3;
-    const int peer = m < step ? m + step : m - step;
     const bool turns = m < 2 * step;
+    const int peer = !turns ? m : m < step ? m + step : m - step;
+    uint4 other;
+    other.x = __shfl_sync(0xffffffffu, raw.x, peer, 16);
+    other.y = __shfl_sync(0xffffffffu, raw.y, peer, 16);
+    other.z = __shfl_sync(0xffffffffu, raw.z, peer, 16);
+    other.w = __shfl_sync(0xffffffffu, raw.w, peer, 16);
+    float o[8];
+    unpack8<T>(other, o);
+    if (turns) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float o = __shfl_sync(0xffffffffu, x[i], turns ? peer : m, 16);
-      const float a = __fmul_rn(x[i], c[i]), b = __fmul_rn(o, s[i]);
-      if (turns) x[i] = m < step ? __fsub_rn(a, b) : __fadd_rn(a, b);
+      for (int i = 0; i < 8; ++i)
+        x[i] = __fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(o[i], s[i]));
     }
   } else {
 #pragma unroll
@@ -252,7 +298,8 @@ __device__ __forceinline__ void subtract_center(const Int4AppendParams& p, const
                                                 const void* centers, int h, int m, float* x) {
   if (centers == nullptr) return;
   float y[8];
-  load8<T, true>(static_cast<const T*>(centers) + (k.center * p.hkv + h) * kHeadDim + 8 * m, y);
+  unpack8<T>(load8<T, true>(static_cast<const T*>(centers) +
+                            (k.center * p.hkv + h) * kHeadDim + 8 * m), y);
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = __fsub_rn(x[i], y[i]);
 }
@@ -263,7 +310,7 @@ __device__ __forceinline__ void subtract_center(const Int4AppendParams& p, const
 // table entries, slot and position are then read once per token; U = 1 with
 // a warp per row pair for few tokens, where latency is all.
 template <typename T, bool FAST, int U>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 4)
     pg_rope_append_int4_kernel(const __grid_constant__ Int4AppendParams p) {
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, half = lane >> 4, m = lane & 15;
@@ -302,7 +349,8 @@ __global__ void __launch_bounds__(256)
       const float4 a = in ? __ldg(reinterpret_cast<const float4*>(k.cos_row + j + i)) : z;
       const float4 b = in ? __ldg(reinterpret_cast<const float4*>(k.sin_row + j + i)) : z;
       c[i] = a.x; c[i + 1] = a.y; c[i + 2] = a.z; c[i + 3] = a.w;
-      s[i] = b.x; s[i + 1] = b.y; s[i + 2] = b.z; s[i + 3] = b.w;
+      const float sign = !p.interleaved && m < step ? -1.f : 1.f;
+      s[i] = sign * b.x; s[i + 1] = sign * b.y; s[i + 2] = sign * b.z; s[i + 3] = sign * b.w;
     }
   }
   const T* q = static_cast<const T*>(p.q) + k.token * p.q_stride_t;
@@ -310,18 +358,21 @@ __global__ void __launch_bounds__(256)
   const T* vr = static_cast<const T*>(p.v) + k.token * p.v_stride_t;
   T* rq = static_cast<T*>(p.rotated_q) + k.token * p.rq_stride_t;
   // Row h of two halves; an odd last row is loaded by both, stored by one.
-  auto turn_and_store = [&](float* x, const T* row, T* out, bool store) {
-    rotate8<T, FAST>(x, row, m, p.pairs, p.interleaved, c, s, k.cos_row, k.sin_row);
+  auto turn_and_store = [&](float* x, const uint4& raw, const T* row, T* out, bool store) {
+    rotate8<T, FAST>(x, raw, row, m, p.pairs, p.interleaved, c, s, k.cos_row, k.sin_row);
     // In place, other lanes' partner dims are this lane's.
     if constexpr (!FAST) __syncwarp();
     if (store) store8<T, FAST>(out + 8 * m, x);
   };
-  auto append_row = [&](float* x, bool is_key, int h, const T* row) {
+  auto append_row = [&](const uint4& raw, bool is_key, int h, const T* row) {
     const int hc = h < p.hkv ? h : p.hkv - 1;
+    float x[8];
     if (is_key)
-      turn_and_store(x, row,
+      turn_and_store(x, raw, row,
                      static_cast<T*>(p.rotated_k) + k.token * p.rk_stride_t + hc * p.rk_stride_h,
                      p.rotated_k != nullptr && h < p.hkv);
+    else
+      unpack8<T>(raw, x);
     subtract_center<T>(p, k, is_key ? p.key_center : p.value_center, hc, m, x);
     store_int4_row(p, k, is_key, h, m, x);
   };
@@ -329,44 +380,43 @@ __global__ void __launch_bounds__(256)
   if constexpr (U > 1) {
     for (int u = part; u < nq + nk; u += p.split) {
       if (u < nq) {
-        float x[U][8];
+        uint4 raw[U];
 #pragma unroll
         for (int i = 0; i < U; ++i) {
           const int h = 2 * (u * U + i) + half;
-          load8<T, FAST>(q + (h < p.hq ? h : p.hq - 1) * p.q_stride_h + 8 * m, x[i]);
+          raw[i] = load8<T, FAST>(q + (h < p.hq ? h : p.hq - 1) * p.q_stride_h + 8 * m);
         }
 #pragma unroll
         for (int i = 0; i < U; ++i) {
           const int h = 2 * (u * U + i) + half;
           if (2 * (u * U + i) >= p.hq) break;
           const int hc = h < p.hq ? h : p.hq - 1;
-          turn_and_store(x[i], q + hc * p.q_stride_h, rq + hc * p.rq_stride_h, h < p.hq);
+          float x[8];
+          turn_and_store(x, raw[i], q + hc * p.q_stride_h, rq + hc * p.rq_stride_h, h < p.hq);
         }
       } else {
         const int h = 2 * (u - nq) + half;
         const int hc = h < p.hkv ? h : p.hkv - 1;
-        float x[8], y[8];
-        load8<T, FAST>(kr + hc * p.k_stride_h + 8 * m, x);
-        load8<T, FAST>(vr + hc * p.v_stride_h + 8 * m, y);
+        const uint4 x = load8<T, FAST>(kr + hc * p.k_stride_h + 8 * m);
+        const uint4 y = load8<T, FAST>(vr + hc * p.v_stride_h + 8 * m);
         append_row(x, true, h, kr + hc * p.k_stride_h);
         append_row(y, false, h, nullptr);
       }
     }
   } else {
     for (int u = part; u < nq + 2 * nk; u += p.split) {
-      float x[8];
       if (u < nq) {
         const int h = 2 * u + half;
         const int hc = h < p.hq ? h : p.hq - 1;
-        load8<T, FAST>(q + hc * p.q_stride_h + 8 * m, x);
-        turn_and_store(x, q + hc * p.q_stride_h, rq + hc * p.rq_stride_h, h < p.hq);
+        float x[8];
+        turn_and_store(x, load8<T, FAST>(q + hc * p.q_stride_h + 8 * m), q + hc * p.q_stride_h,
+                       rq + hc * p.rq_stride_h, h < p.hq);
       } else {
         const bool is_key = u < nq + nk;
         const int h = 2 * (u - nq - (is_key ? 0 : nk)) + half;
         const int hc = h < p.hkv ? h : p.hkv - 1;
         const T* row = is_key ? kr + hc * p.k_stride_h : vr + hc * p.v_stride_h;
-        load8<T, FAST>(row + 8 * m, x);
-        append_row(x, is_key, h, row);
+        append_row(load8<T, FAST>(row + 8 * m), is_key, h, row);
       }
     }
   }
@@ -419,9 +469,13 @@ __global__ void __launch_bounds__(256)
     T* out = static_cast<T*>(kv == 0 ? p.key : p.value) + th * kHeadDim + 8 * m;
     float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float z = static_cast<float>(static_cast<int>((codes[kv] >> (4 * i)) & 15u) - 8);
-      x[i] = __fadd_rn(__fmul_rn(z, s[kv]), mid[kv]);
+    for (int i = 0; i < 4; ++i) {
+      // Nibbles i and i + 4 as the halves 1024 + z, less 1032 (exact).
+      const uint32_t w = ((codes[kv] >> (4 * i)) & 0x000f000fu) | 0x64006400u;
+      const uint32_t z = hsub2_u32(w, 0x64086408u);
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&z));
+      x[i] = __fadd_rn(__fmul_rn(f.x, s[kv]), mid[kv]);
+      x[i + 4] = __fadd_rn(__fmul_rn(f.y, s[kv]), mid[kv]);
     }
     if constexpr (sizeof(T) == 2) {
       store8<T, true>(out, x);

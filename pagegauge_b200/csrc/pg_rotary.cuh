@@ -23,25 +23,25 @@ struct RotaryParams {
   const int32_t* positions;
   int* error_flag;
   // pg_rotary_kernel only:
-  int32_t chunks;       // 16-byte units of a row that a thread takes
+  int32_t chunks;       // turning 16-byte chunks of a row, one per thread
   int32_t row_groups;   // threads that share a chunk over a token's rows
   int32_t in_place[2];  // the dims past the pairs are there already
 };
 
 // Rows that are 16-byte aligned and whose parts are whole 16-byte chunks.  A
-// thread takes one chunk (half layout: of both halves) of every
-// row_groups-th row of one token, so it reads its table entries once, and
-// requests four rows before it uses the first.  Bound by HBM: each row is
-// read and written once.
-template <typename T>
-__global__ void __launch_bounds__(256)
+// thread takes one turning chunk (half layout: of both halves) of every
+// row_groups-th row of one token, so it reads its table entries once, and the
+// rows' copied chunks with it, U rows requested before the first is used.
+// Bound by HBM: each row is read and written once.
+template <typename T, bool INTERLEAVED>
+__global__ void __launch_bounds__(256, 4)
     pg_rotary_kernel(const __grid_constant__ RotaryParams p) {
-  constexpr int V = 16 / sizeof(T), U = 4;
+  constexpr int V = 16 / sizeof(T), U = INTERLEAVED ? 4 : 2;
+  constexpr int E = INTERLEAVED ? V / 2 : V;  // table entries of a chunk
   pdl_launch_dependents();
   pdl_wait_primary();
   const int per_token = p.chunks * p.row_groups;
   const int rows = p.heads[0] + p.heads[1];
-  const int turning = p.interleaved ? 2 * p.pairs / V : p.pairs / V;
   const int64_t u = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   // A 32-bit division where the index allows it.
   const int64_t token = u < (int64_t(1) << 31)
@@ -56,77 +56,75 @@ __global__ void __launch_bounds__(256)
     record_error(p.error_flag, kDevBadPosition);
     return;
   }
-  const bool turns = chunk < turning;
-  // Element offsets of the thread's one or two vectors, and its entries.
-  const int da = !turns ? 2 * p.pairs + (chunk - turning) * V : chunk * V;
-  const int db = p.interleaved ? da : da + p.pairs;
-  const bool two = turns && !p.interleaved;
-  float c[V], s[V];
-  if (turns) {
-    const float* cr = p.cos + pos * p.table_stride;
-    const float* sr = p.sin + pos * p.table_stride;
-    if (p.interleaved) {
+  float c[E], s[E];
+  {
+    const float* cr = p.cos + pos * p.table_stride + chunk * E;
+    const float* sr = p.sin + pos * p.table_stride + chunk * E;
+    constexpr int W = E >= 4 ? 4 : 2;
 #pragma unroll
-      for (int i = 0; i < V / 2; i += 2) {
-        const float2 a = __ldg(reinterpret_cast<const float2*>(cr + chunk * (V / 2) + i));
-        const float2 b = __ldg(reinterpret_cast<const float2*>(sr + chunk * (V / 2) + i));
-        c[i] = a.x; c[i + 1] = a.y;
-        s[i] = b.x * p.sign; s[i + 1] = b.y * p.sign;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; i += 4) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(cr + chunk * V + i));
-        const float4 b = __ldg(reinterpret_cast<const float4*>(sr + chunk * V + i));
+    for (int i = 0; i < E; i += W) {
+      if constexpr (W == 4) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(cr + i));
+        const float4 b = __ldg(reinterpret_cast<const float4*>(sr + i));
         c[i] = a.x; c[i + 1] = a.y; c[i + 2] = a.z; c[i + 3] = a.w;
-        s[i] = b.x * p.sign; s[i + 1] = b.y * p.sign;
-        s[i + 2] = b.z * p.sign; s[i + 3] = b.w * p.sign;
+        s[i] = b.x; s[i + 1] = b.y; s[i + 2] = b.z; s[i + 3] = b.w;
+      } else {
+        const float2 a = __ldg(reinterpret_cast<const float2*>(cr + i));
+        const float2 b = __ldg(reinterpret_cast<const float2*>(sr + i));
+        c[i] = a.x; c[i + 1] = a.y;
+        s[i] = b.x; s[i + 1] = b.y;
       }
     }
+#pragma unroll
+    for (int i = 0; i < E; ++i) s[i] *= p.sign;
   }
+  const T* xq = static_cast<const T*>(p.x[0]) + token * p.x_stride_t[0];
+  const T* xk = static_cast<const T*>(p.x[1]) + token * p.x_stride_t[1];
+  T* yq = static_cast<T*>(p.y[0]) + token * p.y_stride_t[0];
+  T* yk = static_cast<T*>(p.y[1]) + token * p.y_stride_t[1];
+  const int copied = (p.head_dim - 2 * p.pairs) / V;
   for (int r0 = group; r0 < rows; r0 += U * p.row_groups) {
+    const T* x[U];
+    T* y[U];
+    bool copies[U];
     uint4 a[U], b[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int row = r0 + i * p.row_groups;
-      if (row >= rows) break;
-      const int which = row < p.heads[0] ? 0 : 1;
-      const int h = which == 0 ? row : row - p.heads[0];
-      const T* x = static_cast<const T*>(p.x[which]) + token * p.x_stride_t[which] +
-                   h * p.x_stride_h[which];
-      a[i] = *reinterpret_cast<const uint4*>(x + da);
-      if (two) b[i] = *reinterpret_cast<const uint4*>(x + db);
+      const bool is_q = row < p.heads[0];
+      const int h = is_q ? row : row - p.heads[0];
+      x[i] = is_q ? xq + h * p.x_stride_h[0] : xk + h * p.x_stride_h[1];
+      y[i] = is_q ? yq + h * p.y_stride_h[0] : yk + h * p.y_stride_h[1];
+      copies[i] = row < rows && !(is_q ? p.in_place[0] : p.in_place[1]);
+      if (row < rows) {
+        a[i] = *reinterpret_cast<const uint4*>(x[i] + chunk * V);
+        if constexpr (!INTERLEAVED)
+          b[i] = *reinterpret_cast<const uint4*>(x[i] + chunk * V + p.pairs);
+      }
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int row = r0 + i * p.row_groups;
-      if (row >= rows) break;
-      const int which = row < p.heads[0] ? 0 : 1;
-      const int h = which == 0 ? row : row - p.heads[0];
-      T* y = static_cast<T*>(p.y[which]) + token * p.y_stride_t[which] +
-             h * p.y_stride_h[which];
+      if (r0 + i * p.row_groups >= rows) break;
       T* ea = reinterpret_cast<T*>(&a[i]);
-      if (two) {
-        T* eb = reinterpret_cast<T*>(&b[i]);
+      T* eb = reinterpret_cast<T*>(&b[i]);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float xa = to_float<T>(ea[e]), xb = to_float<T>(eb[e]);
-          ea[e] = from_float<T>(__fsub_rn(__fmul_rn(xa, c[e]), __fmul_rn(xb, s[e])));
-          eb[e] = from_float<T>(__fadd_rn(__fmul_rn(xb, c[e]), __fmul_rn(xa, s[e])));
-        }
-        *reinterpret_cast<uint4*>(y + db) = b[i];
-      } else if (turns) {
-#pragma unroll
-        for (int e = 0; e < V; e += 2) {
-          const float xa = to_float<T>(ea[e]), xb = to_float<T>(ea[e + 1]);
-          const float ce = c[e / 2], se = s[e / 2];
-          ea[e] = from_float<T>(__fsub_rn(__fmul_rn(xa, ce), __fmul_rn(xb, se)));
-          ea[e + 1] = from_float<T>(__fadd_rn(__fmul_rn(xb, ce), __fmul_rn(xa, se)));
-        }
-      } else if (p.in_place[which]) {
-        continue;
+      for (int e = 0; e < E; ++e) {
+        T& ta = INTERLEAVED ? ea[2 * e] : ea[e];
+        T& tb = INTERLEAVED ? ea[2 * e + 1] : eb[e];
+        const float xa = to_float<T>(ta), xb = to_float<T>(tb);
+        ta = from_float<T>(__fsub_rn(__fmul_rn(xa, c[e]), __fmul_rn(xb, s[e])));
+        tb = from_float<T>(__fadd_rn(__fmul_rn(xb, c[e]), __fmul_rn(xa, s[e])));
       }
-      *reinterpret_cast<uint4*>(y + da) = a[i];
+      *reinterpret_cast<uint4*>(y[i] + chunk * V) = a[i];
+      if constexpr (!INTERLEAVED) *reinterpret_cast<uint4*>(y[i] + chunk * V + p.pairs) = b[i];
+    }
+    for (int d = chunk; d < copied; d += p.chunks) {
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (copies[i]) a[i] = *reinterpret_cast<const uint4*>(x[i] + 2 * p.pairs + d * V);
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (copies[i]) *reinterpret_cast<uint4*>(y[i] + 2 * p.pairs + d * V) = a[i];
     }
   }
 }
