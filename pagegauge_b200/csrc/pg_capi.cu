@@ -1087,10 +1087,14 @@ int32_t pg_rotary(const pg_rotary_args* a, void* stream) {
     if (p.heads[i] > 0) PG_REQUIRE(a->y[i] != nullptr, "rotated rows need an output");
     p.x[i] = a->x[i];
     p.y[i] = a->y[i];
+    for (const int64_t stride : {a->x_stride_h[i], a->y_stride_h[i]})
+      PG_REQUIRE(p.heads[i] == 0 || (stride >= 0 && p.heads[i] * stride < (int64_t(1) << 31)),
+                 "head strides must be non-negative and the heads of a token within 2^31 "
+                 "elements");
     p.x_stride_t[i] = a->x_stride_t[i];
-    p.x_stride_h[i] = a->x_stride_h[i];
+    p.x_stride_h[i] = static_cast<int32_t>(a->x_stride_h[i]);
     p.y_stride_t[i] = a->y_stride_t[i];
-    p.y_stride_h[i] = a->y_stride_h[i];
+    p.y_stride_h[i] = static_cast<int32_t>(a->y_stride_h[i]);
     rows += p.heads[i];
   }
   if (a->tokens == 0 || rows == 0) return PG_OK;
@@ -1177,22 +1181,28 @@ int32_t pg_rope_append_int4(const pg_int4_append_args* a, void* stream) {
              "rows, tables, positions, slots and records are required");
   PG_REQUIRE(aligned(a->records, 16) && aligned(a->key_center, 16) && aligned(a->value_center, 16),
              "records and centres must be 16-byte aligned");
+  const int64_t head_stride[5] = {a->q_stride_h, a->rq_stride_h, a->k_stride_h, a->v_stride_h,
+                                  a->rotated_key == nullptr ? 0 : a->rk_stride_h};
+  for (int i = 0; i < 5; ++i)
+    PG_REQUIRE(head_stride[i] >= 0 && (i < 2 ? a->query_heads : a->kv_heads) * head_stride[i] <
+                                          (int64_t(1) << 31),
+               "head strides must be non-negative and the heads of a token within 2^31 elements");
   pg::Int4AppendParams p{};
   p.q = a->query;
   p.k = a->key;
   p.v = a->value;
   p.q_stride_t = a->q_stride_t;
-  p.q_stride_h = a->q_stride_h;
+  p.q_stride_h = static_cast<int32_t>(a->q_stride_h);
   p.k_stride_t = a->k_stride_t;
-  p.k_stride_h = a->k_stride_h;
+  p.k_stride_h = static_cast<int32_t>(a->k_stride_h);
   p.v_stride_t = a->v_stride_t;
-  p.v_stride_h = a->v_stride_h;
+  p.v_stride_h = static_cast<int32_t>(a->v_stride_h);
   p.rotated_q = a->rotated_query;
   p.rotated_k = a->rotated_key;
   p.rq_stride_t = a->rq_stride_t;
-  p.rq_stride_h = a->rq_stride_h;
+  p.rq_stride_h = static_cast<int32_t>(a->rq_stride_h);
   p.rk_stride_t = a->rk_stride_t;
-  p.rk_stride_h = a->rk_stride_h;
+  p.rk_stride_h = static_cast<int32_t>(head_stride[4]);
   p.cos = a->cosine;
   p.sin = a->sine;
   p.table_stride = a->table_stride;

@@ -96,6 +96,23 @@ __device__ __forceinline__ void store8(T* p, const float* x) {
   }
 }
 
+// Two FP32 operations in one instruction.  A sum of products in this form may
+// be contracted, so no product of it feeds a sum of it.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 // Minimum and maximum that keep a NaN, so that one shows in what is read.
 __device__ __forceinline__ float min_nan(float a, float b) {
   float r;
@@ -153,7 +170,12 @@ __device__ __forceinline__ uint32_t int4_quantize8(float* x, __half& scale, __ha
   const float m = __half2float(mid);
   const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fsub_rn(x[i], m), inv);
+  for (int i = 0; i < 8; i += 2) {
+    const float2 r = mul2(add2(make_float2(x[i], x[i + 1]), make_float2(-m, -m)),
+                          make_float2(inv, inv));
+    x[i] = r.x;
+    x[i + 1] = r.y;
+  }
   // The map is monotonic, so its extremes say whether any code needs a clamp
   // (where the midpoint's rounding is a large part of a step, or for a NaN,
   // which keeps code 0: its group's scale and midpoint are NaN).
@@ -168,7 +190,13 @@ __device__ __forceinline__ uint32_t int4_quantize8(float* x, __half& scale, __ha
   for (int i = 0; i < 2; ++i) {
     float c[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) c[j] = __fsub_rn(__fadd_rn(x[4 * i + j], 12582920.f), 12582912.f);
+    for (int j = 0; j < 4; j += 2) {
+      const float2 r = add2(make_float2(__fadd_rn(x[4 * i + j], 12582920.f),
+                                        __fadd_rn(x[4 * i + j + 1], 12582920.f)),
+                            make_float2(-12582912.f, -12582912.f));
+      c[j] = r.x;
+      c[j + 1] = r.y;
+    }
     const float sum = fmaf(c[3], 4096.f, fmaf(c[2], 256.f, fmaf(c[1], 16.f, c[0])));
     half[i] = __float_as_uint(__fadd_rn(sum, 8388608.f));
   }
@@ -179,10 +207,12 @@ struct Int4AppendParams {
   const void* q;
   const void* k;
   const void* v;
-  int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+  int64_t q_stride_t, k_stride_t, v_stride_t;
   void* rotated_q;  // [T, Hq, 128]
   void* rotated_k;  // [T, Hkv, 128] or null
-  int64_t rq_stride_t, rq_stride_h, rk_stride_t, rk_stride_h;
+  int64_t rq_stride_t, rk_stride_t;
+  // Heads times these stay below 2^31.
+  int32_t q_stride_h, k_stride_h, v_stride_h, rq_stride_h, rk_stride_h;
   const float* cos;  // [table_rows, pairs]
   const float* sin;
   int64_t table_stride, table_rows;
@@ -237,8 +267,13 @@ __device__ __forceinline__ void rotate8(float* x, const uint4& raw, const T* bas
     unpack8<T>(other, o);
     if (turns) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        x[i] = __fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(o[i], s[i]));
+      for (int i = 0; i < 8; i += 2) {
+        const float2 r = add2(
+            make_float2(__fmul_rn(x[i], c[i]), __fmul_rn(x[i + 1], c[i + 1])),
+            make_float2(__fmul_rn(o[i], s[i]), __fmul_rn(o[i + 1], s[i + 1])));
+        x[i] = r.x;
+        x[i + 1] = r.y;
+      }
     }
   } else {
 #pragma unroll
@@ -301,7 +336,11 @@ __device__ __forceinline__ void subtract_center(const Int4AppendParams& p, const
   unpack8<T>(load8<T, true>(static_cast<const T*>(centers) +
                             (k.center * p.hkv + h) * kHeadDim + 8 * m), y);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = __fsub_rn(x[i], y[i]);
+  for (int i = 0; i < 8; i += 2) {
+    const float2 r = add2(make_float2(x[i], x[i + 1]), make_float2(-y[i], -y[i + 1]));
+    x[i] = r.x;
+    x[i + 1] = r.y;
+  }
 }
 
 // `split` warps share one token.  A warp takes two rows at a time (16 lanes of
@@ -316,13 +355,25 @@ __global__ void __launch_bounds__(256, 4)
   const int lane = threadIdx.x & 31, half = lane >> 4, m = lane & 15;
   const int64_t w = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
   Int4Token k;
-  k.token = w / p.split;
+  k.token = p.split == 1 ? w : static_cast<uint32_t>(w) / p.split;  // w is small if split
   const int part = static_cast<int>(w - k.token * p.split);
   if (k.token >= p.tokens) return;
   pdl_wait_primary();
   const int slot = p.slots[k.token];
   const int pos = p.positions[k.token];
   k.center = p.center_rows != nullptr ? p.center_rows[k.token] : 0;
+  // The first query rows are asked for along with the token's indices.
+  const T* q = static_cast<const T*>(p.q) + k.token * p.q_stride_t + 8 * m;
+  const int nq = (p.hq + 2 * U - 1) / (2 * U), nk = (p.hkv + 1) >> 1;
+  uint4 raw[U];
+  auto load_queries = [&](int u) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int h = 2 * (u * U + i) + half;
+      raw[i] = load8<T, FAST>(q + (h < p.hq ? h : p.hq - 1) * p.q_stride_h);
+    }
+  };
+  if (part < nq) load_queries(part);
   if (slot < 0) return;
   k.page = slot >> 4;
   k.tok = slot & 15;
@@ -353,7 +404,6 @@ __global__ void __launch_bounds__(256, 4)
       s[i] = sign * b.x; s[i + 1] = sign * b.y; s[i + 2] = sign * b.z; s[i + 3] = sign * b.w;
     }
   }
-  const T* q = static_cast<const T*>(p.q) + k.token * p.q_stride_t;
   const T* kr = static_cast<const T*>(p.k) + k.token * p.k_stride_t;
   const T* vr = static_cast<const T*>(p.v) + k.token * p.v_stride_t;
   T* rq = static_cast<T*>(p.rotated_q) + k.token * p.rq_stride_t;
@@ -376,48 +426,35 @@ __global__ void __launch_bounds__(256, 4)
     subtract_center<T>(p, k, is_key ? p.key_center : p.value_center, hc, m, x);
     store_int4_row(p, k, is_key, h, m, x);
   };
-  const int nq = (p.hq + 2 * U - 1) / (2 * U), nk = (p.hkv + 1) >> 1;
+  for (int u = part; u < nq; u += p.split) {
+    if (u != part) load_queries(u);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int h = 2 * (u * U + i) + half;
+      if (2 * (u * U + i) >= p.hq) break;
+      const int hc = h < p.hq ? h : p.hq - 1;
+      float x[8];
+      turn_and_store(x, raw[i], q - 8 * m + hc * p.q_stride_h, rq + hc * p.rq_stride_h, h < p.hq);
+    }
+  }
+  // This warp's first unit past the query rows.
+  const int first = part >= nq ? part - nq : (p.split - (nq - part) % p.split) % p.split;
   if constexpr (U > 1) {
-    for (int u = part; u < nq + nk; u += p.split) {
-      if (u < nq) {
-        uint4 raw[U];
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-          const int h = 2 * (u * U + i) + half;
-          raw[i] = load8<T, FAST>(q + (h < p.hq ? h : p.hq - 1) * p.q_stride_h + 8 * m);
-        }
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-          const int h = 2 * (u * U + i) + half;
-          if (2 * (u * U + i) >= p.hq) break;
-          const int hc = h < p.hq ? h : p.hq - 1;
-          float x[8];
-          turn_and_store(x, raw[i], q + hc * p.q_stride_h, rq + hc * p.rq_stride_h, h < p.hq);
-        }
-      } else {
-        const int h = 2 * (u - nq) + half;
-        const int hc = h < p.hkv ? h : p.hkv - 1;
-        const uint4 x = load8<T, FAST>(kr + hc * p.k_stride_h + 8 * m);
-        const uint4 y = load8<T, FAST>(vr + hc * p.v_stride_h + 8 * m);
-        append_row(x, true, h, kr + hc * p.k_stride_h);
-        append_row(y, false, h, nullptr);
-      }
+    for (int u = first; u < nk; u += p.split) {
+      const int h = 2 * u + half;
+      const int hc = h < p.hkv ? h : p.hkv - 1;
+      const uint4 x = load8<T, FAST>(kr + hc * p.k_stride_h + 8 * m);
+      const uint4 y = load8<T, FAST>(vr + hc * p.v_stride_h + 8 * m);
+      append_row(x, true, h, kr + hc * p.k_stride_h);
+      append_row(y, false, h, nullptr);
     }
   } else {
-    for (int u = part; u < nq + 2 * nk; u += p.split) {
-      if (u < nq) {
-        const int h = 2 * u + half;
-        const int hc = h < p.hq ? h : p.hq - 1;
-        float x[8];
-        turn_and_store(x, load8<T, FAST>(q + hc * p.q_stride_h + 8 * m), q + hc * p.q_stride_h,
-                       rq + hc * p.rq_stride_h, h < p.hq);
-      } else {
-        const bool is_key = u < nq + nk;
-        const int h = 2 * (u - nq - (is_key ? 0 : nk)) + half;
-        const int hc = h < p.hkv ? h : p.hkv - 1;
-        const T* row = is_key ? kr + hc * p.k_stride_h : vr + hc * p.v_stride_h;
-        append_row(load8<T, FAST>(row + 8 * m), is_key, h, row);
-      }
+    for (int u = first; u < 2 * nk; u += p.split) {
+      const bool is_key = u < nk;
+      const int h = 2 * (u - (is_key ? 0 : nk)) + half;
+      const int hc = h < p.hkv ? h : p.hkv - 1;
+      const T* row = is_key ? kr + hc * p.k_stride_h : vr + hc * p.v_stride_h;
+      append_row(load8<T, FAST>(row + 8 * m), is_key, h, row);
     }
   }
 }
@@ -442,7 +479,10 @@ __global__ void __launch_bounds__(256)
   pdl_wait_primary();
   const int m = threadIdx.x & 15, grp = m >> 2;
   const int64_t th = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 4;
-  const int64_t token = th / p.hkv;
+  // A 32-bit division where the index allows it.
+  const int64_t token = th < (int64_t(1) << 31)
+                            ? static_cast<int64_t>(static_cast<uint32_t>(th) / p.hkv)
+                            : th / p.hkv;
   if (token >= p.tokens) return;
   const int h = static_cast<int>(th - token * p.hkv);
   const int slot = p.slots[token];

@@ -12,7 +12,8 @@ namespace pg {
 struct RotaryParams {
   const void* x[2];  // query rows, key rows (or null)
   void* y[2];
-  int64_t x_stride_t[2], x_stride_h[2], y_stride_t[2], y_stride_h[2];
+  int64_t x_stride_t[2], y_stride_t[2];
+  int32_t x_stride_h[2], y_stride_h[2];  // heads times these stay below 2^31
   int32_t heads[2];
   int64_t tokens;
   int32_t head_dim, pairs, interleaved;
@@ -52,6 +53,22 @@ __global__ void __launch_bounds__(256, 4)
   const int group = rest / p.chunks;
   const int chunk = rest - group * p.chunks;
   const int pos = p.positions[token];
+  const T* xq = static_cast<const T*>(p.x[0]) + token * p.x_stride_t[0] + chunk * V;
+  const T* xk = static_cast<const T*>(p.x[1]) + token * p.x_stride_t[1] + chunk * V;
+  uint4 a[U], b[U];
+  auto load_rows = [&](int r0) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int row = r0 + i * p.row_groups;
+      if (row >= rows) continue;
+      const T* x = row < p.heads[0] ? xq + row * p.x_stride_h[0]
+                                    : xk + (row - p.heads[0]) * p.x_stride_h[1];
+      a[i] = *reinterpret_cast<const uint4*>(x);
+      if constexpr (!INTERLEAVED) b[i] = *reinterpret_cast<const uint4*>(x + p.pairs);
+    }
+  };
+  // The first rows are asked for along with the position.
+  load_rows(group);
   if (pos < 0 || pos >= p.table_rows) {
     record_error(p.error_flag, kDevBadPosition);
     return;
@@ -64,44 +81,28 @@ __global__ void __launch_bounds__(256, 4)
 #pragma unroll
     for (int i = 0; i < E; i += W) {
       if constexpr (W == 4) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(cr + i));
-        const float4 b = __ldg(reinterpret_cast<const float4*>(sr + i));
-        c[i] = a.x; c[i + 1] = a.y; c[i + 2] = a.z; c[i + 3] = a.w;
-        s[i] = b.x; s[i + 1] = b.y; s[i + 2] = b.z; s[i + 3] = b.w;
+        const float4 u4 = __ldg(reinterpret_cast<const float4*>(cr + i));
+        const float4 v4 = __ldg(reinterpret_cast<const float4*>(sr + i));
+        c[i] = u4.x; c[i + 1] = u4.y; c[i + 2] = u4.z; c[i + 3] = u4.w;
+        s[i] = v4.x; s[i + 1] = v4.y; s[i + 2] = v4.z; s[i + 3] = v4.w;
       } else {
-        const float2 a = __ldg(reinterpret_cast<const float2*>(cr + i));
-        const float2 b = __ldg(reinterpret_cast<const float2*>(sr + i));
-        c[i] = a.x; c[i + 1] = a.y;
-        s[i] = b.x; s[i + 1] = b.y;
+        const float2 u2 = __ldg(reinterpret_cast<const float2*>(cr + i));
+        const float2 v2 = __ldg(reinterpret_cast<const float2*>(sr + i));
+        c[i] = u2.x; c[i + 1] = u2.y;
+        s[i] = v2.x; s[i + 1] = v2.y;
       }
     }
 #pragma unroll
     for (int i = 0; i < E; ++i) s[i] *= p.sign;
   }
-  const T* xq = static_cast<const T*>(p.x[0]) + token * p.x_stride_t[0];
-  const T* xk = static_cast<const T*>(p.x[1]) + token * p.x_stride_t[1];
-  T* yq = static_cast<T*>(p.y[0]) + token * p.y_stride_t[0];
-  T* yk = static_cast<T*>(p.y[1]) + token * p.y_stride_t[1];
+  T* yq = static_cast<T*>(p.y[0]) + token * p.y_stride_t[0] + chunk * V;
+  T* yk = static_cast<T*>(p.y[1]) + token * p.y_stride_t[1] + chunk * V;
+  // The copied chunks d = chunk, chunk + chunks, ... of a row start here,
+  // relative to its turning chunk.
+  const int tail = 2 * p.pairs;
   const int copied = (p.head_dim - 2 * p.pairs) / V;
   for (int r0 = group; r0 < rows; r0 += U * p.row_groups) {
-    const T* x[U];
-    T* y[U];
-    bool copies[U];
-    uint4 a[U], b[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int row = r0 + i * p.row_groups;
-      const bool is_q = row < p.heads[0];
-      const int h = is_q ? row : row - p.heads[0];
-      x[i] = is_q ? xq + h * p.x_stride_h[0] : xk + h * p.x_stride_h[1];
-      y[i] = is_q ? yq + h * p.y_stride_h[0] : yk + h * p.y_stride_h[1];
-      copies[i] = row < rows && !(is_q ? p.in_place[0] : p.in_place[1]);
-      if (row < rows) {
-        a[i] = *reinterpret_cast<const uint4*>(x[i] + chunk * V);
-        if constexpr (!INTERLEAVED)
-          b[i] = *reinterpret_cast<const uint4*>(x[i] + chunk * V + p.pairs);
-      }
-    }
+    if (r0 != group) load_rows(r0);
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       if (r0 + i * p.row_groups >= rows) break;
@@ -115,16 +116,29 @@ __global__ void __launch_bounds__(256, 4)
         ta = from_float<T>(__fsub_rn(__fmul_rn(xa, c[e]), __fmul_rn(xb, s[e])));
         tb = from_float<T>(__fadd_rn(__fmul_rn(xb, c[e]), __fmul_rn(xa, s[e])));
       }
-      *reinterpret_cast<uint4*>(y[i] + chunk * V) = a[i];
-      if constexpr (!INTERLEAVED) *reinterpret_cast<uint4*>(y[i] + chunk * V + p.pairs) = b[i];
+      T* y = r0 + i * p.row_groups < p.heads[0]
+                 ? yq + (r0 + i * p.row_groups) * p.y_stride_h[0]
+                 : yk + (r0 + i * p.row_groups - p.heads[0]) * p.y_stride_h[1];
+      *reinterpret_cast<uint4*>(y) = a[i];
+      if constexpr (!INTERLEAVED) *reinterpret_cast<uint4*>(y + p.pairs) = b[i];
     }
     for (int d = chunk; d < copied; d += p.chunks) {
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (copies[i]) a[i] = *reinterpret_cast<const uint4*>(x[i] + 2 * p.pairs + d * V);
+      for (int i = 0; i < U; ++i) {
+        const int row = r0 + i * p.row_groups;
+        if (row >= rows) continue;
+        const T* x = row < p.heads[0] ? xq + row * p.x_stride_h[0]
+                                      : xk + (row - p.heads[0]) * p.x_stride_h[1];
+        a[i] = *reinterpret_cast<const uint4*>(x + tail + (d - chunk) * V);
+      }
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (copies[i]) *reinterpret_cast<uint4*>(y[i] + 2 * p.pairs + d * V) = a[i];
+      for (int i = 0; i < U; ++i) {
+        const int row = r0 + i * p.row_groups;
+        const bool is_q = row < p.heads[0];
+        if (row >= rows || (is_q ? p.in_place[0] : p.in_place[1])) continue;
+        T* y = is_q ? yq + row * p.y_stride_h[0] : yk + (row - p.heads[0]) * p.y_stride_h[1];
+        *reinterpret_cast<uint4*>(y + tail + (d - chunk) * V) = a[i];
+      }
     }
   }
 }
