@@ -1278,17 +1278,19 @@ int32_t pg_int4_read(const void* records, int64_t num_pages, int32_t kv_heads,
   p.key = key;
   p.value = value;
   p.error_flag = device_error_ptr();
-  const int64_t rows = tokens * kv_heads;
-  PG_REQUIRE((rows + 15) / 16 < (int64_t(1) << 31), "too many tokens");
-  const dim3 grid(static_cast<unsigned>((rows + 15) / 16));
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == PG_DTYPE_F16)
-    return launch_pdl(pg::pg_int4_read_kernel<__half>, grid, dim3(256), 0, st, "int4 read launch",
-                      p);
-  if (dtype == PG_DTYPE_BF16)
-    return launch_pdl(pg::pg_int4_read_kernel<__nv_bfloat16>, grid, dim3(256), 0, st,
-                      "int4 read launch", p);
-  return launch_pdl(pg::pg_int4_read_kernel<float>, grid, dim3(256), 0, st, "int4 read launch", p);
+  const bool wide = tokens * kv_heads > 148 * 64;
+  p.split = wide ? (kv_heads + 7) / 8 : (kv_heads + 1) / 2;
+  const int64_t warps = tokens * p.split;
+  PG_REQUIRE((warps + 7) / 8 < (int64_t(1) << 31), "too many tokens");
+  const int block = wide ? 8 : 2;
+  const dim3 grid(static_cast<unsigned>((warps + block - 1) / block));
+  using Kernel = void (*)(pg::Int4ReadParams);
+  const Kernel kernels[3][2] = {
+      {pg::pg_int4_read_kernel<__half, 1>, pg::pg_int4_read_kernel<__half, 4>},
+      {pg::pg_int4_read_kernel<__nv_bfloat16, 1>, pg::pg_int4_read_kernel<__nv_bfloat16, 4>},
+      {pg::pg_int4_read_kernel<float, 1>, pg::pg_int4_read_kernel<float, 4>}};
+  return launch_pdl(kernels[dtype][wide], grid, dim3(block * 32), 0,
+                    static_cast<cudaStream_t>(stream), "int4 read launch", p);
 }
 
 int32_t pg_decode_int4_run(const pg_int4_decode_args* a, void* stream) {

@@ -465,63 +465,85 @@ struct Int4ReadParams {
   const int32_t* slots;
   int64_t tokens;
   int32_t hkv;
-  void* key;    // [T, Hkv, 128]
-  void* value;  // [T, Hkv, 128]
+  int32_t split;  // warps that share one token's heads
+  void* key;      // [T, Hkv, 128]
+  void* value;    // [T, Hkv, 128]
   int* error_flag;
 };
 
-// 16 lanes per (token, head): the key row and the value row; skipped slots
-// read as zeros.
-template <typename T>
+// One warp per token and 2 U KV heads (16 lanes per head's key and value row),
+// with everything requested before it is used; skipped slots read as zeros.
+// U = 4 where tokens alone fill the GPU, as in the append.
+template <typename T, int U>
 __global__ void __launch_bounds__(256)
     pg_int4_read_kernel(const __grid_constant__ Int4ReadParams p) {
   pdl_launch_dependents();
-  pdl_wait_primary();
-  const int m = threadIdx.x & 15, grp = m >> 2;
-  const int64_t th = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 4;
+  const int lane = threadIdx.x & 31, half = lane >> 4, m = lane & 15, grp = m >> 2;
+  const int64_t w = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
   // A 32-bit division where the index allows it.
-  const int64_t token = th < (int64_t(1) << 31)
-                            ? static_cast<int64_t>(static_cast<uint32_t>(th) / p.hkv)
-                            : th / p.hkv;
+  const int64_t token = w < (int64_t(1) << 31)
+                            ? static_cast<int64_t>(static_cast<uint32_t>(w) / p.split)
+                            : w / p.split;
   if (token >= p.tokens) return;
-  const int h = static_cast<int>(th - token * p.hkv);
+  const int h0 = 2 * U * static_cast<int>(w - token * p.split) + half;
+  pdl_wait_primary();
   const int slot = p.slots[token];
-  uint32_t codes[2] = {0x88888888u, 0x88888888u};
-  float s[2] = {0.f, 0.f}, mid[2] = {0.f, 0.f};
-  if (slot >= 0 && (slot >> 4) >= p.num_pages) {
-    record_error(p.error_flag, kDevBadPageId);
-  } else if (slot >= 0) {
-    const int tok = slot & 15;
-    const uint8_t* rec = p.records + (static_cast<int64_t>(slot >> 4) * p.hkv + h) * kInt4Record;
-    codes[0] = *reinterpret_cast<const uint32_t*>(rec + tok * 64 + (m & 3) * 16 + grp * 4);
-    const uint8_t* vr = rec + kInt4Value + value_code_row(tok) * 64 + (m & 3) * 16 + grp * 2;
-    codes[1] = *reinterpret_cast<const uint16_t*>(vr) |
-               (static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(vr + 8)) << 16);
-    const __half* km = reinterpret_cast<const __half*>(rec + kInt4KeyMeta + tok * 16) + grp;
-    const __half* vm = reinterpret_cast<const __half*>(rec + kInt4ValueMeta + tok * 16) + grp;
-    s[0] = __half2float(km[0]);
-    mid[0] = __half2float(km[4]);
-    s[1] = __half2float(vm[0]);
-    mid[1] = __half2float(vm[4]);
+  const bool held = slot >= 0 && (slot >> 4) < p.num_pages;
+  if (slot >= 0 && !held) record_error(p.error_flag, kDevBadPageId);
+  uint32_t codes[U][2];
+  __half s[U][2], mid[U][2];
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      codes[i][kv] = 0u;
+      s[i][kv] = mid[i][kv] = __ushort_as_half(0);
+    }
+    const int h = h0 + 2 * i;
+    if (held && h < p.hkv) {
+      const int tok = slot & 15;
+      const uint8_t* rec =
+          p.records + (static_cast<int64_t>(slot >> 4) * p.hkv + h) * kInt4Record;
+      const __half* km = reinterpret_cast<const __half*>(rec + kInt4KeyMeta + tok * 16) + grp;
+      const __half* vm = reinterpret_cast<const __half*>(rec + kInt4ValueMeta + tok * 16) + grp;
+      codes[i][0] = *reinterpret_cast<const uint32_t*>(rec + tok * 64 + (m & 3) * 16 + grp * 4);
+      // The word of store_int4_row; its other lane's makes the two halves.
+      codes[i][1] = *reinterpret_cast<const uint32_t*>(
+          rec + kInt4Value + value_code_row(tok) * 64 + (m & 3) * 16 + (grp & 1) * 8 +
+          (grp >> 1) * 4);
+      s[i][0] = km[0];
+      mid[i][0] = km[4];
+      s[i][1] = vm[0];
+      mid[i][1] = vm[4];
+    }
   }
 #pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    T* out = static_cast<T*>(kv == 0 ? p.key : p.value) + th * kHeadDim + 8 * m;
-    float x[8];
+  for (int i = 0; i < U; ++i) {
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, codes[i][1], 4);
+    codes[i][1] = (grp & 1) ? prmt(other, codes[i][1], 0x7632u) : prmt(codes[i][1], other, 0x5410u);
+    const int h = h0 + 2 * i;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // Nibbles i and i + 4 as the halves 1024 + z, less 1032 (exact).
-      const uint32_t w = ((codes[kv] >> (4 * i)) & 0x000f000fu) | 0x64006400u;
-      const uint32_t z = hsub2_u32(w, 0x64086408u);
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&z));
-      x[i] = __fadd_rn(__fmul_rn(f.x, s[kv]), mid[kv]);
-      x[i + 4] = __fadd_rn(__fmul_rn(f.y, s[kv]), mid[kv]);
-    }
-    if constexpr (sizeof(T) == 2) {
-      store8<T, true>(out, x);
-    } else {
-      reinterpret_cast<float4*>(out)[0] = make_float4(x[0], x[1], x[2], x[3]);
-      reinterpret_cast<float4*>(out)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    for (int kv = 0; kv < 2; ++kv) {
+      T* out = static_cast<T*>(kv == 0 ? p.key : p.value) +
+               (token * p.hkv + (h < p.hkv ? h : 0)) * kHeadDim + 8 * m;
+      const float sc = __half2float(s[i][kv]), md = __half2float(mid[i][kv]);
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // Nibbles j and j + 4 as the halves 1024 + z, less 1032 (exact).
+        const uint32_t c = ((codes[i][kv] >> (4 * j)) & 0x000f000fu) | 0x64006400u;
+        const uint32_t z = hsub2_u32(c, 0x64086408u);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&z));
+        x[j] = __fadd_rn(__fmul_rn(f.x, sc), md);
+        x[j + 4] = __fadd_rn(__fmul_rn(f.y, sc), md);
+      }
+      if (h >= p.hkv) continue;
+      if constexpr (sizeof(T) == 2) {
+        store8<T, true>(out, x);
+      } else {
+        reinterpret_cast<float4*>(out)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4*>(out)[1] = make_float4(x[4], x[5], x[6], x[7]);
+      }
     }
   }
 }

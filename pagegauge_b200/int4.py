@@ -69,16 +69,16 @@ class Int4PagePool:
         records = self.records
         device, tokens, kv_heads = records.device, slots.numel(), self.kv_heads
         slot_ptr = check_token_index(slots, "slots", tokens, device)
-        shape = (tokens, kv_heads, HEAD_DIM)
-        if key_out is None:
-            key_out = torch.empty(shape, dtype=dtype, device=device)
-        if value_out is None:
-            value_out = torch.empty(shape, dtype=dtype, device=device)
-        for name, t in (("key_out", key_out), ("value_out", value_out)):
-            if (t.shape != shape or t.dtype is not dtype or t.device != device
-                    or not t.is_contiguous() or t.data_ptr() % 16):
-                raise ValueError(f"{name} must be contiguous 16-byte aligned "
-                                 f"[T,{kv_heads},{HEAD_DIM}] {dtype}")
+        if key_out is None and value_out is None:
+            key_out, value_out = torch.empty((2, tokens, kv_heads, HEAD_DIM), dtype=dtype,
+                                             device=device).unbind(0)
+        else:
+            shape = (tokens, kv_heads, HEAD_DIM)
+            for name, t in (("key_out", key_out), ("value_out", value_out)):
+                if (t is None or t.shape != shape or t.dtype is not dtype or t.device != device
+                        or not t.is_contiguous() or t.data_ptr() % 16):
+                    raise ValueError(f"{name} must be contiguous 16-byte aligned "
+                                     f"[T,{kv_heads},{HEAD_DIM}] {dtype} (both outputs or none)")
         _lib.launch("pg_int4_read", device, records.data_ptr(), self.num_pages, kv_heads,
                     slot_ptr, tokens, key_out.data_ptr(), value_out.data_ptr(), DTYPES[dtype])
         return key_out, value_out
