@@ -503,6 +503,9 @@ typedef struct pg_int4_decode_args {
   const int32_t* item_off;      /* device [B*Hkv+1] */
   float* part_o;                /* device workspace [num_items*group*128] */
   float* part_lse;              /* device workspace [num_items*group] */
+  int32_t* work_counter;        /* device int32, zero before the first call and
+                                   left zero; like part_o, not shared by calls
+                                   that may run at the same time */
   int32_t num_items, batch, kv_heads, group;
   int32_t final_mode; /* 1: one item per (request, head): no merge launch */
   int32_t dtype;      /* PG_DTYPE_F16 or PG_DTYPE_BF16 */

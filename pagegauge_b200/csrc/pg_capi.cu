@@ -1312,11 +1312,13 @@ int32_t pg_decode_int4_run(const pg_int4_decode_args* a, void* stream) {
              "records must be 16-byte aligned");
   PG_REQUIRE(a->num_items == 0 || (a->indices != nullptr && a->last_page_len != nullptr),
              "page table is incomplete");
-  PG_REQUIRE(a->num_items == 0 || a->items != nullptr, "work items are required");
+  PG_REQUIRE(a->num_items == 0 || (a->items != nullptr && a->work_counter != nullptr),
+             "work items and their counter are required");
   const bool final_mode = a->final_mode != 0 && a->num_items > 0;
   PG_REQUIRE(final_mode || a->item_off != nullptr, "item offsets are required for the merge");
-  PG_REQUIRE(final_mode || a->num_items == 0 || (a->part_o != nullptr && a->part_lse != nullptr),
-             "split decode needs a partial-state workspace");
+  PG_REQUIRE(final_mode || a->num_items == 0 ||
+                 (a->part_o != nullptr && aligned(a->part_o, 16) && a->part_lse != nullptr),
+             "split decode needs a 16-byte aligned partial-state workspace");
   pg::Int4DecodeParams p{};
   p.q = a->q;
   p.q_stride_b = a->q_stride_b;
@@ -1334,6 +1336,7 @@ int32_t pg_decode_int4_run(const pg_int4_decode_args* a, void* stream) {
   p.sm_scale_log2 = a->sm_scale * 1.4426950408889634f;
   p.part_o = a->part_o;
   p.part_lse = a->part_lse;
+  p.counter = a->work_counter;
   p.final_mode = final_mode;
   p.out = a->out;
   p.out_stride_b = a->out_stride_b;
@@ -1347,13 +1350,19 @@ int32_t pg_decode_int4_run(const pg_int4_decode_args* a, void* stream) {
   if (a->num_items > 0) {
     int32_t rc = ensure_int4_smem();
     if (rc != PG_OK) return rc;
+    int dev = 0, sms = 0;
+    rc = cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+    if (rc == PG_OK)
+      rc = cuda_check(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev),
+                      "SM count");
+    if (rc != PG_OK) return rc;
     const bool narrow = a->group <= 4;
     rc = launch_pdl(half ? (narrow ? pg::pg_decode_int4_kernel<__half, true>
                                    : pg::pg_decode_int4_kernel<__half, false>)
                          : (narrow ? pg::pg_decode_int4_kernel<__nv_bfloat16, true>
                                    : pg::pg_decode_int4_kernel<__nv_bfloat16, false>),
-                    dim3(a->num_items), dim3(pg::kInt4Warps * 32), pg::kInt4SmemBytes, st,
-                    "int4 decode launch", p);
+                    dim3(std::min(a->num_items, pg::kInt4CtasPerSm * sms)),
+                    dim3(pg::kInt4Warps * 32), pg::kInt4SmemBytes, st, "int4 decode launch", p);
     if (rc != PG_OK || final_mode) return rc;
   }
   return launch_pdl(half ? pg::pg_int4_merge_kernel<__half>

@@ -44,6 +44,7 @@ struct Int4DecodeParams {
   float sm_scale_log2;
   float* part_o;    // [num_items, group, 128]
   float* part_lse;  // [num_items, group]
+  int32_t* counter; // items handed out past the grid; zero between launches
   int32_t final_mode;
   void* out;
   int64_t out_stride_b, out_stride_h;
@@ -56,17 +57,16 @@ struct Int4DecodeParams {
 constexpr int kInt4Warps = 4;
 constexpr int kInt4Slots = 2;  // pairs of pages in a warp's ring
 constexpr int kInt4CtasPerSm = 3;
-// Pages per warp asked of the L2 ahead of the dependency wait, by the blocks
-// that can be waiting there (later blocks start long after it): 49,152 tokens
-// 18.2 -> 17.6 us; 16 pages would cost 0.5 us, and asking in every block 1.2
-// us of 77 at eight long requests.
-constexpr int kInt4Prefetch = 4;
-constexpr int kInt4FirstWave = 148 * kInt4CtasPerSm;
 constexpr int kInt4RingBytes = kInt4Slots * 2 * kInt4Record;
-// The warps' rings, then their barriers; the epilogue reuses the rings.
-constexpr int kInt4SmemBytes = kInt4Warps * (kInt4RingBytes + kInt4Slots * 8);
-static_assert(kInt4Warps * (16 + 8 * kCoStride) * 4 <= kInt4Warps * kInt4RingBytes,
-              "the combine buffer lies in the rings");
+// The warps' rings, then their barriers, then the combine buffer (its own, so
+// that the next item's pages can arrive while it is in use).
+constexpr int kInt4CombineFloats = kInt4Warps * (16 + 8 * kCoStride);
+constexpr int kInt4CombineAt = kInt4Warps * (kInt4RingBytes + kInt4Slots * 8);
+constexpr int kInt4SmemBytes = kInt4CombineAt + kInt4CombineFloats * 4;
+static_assert(kInt4CombineAt % 16 == 0, "the combine buffer is read in 16-byte rows");
+// Pages per warp asked of the L2 ahead of the dependency wait: 49,152 tokens
+// 18.2 -> 17.6 us (16 pages would cost 0.5 us).
+constexpr int kInt4Prefetch = 4;
 // The running maximum is raised when a score passes it by this (log2).
 constexpr float kInt4Slack = 2.f;
 
@@ -354,6 +354,17 @@ __device__ __forceinline__ void int4_store_out(const Int4DecodeParams& p, int r,
     p.lse_out[static_cast<int64_t>(r) * (p.hkv * p.group) + qh] = lse;
 }
 
+// A warp's share of a work item: every kInt4Warps-th page from its own.
+__device__ __forceinline__ int int4_warp_pages(int count, int warp) {
+  const int n = count & 0x7fffffff;
+  return n > warp ? (n - warp + kInt4Warps - 1) / kInt4Warps : 0;
+}
+
+// Persistent: block b takes item b, then the next item that no block has (a
+// counter, which the last block to ask sets back to zero).  An item's page ids
+// are read, and its first pages requested, before the item ahead of it is
+// finished, so only the first item of a block waits for them.  Which block
+// takes an item changes no result: partial states are stored by item.
 template <typename T, bool NARROW>
 __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
     pg_decode_int4_kernel(const __grid_constant__ Int4DecodeParams p) {
@@ -369,151 +380,212 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
   }
   __syncwarp();
   pdl_launch_dependents();
-  const DecodeItem item = p.items[blockIdx.x];  // plan data
-  const int r = item.request, h = item.head_seg & 0xffff;
-  const int n_pages = item.count & 0x7fffffff;
-  const int n_w = n_pages > warp ? (n_pages - warp + kInt4Warps - 1) / kInt4Warps : 0;
-  const int n_pairs = (n_w + 1) >> 1;
+  __shared__ int s_next[2];  // the item after the next one, by parity
+  const bool hand_out = p.num_items > static_cast<int>(gridDim.x);
+  auto take = [&] {  // one thread; called until it returns no item
+    const int taken = atomicAdd(p.counter, 1);
+    if (taken == p.num_items - 1) *p.counter = 0;
+    return taken + static_cast<int>(gridDim.x);
+  };
+  int index = blockIdx.x;
+  DecodeItem item = p.items[index];  // plan data
+  int n_w = int4_warp_pages(item.count, warp);
   // Pages and page ids may be written by the kernel just before: what counts
   // is read after the wait.  Ahead of it the warp only asks the L2 for its
   // first pages, under ids that may be stale.
-  if (lane < n_w && lane < kInt4Prefetch && blockIdx.x < kInt4FirstWave) {
+  if (lane < n_w && lane < kInt4Prefetch) {
     const int guess = load_volatile(p.indices + item.idx_begin + warp + kInt4Warps * lane);
     if (guess >= 0 && guess < p.num_pages)
-      prefetch_l2(p.records + (static_cast<int64_t>(guess) * p.hkv + h) * kInt4Record,
+      prefetch_l2(p.records + (static_cast<int64_t>(guess) * p.hkv + (item.head_seg & 0xffff)) *
+                                  kInt4Record,
                   kInt4Record);
   }
   pdl_wait_primary();
+  const uint64_t policy = l2_evict_first_policy();
   // Lane u holds the record of the warp's page u (at most 32 per warp) and
-  // copies it itself.
+  // copies it itself; ids outside the pool leave their page out.
   const uint8_t* mine = nullptr;
-  bool bad = false;
-  if (lane < n_w) {
-    int id = load_volatile(p.indices + item.idx_begin + warp + kInt4Warps * lane);
-    bad = id < 0 || id >= p.num_pages;
+  uint32_t bad_pages = 0;
+  auto resolve = [&](int id, const DecodeItem& it, int pages) {
+    const bool bad = lane < pages && (id < 0 || id >= p.num_pages);
     if (bad) {
       record_error(p.error_flag, kDevBadPageId);
       id = 0;
     }
-    mine = p.records + (static_cast<int64_t>(id) * p.hkv + h) * kInt4Record;
-  }
-  const uint32_t bad_pages = __ballot_sync(0xffffffffu, bad);
-  const uint64_t policy = l2_evict_first_policy();
-  // Pair u's copies into slot `slot`: its first lane announces the bytes.
-  auto issue = [&](int u, int slot) {
-    const int first = 2 * u;
-    if (lane == first)
-      mbar_arrive_expect_tx(bars + slot, first + 1 < n_w ? 2 * kInt4Record : kInt4Record);
+    bad_pages = __ballot_sync(0xffffffffu, bad);
+    mine = lane < pages ? p.records + (static_cast<int64_t>(id) * p.hkv +
+                                       (it.head_seg & 0xffff)) * kInt4Record
+                        : nullptr;
+  };
+  // Pair u's copies into slot `at`: its first lane announces the bytes.
+  auto issue = [&](int u, int at) {
+    if (lane == 2 * u)
+      mbar_arrive_expect_tx(bars + at, 2 * u + 1 < n_w ? 2 * kInt4Record : kInt4Record);
     __syncwarp();
     if ((lane >> 1) == u && mine != nullptr)
-      bulk_load_hint(ring + (2 * slot + (lane & 1)) * kInt4Record, mine, kInt4Record, bars + slot,
+      bulk_load_hint(ring + (2 * at + (lane & 1)) * kInt4Record, mine, kInt4Record, bars + at,
                      policy);
   };
-  for (int u = 0; u < kInt4Slots && u < n_pairs; ++u) issue(u, u);
-  int last = kPage;
-  if (item.count < 0) {
-    const int lv = __ldg(p.last_len + r);
-    last = lv < 1 ? 1 : (lv > kPage ? kPage : lv);
-  }
-  Int4Query iq;
-  load_query_int4<T, NARROW>(p, r, h, g, t, iq);
-  Int4State st;
-  st.m[0] = st.m[1] = kNegInf;
-  st.l[0] = st.l[1] = 0.f;
-  st.ref[0] = st.ref[1] = 0.f;
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) st.o[j][i] = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) st.sums[i] = 0.f;
-  // Tokens that count in the warp's last page, if it is the request's last.
-  const int tail = n_w > 0 && warp + kInt4Warps * (n_w - 1) == n_pages - 1 ? last : kPage;
-
-  bool ok = true;
   int slot = 0;
   uint32_t phase = 0;
-  for (int u = 0; u < n_pairs; ++u) {
-    const bool waited = mbar_wait_bounded(bars + slot, phase);
-    if (!__all_sync(0xffffffffu, waited)) {
-      // Let the copies in flight land before the block ends.
-      record_error(p.error_flag, kDevWaitTimeout);
-      const int end = u + kInt4Slots < n_pairs ? u + kInt4Slots : n_pairs;
-      for (int v = u; v < end; ++v)
-        mbar_wait_bounded(bars + v % kInt4Slots, static_cast<uint32_t>(v / kInt4Slots) & 1u);
-      ok = false;
-      break;
+  bool ok = true;  // no wait of this warp has run out
+  // The item's first pairs go to the slots from `slot` on.
+  auto issue_first = [&] {
+    int at = slot;
+    for (int u = 0; u < kInt4Slots && 2 * u < n_w; ++u) {
+      issue(u, at);
+      if (++at == kInt4Slots) at = 0;
     }
-    int valid[2] = {kPage, kPage};
-    if (u == n_pairs - 1) {
-      const bool two = (n_w & 1) == 0;
-      valid[0] = two ? kPage : tail;
-      valid[1] = two ? tail : 0;
-    }
-    if (bad_pages != 0u) {
-      if ((bad_pages >> (2 * u)) & 1u) valid[0] = 0;
-      if ((bad_pages >> (2 * u)) & 2u) valid[1] = 0;
-    }
-    pages_int4<NARROW>(ring + 2 * slot * kInt4Record, iq, st, valid, g, t);
-    __syncwarp();
-    if (u + kInt4Slots < n_pairs) issue(u + kInt4Slots, slot);
-    if (++slot == kInt4Slots) {
-      slot = 0;
-      phase ^= 1u;
-    }
+  };
+  resolve(lane < n_w ? load_volatile(p.indices + item.idx_begin + warp + kInt4Warps * lane) : 0,
+          item, n_w);
+  issue_first();
+  int next_index = p.num_items;
+  if (hand_out) {
+    if (threadIdx.x == 0) s_next[0] = take();
+    __syncthreads();
+    next_index = s_next[0];
   }
 
-  // Warp totals: l over the 8 token lanes, then the output rows.
-  const float l0 = warp_sum_xor_g(st.l[0]), l1 = warp_sum_xor_g(st.l[1]);
-  __syncthreads();  // every warp has drained its ring
-  float* cm = reinterpret_cast<float*>(smem_int4);  // [W][8]
-  float* cl = cm + kInt4Warps * 8;                  // [W][8]
-  float* co = cl + kInt4Warps * 8;                  // [W][8][kCoStride]
-  if (g == 0) {
-    cm[warp * 8 + 2 * t] = ok ? st.m[0] : kNegInf;
-    cm[warp * 8 + 2 * t + 1] = ok ? st.m[1] : kNegInf;
-    cl[warp * 8 + 2 * t] = ok ? l0 : 0.f;
-    cl[warp * 8 + 2 * t + 1] = ok ? l1 : 0.f;
-  }
+  for (int parity = 1;; parity ^= 1) {
+    const int r = item.request, h = item.head_seg & 0xffff;
+    const int n_pages = item.count & 0x7fffffff, n_pairs = (n_w + 1) >> 1;
+    const bool more = next_index < p.num_items;
+    if (more && threadIdx.x == 0) s_next[parity] = take();
+    DecodeItem next;
+    next.count = 0;
+    if (more) next = p.items[next_index];
+    // Tokens that count in the warp's last page, if it is the request's last.
+    int tail = kPage;
+    if (item.count < 0 && n_w > 0 && warp + kInt4Warps * (n_w - 1) == n_pages - 1) {
+      const int lv = __ldg(p.last_len + r);
+      tail = lv < 1 ? 1 : (lv > kPage ? kPage : lv);
+    }
+    Int4Query iq;
+    load_query_int4<T, NARROW>(p, r, h, g, t, iq);
+    const int next_w = int4_warp_pages(next.count, warp);
+    const int next_id = lane < next_w ? load_volatile(p.indices + next.idx_begin + warp +
+                                                      kInt4Warps * lane)
+                                      : 0;
+    Int4State st;
+    st.m[0] = st.m[1] = kNegInf;
+    st.l[0] = st.l[1] = 0.f;
+    st.ref[0] = st.ref[1] = 0.f;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    // The row of this lane's column, and its sums (shuffled by every lane).
-    const int q = NARROW ? (2 * t + i) & 3 : 2 * t + i;
-    float* row = co + (warp * 8 + q) * kCoStride;
+    for (int j = 0; j < 8; ++j)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float add = __shfl_sync(0xffffffffu, st.sums[i], 16 + 4 * j + t) -
-                        8.f * __shfl_sync(0xffffffffu, st.sums[i], 4 * (NARROW ? j >> 1 : j) + t);
-      if (q < p.group && (!NARROW || (t >> 1) == (j & 1))) {
-        const float* a = st.o[2 * j];
-        const float* b = st.o[2 * j + 1];
-        *reinterpret_cast<float4*>(row + 32 * j + 4 * g) =
-            make_float4(fmaf(a[i], 0x1p24f, add), fmaf(a[2 + i] - a[i], 0x1p20f, add),
-                        fmaf(b[i], 0x1p24f, add), fmaf(b[2 + i] - b[i], 0x1p20f, add));
+      for (int i = 0; i < 4; ++i) st.o[j][i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) st.sums[i] = 0.f;
+
+    for (int u = 0; u < n_pairs && ok; ++u) {
+      const bool waited = mbar_wait_bounded(bars + slot, phase);
+      if (!__all_sync(0xffffffffu, waited)) {
+        // Let the copies in flight land; this warp copies nothing more.
+        record_error(p.error_flag, kDevWaitTimeout);
+        int at = slot;
+        uint32_t ph = phase;
+        for (int v = u; v < n_pairs && v < u + kInt4Slots; ++v) {
+          mbar_wait_bounded(bars + at, ph);
+          if (++at == kInt4Slots) {
+            at = 0;
+            ph ^= 1u;
+          }
+        }
+        ok = false;
+        break;
+      }
+      int valid[2] = {kPage, kPage};
+      if (u == n_pairs - 1) {
+        const bool two = (n_w & 1) == 0;
+        valid[0] = two ? kPage : tail;
+        valid[1] = two ? tail : 0;
+      }
+      if (bad_pages != 0u) {
+        if ((bad_pages >> (2 * u)) & 1u) valid[0] = 0;
+        if ((bad_pages >> (2 * u)) & 2u) valid[1] = 0;
+      }
+      pages_int4<NARROW>(ring + 2 * slot * kInt4Record, iq, st, valid, g, t);
+      __syncwarp();
+      if (u + kInt4Slots < n_pairs) issue(u + kInt4Slots, slot);
+      if (++slot == kInt4Slots) {
+        slot = 0;
+        phase ^= 1u;
       }
     }
-  }
-  __syncthreads();
-  for (int idx = threadIdx.x; idx < p.group * kHeadDim; idx += blockDim.x) {
-    const int q = idx >> 7, d = idx & 127;
-    float M = kNegInf, L = 0.f, O = 0.f;
-#pragma unroll
-    for (int w = 0; w < kInt4Warps; ++w) M = fmaxf(M, cm[w * 8 + q]);
-#pragma unroll
-    for (int w = 0; w < kInt4Warps; ++w) {
-      if (cl[w * 8 + q] == 0.f) continue;
-      const float e = fast_exp2(cm[w * 8 + q] - M);
-      L += cl[w * 8 + q] * e;
-      O += co[(w * 8 + q) * kCoStride + d] * e;
+    if (more) {
+      n_w = ok ? next_w : 0;
+      resolve(next_id, next, n_w);
+      issue_first();
     }
-    const float v = L == 0.f ? 0.f : O / L, lse = L == 0.f ? kNegInf : M + fast_log2(L);
-    if (p.final_mode) {
-      int4_store_out<T>(p, r, h, q, d, v, lse);
-    } else {
-      const int64_t base = static_cast<int64_t>(blockIdx.x) * p.group + q;
-      p.part_o[base * kHeadDim + d] = v;
-      if (d == 0) p.part_lse[base] = lse;
+
+    // Warp totals: l over the 8 token lanes, then the output rows.
+    const float l0 = warp_sum_xor_g(st.l[0]), l1 = warp_sum_xor_g(st.l[1]);
+    __syncthreads();  // the combine buffer is free
+    float* cm = reinterpret_cast<float*>(smem_int4 + kInt4CombineAt);  // [W][8]
+    float* cl = cm + kInt4Warps * 8;                                   // [W][8]
+    float* co = cl + kInt4Warps * 8;                                   // [W][8][kCoStride]
+    if (g == 0) {
+      cm[warp * 8 + 2 * t] = ok ? st.m[0] : kNegInf;
+      cm[warp * 8 + 2 * t + 1] = ok ? st.m[1] : kNegInf;
+      cl[warp * 8 + 2 * t] = ok ? l0 : 0.f;
+      cl[warp * 8 + 2 * t + 1] = ok ? l1 : 0.f;
     }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      // The row of this lane's column, and its sums (shuffled by every lane).
+      const int q = NARROW ? (2 * t + i) & 3 : 2 * t + i;
+      float* row = co + (warp * 8 + q) * kCoStride;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float add = __shfl_sync(0xffffffffu, st.sums[i], 16 + 4 * j + t) -
+                          8.f * __shfl_sync(0xffffffffu, st.sums[i], 4 * (NARROW ? j >> 1 : j) + t);
+        if (q < p.group && (!NARROW || (t >> 1) == (j & 1))) {
+          const float* a = st.o[2 * j];
+          const float* b = st.o[2 * j + 1];
+          *reinterpret_cast<float4*>(row + 32 * j + 4 * g) =
+              make_float4(fmaf(a[i], 0x1p24f, add), fmaf(a[2 + i] - a[i], 0x1p20f, add),
+                          fmaf(b[i], 0x1p24f, add), fmaf(b[2 + i] - b[i], 0x1p20f, add));
+        }
+      }
+    }
+    __syncthreads();
+    // Thread -> four dims of one row.
+    for (int idx = threadIdx.x; idx < p.group * 32; idx += blockDim.x) {
+      const int q = idx >> 5, d = 4 * (idx & 31);
+      float M = kNegInf, L = 0.f;
+      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kInt4Warps; ++w) M = fmaxf(M, cm[w * 8 + q]);
+#pragma unroll
+      for (int w = 0; w < kInt4Warps; ++w) {
+        if (cl[w * 8 + q] == 0.f) continue;
+        const float e = fast_exp2(cm[w * 8 + q] - M);
+        const float4 o = *reinterpret_cast<const float4*>(co + (w * 8 + q) * kCoStride + d);
+        L += cl[w * 8 + q] * e;
+        O.x += o.x * e;
+        O.y += o.y * e;
+        O.z += o.z * e;
+        O.w += o.w * e;
+      }
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      const float lse = L == 0.f ? kNegInf : M + fast_log2(L);
+      O = make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv);
+      if (p.final_mode) {
+        int4_store_out<T>(p, r, h, q, d + 0, O.x, lse);
+        int4_store_out<T>(p, r, h, q, d + 1, O.y, lse);
+        int4_store_out<T>(p, r, h, q, d + 2, O.z, lse);
+        int4_store_out<T>(p, r, h, q, d + 3, O.w, lse);
+      } else {
+        const int64_t base = static_cast<int64_t>(index) * p.group + q;
+        *reinterpret_cast<float4*>(p.part_o + base * kHeadDim + d) = O;
+        if (d == 0) p.part_lse[base] = lse;
+      }
+    }
+    if (!more) break;
+    index = next_index;
+    next_index = s_next[parity];  // stored ahead of the two barriers above
+    item = next;
   }
 }
 

@@ -439,7 +439,7 @@ class Int4DecodeWrapper(BatchDecodeWithPagedKVCacheWrapper):
             q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], lse_ptr, vc_ptr,
             kv_heads * HEAD_DIM, records_ptr, pages, self._indices.data_ptr(),
             self._last_len.data_ptr(), plan.items_ptr, plan.off_ptr, plan.o_ptr, plan.lse_ptr,
-            plan.num_items, plan.batch, kv_heads, plan.group,
+            plan.sem_ptr, plan.num_items, plan.batch, kv_heads, plan.group,
             plan.single and plan.num_items > 0, DTYPES[dtype],
             self._sm_scale if sm_scale is None else sm_scale, 0))
         return (out, lse) if return_lse else out

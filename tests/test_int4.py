@@ -75,7 +75,7 @@ def append_args(**kw):
 def decode_args(**kw):
     a = _lib.PgInt4DecodeArgs()
     a.q = a.out = a.records = a.indices = a.last_page_len = a.items = a.item_off = 0x1000
-    a.part_o = a.part_lse = 0x1000
+    a.part_o = a.part_lse = a.work_counter = 0x1000
     a.num_items, a.batch, a.kv_heads, a.group, a.num_pages, a.sm_scale = 2, 1, 1, 4, 4, 0.1
     for k, v in kw.items():
         setattr(a, k, v)
@@ -93,7 +93,7 @@ def decode_args(**kw):
      [dict(batch=0), dict(group=9), dict(group=0), dict(sm_scale=0.0),
       dict(sm_scale=float("nan")), dict(dtype=2), dict(q=0x1002), dict(q_stride_h=3),
       dict(out=None), dict(num_items=-1), dict(num_pages=0), dict(records=0x1004),
-      dict(indices=None), dict(items=None), dict(item_off=None), dict(part_o=None)]),
+      dict(indices=None), dict(items=None), dict(item_off=None), dict(part_o=None), dict(part_o=0x1004), dict(work_counter=None)]),
 ])
 def test_c_entries_refuse(entry, make, bad):
     fn = getattr(_lib.load(), entry)
