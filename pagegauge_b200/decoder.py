@@ -45,9 +45,12 @@ from . import _lib, scheduler
 from .cache import GaugeCache, apply_rope_fp16, rope_tables
 from .decode import PageGaugeDecode
 from .gemm import RESIDUAL, SILU_MUL, STORE, PackedWeight, SkinnyGemm
+from .int4 import Int4PagePool
 from .peer import TpExchange
 from .quantize import quantize_pages_into
+from .rotary import apply_rotary, rotary_tables
 from .runtime import load_append_extension
+from .wrapper import make_int4_wrapper
 
 PAGE = 16
 HEAD_DIM = 128
@@ -257,6 +260,10 @@ class PageGaugeDecoder:
     streaming GEMM publishes its tiles, or a small kernel publishes cuBLAS's
     output; the next kernel reduces and adds the residual + RMSNorm),
     "nccl" uses NCCL all-reduces.
+    ``kv_cache``: "page_gauge" (INT8 pages and the exact FP16 pages), or "int4":
+    every token in 4 bits, centred by the prompt's means, appended by
+    ``rope_append_int4`` and attended over by the 4-bit decode; exact pages do
+    not apply there, and the rotation is FP32 (``rotary_tables``).
     ``fuse_norm`` (one GPU, streaming GEMMs): compute the RMSNorms inside the
     qkv, gate/up and LM-head GEMMs instead of separate launches; measured
     slower on B200 (4.1-4.4 ms against 3.6-3.9 ms per B=1 step), so off by
@@ -266,11 +273,17 @@ class PageGaugeDecoder:
     def __init__(self, weights: DecoderWeights, batch: int, max_context: int,
                  process_group=None, ring_pages: int = 16, workspace_mb: int = 32,
                  gemm: str = "auto", sink_pages: int = 0, suffix_pages: int = 0,
-                 fuse_norm: bool = False, tp_reduce: str = "peer"):
+                 fuse_norm: bool = False, tp_reduce: str = "peer",
+                 kv_cache: str = "page_gauge"):
         cfg, tp = weights.cfg, weights.tp
         if cfg.head_dim != HEAD_DIM:
             raise ValueError("head_dim must be 128")
         self.cfg, self.tp, self.w = cfg, tp, weights
+        if kv_cache not in ("page_gauge", "int4"):
+            raise ValueError("kv_cache must be 'page_gauge' or 'int4'")
+        if kv_cache == "int4" and (ring_pages != 16 or sink_pages or suffix_pages):
+            raise ValueError("exact pages do not apply to the 4-bit cache")
+        self.kv_cache = kv_cache
         self.pg = process_group
         self.fuse_norm = bool(fuse_norm)
         self.tpx = None
@@ -301,14 +314,27 @@ class PageGaugeDecoder:
         B, cap, hkv = batch, self.capacity_pages, self.hkv
         z = dict(device=dev)
         self.caches: list[GaugeCache] = []
+        self.pools: list[Int4PagePool] = []
+        self.centers: list[torch.Tensor] = []  # [2 (key, value), B, Hkv, 128] per pool
         for _ in range(cfg.layers):
+            if kv_cache == "int4":
+                self.pools.append(Int4PagePool(B * cap, hkv, device=dev))
+                self.centers.append(torch.zeros(2, B, hkv, HEAD_DIM, dtype=torch.float16, **z))
+                continue
             codes = lambda: torch.zeros(B * cap, PAGE, hkv, HEAD_DIM, dtype=torch.int8, **z)
             scales = lambda: torch.zeros(B * cap, hkv, dtype=torch.float16, **z)
             ring = lambda: torch.zeros(B * storage, PAGE, hkv, HEAD_DIM, dtype=torch.float16, **z)
             cen = lambda: torch.zeros(B, hkv, HEAD_DIM, dtype=torch.float16, **z)
             self.caches.append(GaugeCache(ring(), ring(), codes(), codes(), scales(), scales(),
                                           cen(), cen(), ring_pages, self.fixed_pages))
-        self.cos, self.sin = rope_tables(self.max_context, cfg.rope_theta, device=dev)
+        if kv_cache == "int4":
+            self.cos, self.sin = rotary_tables(self.max_context, HEAD_DIM, cfg.rope_theta,
+                                               device=dev)
+            # Request r's token at position p lies at slot r * capacity + p.
+            self.slots = torch.zeros(B, dtype=torch.int32, **z)
+            self.center_rows = torch.arange(B, dtype=torch.int32, **z)
+        else:
+            self.cos, self.sin = rope_tables(self.max_context, cfg.rope_theta, device=dev)
         qkv_w = (self.hq + 2 * hkv) * HEAD_DIM
         h16 = dict(dtype=torch.float16, **z)
         self.residual = torch.zeros(B, cfg.hidden, **h16)
@@ -425,6 +451,8 @@ class PageGaugeDecoder:
         self.host_positions[:] = T
         self.positions.fill_(T)
         self.last_len.fill_(T % PAGE + 1)
+        if self.kv_cache == "int4":
+            torch.mul(self.center_rows, self.max_context, out=self.slots).add_(T)
         return out
 
     def _prefill_request(self, r: int, tokens: torch.Tensor) -> torch.Tensor:
@@ -441,9 +469,12 @@ class PageGaugeDecoder:
             q = qkv[:, :self.hq * d].view(T, self.hq, d)
             k = qkv[:, self.hq * d:(self.hq + self.hkv) * d].view(T, self.hkv, d)
             v = qkv[:, (self.hq + self.hkv) * d:].view(T, self.hkv, d)
-            q = apply_rope_fp16(q, cos, sin)
-            k = apply_rope_fp16(k, cos, sin)
-            self._fill_cache(l, r, k, v)
+            if self.kv_cache == "int4":
+                q, k = self._fill_pool(l, r, q, k, v)
+            else:
+                q = apply_rope_fp16(q, cos, sin)
+                k = apply_rope_fp16(k, cos, sin)
+                self._fill_cache(l, r, k, v)
             kk = k.repeat_interleave(group, dim=1)
             vv = v.repeat_interleave(group, dim=1)
             att = torch.nn.functional.scaled_dot_product_attention(
@@ -491,6 +522,22 @@ class PageGaugeDecoder:
             c.exact_key[slot] = (dk[lp].float() - c.key_center[r].float()).half()
             c.exact_value[slot] = (dv[lp].float() - c.value_center[r].float()).half()
 
+    def _fill_pool(self, layer: int, r: int, q: torch.Tensor, k: torch.Tensor,
+                   v: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """The prompt's 4-bit pages: centres are the FP32 means of its rotated
+        keys and its values, then every token is appended.  Returns the
+        rotated rows."""
+        T = k.shape[0]
+        at = torch.arange(T, dtype=torch.int32, device=self.device)
+        rq, rk = apply_rotary(q, k, self.cos, self.sin, at)
+        centers = self.centers[layer]
+        centers[0, r] = rk.float().mean(0).half()
+        centers[1, r] = v.float().mean(0).half()
+        self.ext.rope_append_int4(q, k, v, self.cos, self.sin, at, at + r * self.max_context, rq,
+                                  self.pools[layer].records, key_center=centers[0],
+                                  value_center=centers[1], center_rows=torch.full_like(at, r))
+        return rq, rk
+
     # ------------------------------------------------------------ decode
     def _entry(self, positions) -> dict:
         """The plan (work list + page tables + captured step) of the page
@@ -505,10 +552,14 @@ class PageGaugeDecoder:
             return entry
         if max(int(p) for p in positions) >= self.max_context:
             raise RuntimeError("decode position exceeds the cache capacity")
+        dev = self.device
+        if self.kv_cache == "int4":
+            entry = self._int4_entry(key)
+            self._remember(key, entry)
+            return entry
         o_ptr, o_idx, e_ptr, e_idx = page_tables(positions, self.capacity_pages, self.ring_pages,
                                                  self.sink_pages, self.suffix_pages,
                                                  self.initial_pages)
-        dev = self.device
         dec = PageGaugeDecode(torch.empty(self._ws_bytes, dtype=torch.uint8, device=dev))
         old_idx = torch.from_numpy(o_idx).to(dev)
         ex_idx = torch.from_numpy(e_idx).to(dev)
@@ -518,11 +569,27 @@ class PageGaugeDecoder:
                  torch.from_numpy(e_ptr), ex_idx, self.last_len, self.hq, self.hkv,
                  old_split_pages=split, old_last_page_len=self._old_last if has_old else None)
         entry = {"dec": dec, "old": old_idx, "exact": ex_idx, "graph": None}
+        self._remember(key, entry)
+        return entry
+
+    def _remember(self, key: tuple, entry: dict) -> None:
         self._bank[key] = entry
         while len(self._bank) > self._bank_size:
             self._bank.pop(next(iter(self._bank)))
         self.replans += 1
-        return entry
+
+    def _int4_entry(self, last_pages: tuple) -> dict:
+        """The 4-bit decode's plan for requests that append to ``last_pages``
+        (request r's page p is pool page r * capacity + p)."""
+        counts = [p + 1 for p in last_pages]
+        indices = np.concatenate([r * self.capacity_pages + np.arange(n, dtype=np.int32)
+                                  for r, n in enumerate(counts)]).astype(np.int32)
+        indptr = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+        dec = make_int4_wrapper(workspace=torch.empty(self._ws_bytes, dtype=torch.uint8,
+                                                      device=self.device))
+        dec.plan(torch.from_numpy(indptr), torch.from_numpy(indices).to(self.device),
+                 self.last_len, self.hq, self.hkv, HEAD_DIM, PAGE, kv_data_type=torch.uint8)
+        return {"dec": dec, "graph": None}
 
     def _step_body(self, dec: PageGaugeDecode) -> None:
         """One decode step on the current stream (capturable)."""
@@ -536,8 +603,8 @@ class PageGaugeDecoder:
         pending = False  # a published down_proj awaits its peer reduction
         delta = None
         eps = self.cfg.rms_eps
+        int4 = self.kv_cache == "int4"
         for l, lw in enumerate(self.w.layers):
-            c = self.caches[l]
             pk = self.packed[l] if self.packed else {}
             if fuse_norm:
                 # RMSNorm inside the qkv projection.
@@ -552,15 +619,24 @@ class PageGaugeDecoder:
             q = self.qkv[:, :q_w].view(B, self.hq, d)
             k = self.qkv[:, q_w:q_w + kv_w].view(B, self.hkv, d)
             v = self.qkv[:, q_w + kv_w:].view(B, self.hkv, d)
-            self.ext.rope_append_page_gauge_batched(
-                q, k, v, self.cos, self.sin, self.positions, c.key_center, c.value_center,
-                self.rq, c.exact_key, c.exact_value, c.key_codes, c.value_codes, c.key_scales,
-                c.value_scales, self.fixed_pages)
-            # With a one-page ring the page this step's append closes is
-            # INT8 at the next step, whose decode must then wait for it.
-            dec.run(self.rq, c.key_codes, c.value_codes, c.key_scales, c.value_scales,
-                    c.exact_key, c.exact_value, c.value_center, out=self.attn,
-                    int8_after_wait=self.ring_pages == 1)
+            if int4:
+                centers = self.centers[l]
+                self.ext.rope_append_int4(
+                    q, k, v, self.cos, self.sin, self.positions, self.slots, self.rq,
+                    self.pools[l].records, key_center=centers[0], value_center=centers[1],
+                    center_rows=self.center_rows)
+                dec.run(self.rq, self.pools[l], value_center=centers[1], out=self.attn)
+            else:
+                c = self.caches[l]
+                self.ext.rope_append_page_gauge_batched(
+                    q, k, v, self.cos, self.sin, self.positions, c.key_center, c.value_center,
+                    self.rq, c.exact_key, c.exact_value, c.key_codes, c.value_codes, c.key_scales,
+                    c.value_scales, self.fixed_pages)
+                # With a one-page ring the page this step's append closes is
+                # INT8 at the next step, whose decode must then wait for it.
+                dec.run(self.rq, c.key_codes, c.value_codes, c.key_scales, c.value_scales,
+                        c.exact_key, c.exact_value, c.value_center, out=self.attn,
+                        int8_after_wait=self.ring_pages == 1)
             if fused and tpx is not None:
                 # Row-parallel projections publish their tiles through peer
                 # memory; the next kernel sums the ranks' tiles into the
@@ -619,6 +695,8 @@ class PageGaugeDecoder:
         self.tokens.copy_(self._greedy(self.logits))
         _call("pg_step_positions", self.positions.data_ptr(), self.last_len.data_ptr(), B, 1,
               _stream())
+        if int4:
+            _call("pg_step_positions", self.slots.data_ptr(), None, B, 1, _stream())
 
     def _linear(self, x: torch.Tensor, w: torch.Tensor, out: torch.Tensor,
                 packed: PackedWeight | None = None) -> None:
@@ -629,10 +707,14 @@ class PageGaugeDecoder:
 
     def launches_per_step(self) -> int:
         """Kernel launches of this library in one decode step."""
+        return self._layer_launches() + (self.kv_cache == "int4")  # its slots' update
+
+    def _layer_launches(self) -> int:
         entry = next(iter(self._bank.values()), None)
         attn = 2
         if entry is not None:
-            plan = entry["dec"].work_plan
+            dec = entry["dec"]
+            plan = dec._plan if self.kv_cache == "int4" else dec.work_plan
             attn = 1 if (plan.single and plan.num_items) else 2
         if self.gemm_impl == "pg" and self.pg is None and self.fuse_norm:
             # qkv (+RMSNorm), append, o (+residual), gate_up (+RMSNorm,
