@@ -243,7 +243,7 @@ def launch(name: str, device, *args) -> None:
     which is made the current device for the call."""
     index = device.index
     fn = getattr(_lib or load(), name)
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):

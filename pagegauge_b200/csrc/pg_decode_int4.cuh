@@ -18,7 +18,7 @@
 // q over group g's 32 dims,
 //   score = sum_g s_g (sum_d q_d z_d - 8 qs_g) + m_g qs_g
 // -8 qs_g is the initial accumulator of group g's products, and the last
-// term one TF32 product with qs split in two (22 bits).  For the values
+// term one TF32 product with qs split in two.  For the values
 //   O_d = sum_t (P_t s_tg) z_td - 8 sum_t (P_t s_tg) + sum_t P_t m_tg
 // where P s is formed in FP32 and rounded once to FP16, and the two last sums
 // come from tensor-core products of the same rounded operands, so that a
@@ -92,6 +92,13 @@ __device__ __forceinline__ void mma_1688_tf32(float* d, float a0, float a1, floa
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(__float_as_uint(a0)), "r"(__float_as_uint(a1)), "r"(__float_as_uint(a2)),
         "r"(__float_as_uint(a3)), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)), "f"(0.f));
+}
+// Rounded to TF32's 11 bits (the product itself would cut the rest off): two
+// such parts leave 2^-24 of a value.
+__device__ __forceinline__ float round_tf32(float x) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+  return __uint_as_float(r);
 }
 // The 8x8 matrix of halves whose row g lane (g, t) holds columns 2t, 2t+1
 // of, transposed.
@@ -195,8 +202,8 @@ __device__ __forceinline__ void load_query_int4(const Int4DecodeParams& p, int r
       iq.c0[j][i] = -8.f * __shfl_sync(0xffffffffu, qs[j], 4 * (2 * t + i));
   }
   const float mine = t == 0 ? qs[0] : t == 1 ? qs[1] : t == 2 ? qs[2] : qs[3];
-  iq.qs_hi = __uint_as_float(__float_as_uint(mine) & 0xffffe000u);
-  iq.qs_lo = mine - iq.qs_hi;
+  iq.qs_hi = round_tf32(mine);
+  iq.qs_lo = round_tf32(mine - iq.qs_hi);
   // 2^24 undoes the subnormal codes.
   const float down = p.sm_scale_log2 * 0x1p24f / up;
 #pragma unroll
@@ -589,30 +596,34 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
   }
 }
 
-// Joins the work items of each (request, query head): one CTA per row, warp w
-// folds partials w, w + 8, ... with four dims per lane and up to eight loads
-// in flight, then the warps' states are combined.
-template <typename T>
+// Joins the work items of each (request, query head): R warps per row fold
+// partials w, w + R, ... with four dims per lane and up to eight loads in
+// flight, then a row's warps are combined.  R = 8 (a block per row) where a
+// row has many partials, 1 (eight rows per block) where it has few.
+template <typename T, int R>
 __global__ void __launch_bounds__(256)
     pg_int4_merge_kernel(const __grid_constant__ Int4DecodeParams p) {
   constexpr int W = 8, U = 8;
   __shared__ float s_m[W], s_l[W];
   __shared__ float4 s_o[W][32];
-  const int hq = p.hkv * p.group;
-  const int r = blockIdx.x / hq, qh = blockIdx.x % hq;
-  const int h = qh / p.group, q = qh % p.group;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int begin = p.item_off[r * p.hkv + h], end = p.item_off[r * p.hkv + h + 1];
+  const int hq = p.hkv * p.group;
+  const int row = blockIdx.x * (W / R) + warp / R;
+  const bool live = row < p.batch * hq;
+  const int r = live ? row / hq : 0, qh = live ? row % hq : 0;
+  const int h = qh / p.group, q = qh % p.group;
+  const int begin = p.item_off[r * p.hkv + h];
+  const int end = live ? p.item_off[r * p.hkv + h + 1] : begin;
   pdl_launch_dependents();
   pdl_wait_primary();
   float m = kNegInf, den = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = begin + warp; i0 < end; i0 += W * U) {
+  for (int i0 = begin + warp % R; i0 < end; i0 += R * U) {
     float l[U];
     float4 v[U];
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      const int i = i0 + W * k;
+      const int i = i0 + R * k;
       l[k] = kNegInf;
       v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (i < end) {
@@ -634,26 +645,39 @@ __global__ void __launch_bounds__(256)
       m = mn;
     }
   }
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = den;
-  }
-  s_o[warp][lane] = acc;
-  __syncthreads();
-  if (threadIdx.x >= kHeadDim) return;
-  const int d = threadIdx.x;
-  float M = kNegInf, L = 0.f, O = 0.f;
+  if constexpr (R > 1) {
+    if (lane == 0) {
+      s_m[warp] = m;
+      s_l[warp] = den;
+    }
+    s_o[warp][lane] = acc;
+    __syncthreads();
+    if (warp % R != 0) return;
+    float M = kNegInf;
 #pragma unroll
-  for (int w = 0; w < W; ++w) M = fmaxf(M, s_m[w]);
+    for (int w = 0; w < R; ++w) M = fmaxf(M, s_m[warp + w]);
+    den = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int w = 0; w < W; ++w) {
-    if (s_l[w] == 0.f) continue;
-    const float e = fast_exp2(s_m[w] - M);
-    L += s_l[w] * e;
-    O += reinterpret_cast<const float*>(s_o[w])[d] * e;
+    for (int w = 0; w < R; ++w) {
+      if (s_l[warp + w] == 0.f) continue;
+      const float e = fast_exp2(s_m[warp + w] - M);
+      const float4 o = s_o[warp + w][lane];
+      den += s_l[warp + w] * e;
+      acc.x += o.x * e;
+      acc.y += o.y * e;
+      acc.z += o.z * e;
+      acc.w += o.w * e;
+    }
+    m = M;
   }
-  int4_store_out<T>(p, r, h, q, d, L == 0.f ? 0.f : O / L,
-                    L == 0.f ? kNegInf : M + fast_log2(L));
+  if (!live) return;
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+  const float lse = den == 0.f ? kNegInf : m + fast_log2(den);
+  int4_store_out<T>(p, r, h, q, 4 * lane + 0, acc.x * inv, lse);
+  int4_store_out<T>(p, r, h, q, 4 * lane + 1, acc.y * inv, lse);
+  int4_store_out<T>(p, r, h, q, 4 * lane + 2, acc.z * inv, lse);
+  int4_store_out<T>(p, r, h, q, 4 * lane + 3, acc.w * inv, lse);
 }
 
 }  // namespace pg

@@ -32,12 +32,15 @@ struct RotaryParams {
 // Rows that are 16-byte aligned and whose parts are whole 16-byte chunks.  A
 // thread takes one turning chunk (half layout: of both halves) of every
 // row_groups-th row of one token, so it reads its table entries once, and the
-// rows' copied chunks with it, U rows requested before the first is used.
-// Bound by HBM: each row is read and written once.
+// rows' copied chunks with it, two rows requested before the first is used.
+// Bound by HBM (each row is read and written once), so what counts is bytes in
+// flight against registers: interleaved rows hold half as much per thread and
+// run six blocks per SM (8,191 tokens: 32.9 us, 38.4 us with four rows in
+// flight on four blocks), half-layout rows four.
 template <typename T, bool INTERLEAVED>
-__global__ void __launch_bounds__(256, 4)
+__global__ void __launch_bounds__(256, INTERLEAVED ? 6 : 4)
     pg_rotary_kernel(const __grid_constant__ RotaryParams p) {
-  constexpr int V = 16 / sizeof(T), U = INTERLEAVED ? 4 : 2;
+  constexpr int V = 16 / sizeof(T), U = 2;
   constexpr int E = INTERLEAVED ? V / 2 : V;  // table entries of a chunk
   pdl_launch_dependents();
   pdl_wait_primary();

@@ -70,8 +70,9 @@ class Int4PagePool:
         device, tokens, kv_heads = records.device, slots.numel(), self.kv_heads
         slot_ptr = check_token_index(slots, "slots", tokens, device)
         if key_out is None and value_out is None:
-            key_out, value_out = torch.empty((2, tokens, kv_heads, HEAD_DIM), dtype=dtype,
-                                             device=device).unbind(0)
+            shape, strides = (tokens, kv_heads, HEAD_DIM), (kv_heads * HEAD_DIM, HEAD_DIM, 1)
+            key_out = torch.empty_strided(shape, strides, dtype=dtype, device=device)
+            value_out = torch.empty_strided(shape, strides, dtype=dtype, device=device)
         else:
             shape = (tokens, kv_heads, HEAD_DIM)
             for name, t in (("key_out", key_out), ("value_out", value_out)):
