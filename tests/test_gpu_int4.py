@@ -538,3 +538,13 @@ def test_prompt_then_decode_steps(cuda_lib):
         a.host = cpu(pool.records)
         a.check(out, lse)
     assert read_device_error() == 0
+
+
+def test_plan_rounds_only_its_own_split(cuda_lib):
+    a = Attend([4096], hkv=8, seed=13)
+    assert a.wrapper.split_pages == 8
+    a.check(*a.run())
+    a.split = 5
+    a.plan()
+    assert a.wrapper.split_pages == 5
+    a.check(*a.run())

@@ -137,3 +137,15 @@ def test_packed_arguments_have_the_structure_s_layout(structure):
         value = getattr(a, name)
         got += list(value) if isinstance(value, ctypes.Array) else [value]
     assert got == list(range(1, count + 1))
+
+
+def test_automatic_splits_are_whole_pairs_of_four_warps():
+    from pagegauge_b200.wrapper import Int4DecodeWrapper, plan_items
+
+    assert Int4DecodeWrapper._split_multiple == 8
+    # What plan() does with the planner's automatic split.
+    indptr = np.array([0, 256], np.int32)
+    _, _, info = plan_items(1, 8, indptr, None, 0, 0, 148)
+    split = -(-info.split_pages[0] // 8) * 8
+    items, off, info = plan_items(1, 8, indptr, None, split, split, 148)
+    assert info.split_pages[0] == split == 8 and off[-1] == 8 * 32
