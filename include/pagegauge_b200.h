@@ -499,7 +499,10 @@ typedef struct pg_int4_decode_args {
   int64_t num_pages;
   const int32_t* indices;       /* device page ids */
   const int32_t* last_page_len; /* device [B] */
-  const pg_decode_item* items;  /* device, from pg_decode_plan */
+  const pg_decode_item* items;  /* device, from pg_decode_plan, in any order
+                                   (largest first balances ragged batches) */
+  const int32_t* item_slots;    /* device [num_items]: each item's place in the
+                                   planner's order; NULL: items are in it */
   const int32_t* item_off;      /* device [B*Hkv+1] */
   float* part_o;                /* device workspace [num_items*group*128] */
   float* part_lse;              /* device workspace [num_items*group] */

@@ -103,8 +103,8 @@ class PgInt4DecodeArgs(ctypes.Structure):
         ("out", c_vp), ("out_stride_b", c_i64), ("out_stride_h", c_i64),
         ("lse_out", c_vp), ("value_center", c_vp), ("vc_stride_b", c_i64),
         ("records", c_vp), ("num_pages", c_i64), ("indices", c_vp), ("last_page_len", c_vp),
-        ("items", c_vp), ("item_off", c_vp), ("part_o", c_vp), ("part_lse", c_vp),
-        ("work_counter", c_vp),
+        ("items", c_vp), ("item_slots", c_vp), ("item_off", c_vp), ("part_o", c_vp),
+        ("part_lse", c_vp), ("work_counter", c_vp),
         ("num_items", c_i32), ("batch", c_i32), ("kv_heads", c_i32), ("group", c_i32),
         ("final_mode", c_i32), ("dtype", c_i32), ("sm_scale", ctypes.c_float),
         ("reserved", c_i32),

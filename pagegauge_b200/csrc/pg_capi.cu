@@ -1332,6 +1332,7 @@ int32_t pg_decode_int4_run(const pg_int4_decode_args* a, void* stream) {
   p.indices = a->indices;
   p.last_len = a->last_page_len;
   p.items = reinterpret_cast<const pg::DecodeItem*>(a->items);
+  p.item_slots = a->item_slots;
   p.item_off = a->item_off;
   p.num_items = a->num_items;
   p.batch = a->batch;

@@ -20,9 +20,9 @@
 // -8 qs_g is the initial accumulator of group g's products, and the last
 // term one TF32 product with qs split in two.  For the values
 //   O_d = sum_t (P_t s_tg) z_td - 8 sum_t (P_t s_tg) + sum_t P_t m_tg
-// where P s is formed in FP32 and rounded once to FP16, and the two last sums
-// come from tensor-core products of the same rounded operands, so that a
-// rounding of P s weighs (z - 8) s and not z s.  P <= 4 (the running maximum
+// where P s is formed in FP32 and rounded once to FP16, and the sum times 8
+// comes from tensor-core products of the same rounded operands, so that a
+// rounding of P s weighs (z - 8) s and not z s; the last sum is FP32.  P <= 4 (the running maximum
 // is raised when a score passes it by 2 in log2), so P s <= 4 * 8734.
 #pragma once
 
@@ -39,6 +39,7 @@ struct Int4DecodeParams {
   const int32_t* indices;
   const int32_t* last_len;
   const DecodeItem* items;
+  const int32_t* item_slots;  // where an item's partial state goes (null: its index)
   const int32_t* item_off;
   int32_t num_items, batch, hkv, group;
   float sm_scale_log2;
@@ -141,7 +142,8 @@ struct Int4State {
   // Tile 2j + e, rows g: dims d = 32j + 4g + 2e; rows g + 8: d and d + 1 as
   // z_d + 16 z_(d+1) (one AND less than the two nibbles apart).
   float o[8][4];
-  float sums[4];  // sum P s_g (rows 0-3, NARROW: 0-1), sum P m_g (rows 4-7)
+  float sums[4];     // row k: sum of part k's rounded P s
+  float mid[4][2];   // sum P m of part k (this lane's tokens); NARROW: k < 2
 };
 
 // NARROW (GQA group <= 4): columns 4-7 of the products repeat the query rows
@@ -274,6 +276,10 @@ __device__ __forceinline__ void pages_int4(const uint8_t* rec, const Int4Query& 
       for (int i = 0; i < 4; ++i) st.o[j][i] *= a[i & 1];
 #pragma unroll
     for (int i = 0; i < 4; ++i) st.sums[i] *= a[i & 1];
+#pragma unroll
+    for (int k = 0; k < (NARROW ? 2 : 4); ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) st.mid[k][i] *= a[i];
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -284,43 +290,46 @@ __device__ __forceinline__ void pages_int4(const uint8_t* rec, const Int4Query& 
     const float p3 = fast_exp2(fmaf(s[i][3], iq.cr[1], -st.ref[1]));
     st.l[0] += p0 + p2;
     st.l[1] += p1 + p3;
-    // Rows 4 + j of the sums: P m_j of tokens 2t, 2t+1 and 2t+8, 2t+9.
-    const unsigned short* mid =
-        reinterpret_cast<const unsigned short*>(page + kInt4ValueMeta + 8) + (g & 3) + 16 * t;
-    uint32_t ma = mid[0] | (static_cast<uint32_t>(mid[8]) << 16);
-    uint32_t mb = mid[64] | (static_cast<uint32_t>(mid[72]) << 16);
-    if (g < 4) ma = mb = 0u;
-    // Value scales of tokens g and g + 8, four groups or (NARROW) the two of
-    // this lane's columns.
+    // Value scales and midpoints of tokens g and g + 8: four groups', or
+    // (NARROW) the two of this lane's columns.
     constexpr int kParts = NARROW ? 2 : 4;
     float wa[kParts], wb[kParts];
-    if constexpr (NARROW) {
-      const __half* sa = reinterpret_cast<const __half*>(page + kInt4ValueMeta + 16 * g) + (t >> 1);
+    {
+      float ma[kParts], mb[kParts];
+      const uint8_t* at = page + kInt4ValueMeta + 16 * g;
+      if constexpr (NARROW) {
+        const __half* sa = reinterpret_cast<const __half*>(at) + (t >> 1);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        wa[k] = __half2float(sa[2 * k]);
-        wb[k] = __half2float(sa[64 + 2 * k]);
+        for (int k = 0; k < 2; ++k) {
+          wa[k] = __half2float(sa[2 * k]);
+          ma[k] = __half2float(sa[4 + 2 * k]);
+          wb[k] = __half2float(sa[64 + 2 * k]);
+          mb[k] = __half2float(sa[68 + 2 * k]);
+        }
+      } else {
+        const uint4 x = lds128(at, 0), y = lds128(at, 128);
+        const float2 a0 = half2_float2(x.x), a1 = half2_float2(x.y);
+        const float2 a2 = half2_float2(x.z), a3 = half2_float2(x.w);
+        const float2 b0 = half2_float2(y.x), b1 = half2_float2(y.y);
+        const float2 b2 = half2_float2(y.z), b3 = half2_float2(y.w);
+        wa[0] = a0.x; wa[1] = a0.y; wa[kParts - 2] = a1.x; wa[kParts - 1] = a1.y;
+        ma[0] = a2.x; ma[1] = a2.y; ma[kParts - 2] = a3.x; ma[kParts - 1] = a3.y;
+        wb[0] = b0.x; wb[1] = b0.y; wb[kParts - 2] = b1.x; wb[kParts - 1] = b1.y;
+        mb[0] = b2.x; mb[1] = b2.y; mb[kParts - 2] = b3.x; mb[kParts - 1] = b3.y;
       }
-    } else {
-      const uint2 va = *reinterpret_cast<const uint2*>(page + kInt4ValueMeta + 16 * g);
-      const uint2 vb = *reinterpret_cast<const uint2*>(page + kInt4ValueMeta + 128 + 16 * g);
-      const float2 a0 = half2_float2(va.x), a1 = half2_float2(va.y);
-      const float2 b0 = half2_float2(vb.x), b1 = half2_float2(vb.y);
-      wa[0] = a0.x; wa[1] = a0.y; wa[kParts - 2] = a1.x; wa[kParts - 1] = a1.y;
-      wb[0] = b0.x; wb[1] = b0.y; wb[kParts - 2] = b1.x; wb[kParts - 1] = b1.y;
-    }
-    if (masked) {
-      const int n = valid[i];
-      if (2 * t + 1 >= n) ma = 2 * t < n ? ma & 0xffffu : 0u;
-      if (2 * t + 9 >= n) mb = 2 * t + 8 < n ? mb & 0xffffu : 0u;
+      if (masked) {
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) {
+          if (g >= valid[i]) wa[k] = ma[k] = 0.f;
+          if (g + 8 >= valid[i]) wb[k] = mb[k] = 0.f;
+        }
+      }
 #pragma unroll
       for (int k = 0; k < kParts; ++k) {
-        if (g >= n) wa[k] = 0.f;
-        if (g + 8 >= n) wb[k] = 0.f;
+        st.mid[k][0] = fmaf(p0, ma[k], fmaf(p2, mb[k], st.mid[k][0]));
+        st.mid[k][1] = fmaf(p1, ma[k], fmaf(p3, mb[k], st.mid[k][1]));
       }
     }
-    mma_16816_acc(st.sums, ma, 0u, mb, 0u, transpose_8x8(pack_half2(p0, p1)),
-                  transpose_8x8(pack_half2(p2, p3)));
     // Codes of tokens 2t, 2t+1 and 2t+8, 2t+9.
     const uint8_t* codes = page + kInt4Value + 64 * t + 8 * g;
     const uint2 c00 = *reinterpret_cast<const uint2*>(codes);
@@ -371,7 +380,9 @@ __device__ __forceinline__ int int4_warp_pages(int count, int warp) {
 // counter, which the last block to ask sets back to zero).  An item's page ids
 // are read, and its first pages requested, before the item ahead of it is
 // finished, so only the first item of a block waits for them.  Which block
-// takes an item changes no result: partial states are stored by item.
+// takes an item changes no result: partial states are stored by item.  The
+// plan lists the largest items first, so that the last ones are short and the
+// blocks of one SM get items of all sizes.
 template <typename T, bool NARROW>
 __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
     pg_decode_int4_kernel(const __grid_constant__ Int4DecodeParams p) {
@@ -408,7 +419,6 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
                   kInt4Record);
   }
   pdl_wait_primary();
-  const uint64_t policy = l2_evict_first_policy();
   // Lane u holds the record of the warp's page u (at most 32 per warp) and
   // copies it itself; ids outside the pool leave their page out.
   const uint8_t* mine = nullptr;
@@ -431,7 +441,7 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
     __syncwarp();
     if ((lane >> 1) == u && mine != nullptr)
       bulk_load_hint(ring + (2 * at + (lane & 1)) * kInt4Record, mine, kInt4Record, bars + at,
-                     policy);
+                     l2_evict_first_policy());
   };
   int slot = 0;
   uint32_t phase = 0;
@@ -459,9 +469,6 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
     const int n_pages = item.count & 0x7fffffff, n_pairs = (n_w + 1) >> 1;
     const bool more = next_index < p.num_items;
     if (more && threadIdx.x == 0) s_next[parity] = take();
-    DecodeItem next;
-    next.count = 0;
-    if (more) next = p.items[next_index];
     // Tokens that count in the warp's last page, if it is the request's last.
     int tail = kPage;
     if (item.count < 0 && n_w > 0 && warp + kInt4Warps * (n_w - 1) == n_pages - 1) {
@@ -470,10 +477,12 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
     }
     Int4Query iq;
     load_query_int4<T, NARROW>(p, r, h, g, t, iq);
-    const int next_w = int4_warp_pages(next.count, warp);
-    const int next_id = lane < next_w ? load_volatile(p.indices + next.idx_begin + warp +
-                                                      kInt4Warps * lane)
-                                      : 0;
+    int next_id = 0;
+    if (more) {
+      const DecodeItem next = p.items[next_index];
+      if (lane < int4_warp_pages(next.count, warp))
+        next_id = load_volatile(p.indices + next.idx_begin + warp + kInt4Warps * lane);
+    }
     Int4State st;
     st.m[0] = st.m[1] = kNegInf;
     st.l[0] = st.l[1] = 0.f;
@@ -483,7 +492,7 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
 #pragma unroll
       for (int i = 0; i < 4; ++i) st.o[j][i] = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) st.sums[i] = 0.f;
+    for (int i = 0; i < 4; ++i) st.sums[i] = st.mid[i][0] = st.mid[i][1] = 0.f;
 
     for (int u = 0; u < n_pairs && ok; ++u) {
       const bool waited = mbar_wait_bounded(bars + slot, phase);
@@ -521,13 +530,18 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
       }
     }
     if (more) {
-      n_w = ok ? next_w : 0;
-      resolve(next_id, next, n_w);
+      item = p.items[next_index];
+      n_w = ok ? int4_warp_pages(item.count, warp) : 0;
+      resolve(next_id, item, n_w);
       issue_first();
     }
 
-    // Warp totals: l over the 8 token lanes, then the output rows.
+    // Warp totals over the 8 token lanes, then the output rows.
     const float l0 = warp_sum_xor_g(st.l[0]), l1 = warp_sum_xor_g(st.l[1]);
+#pragma unroll
+    for (int k = 0; k < (NARROW ? 2 : 4); ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) st.mid[k][i] = warp_sum_xor_g(st.mid[k][i]);
     __syncthreads();  // the combine buffer is free
     float* cm = reinterpret_cast<float*>(smem_int4 + kInt4CombineAt);  // [W][8]
     float* cl = cm + kInt4Warps * 8;                                   // [W][8]
@@ -545,8 +559,8 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
       float* row = co + (warp * 8 + q) * kCoStride;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float add = __shfl_sync(0xffffffffu, st.sums[i], 16 + 4 * j + t) -
-                          8.f * __shfl_sync(0xffffffffu, st.sums[i], 4 * (NARROW ? j >> 1 : j) + t);
+        const int k = NARROW ? j >> 1 : j;
+        const float add = st.mid[k][i] - 8.f * __shfl_sync(0xffffffffu, st.sums[i], 4 * k + t);
         if (q < p.group && (!NARROW || (t >> 1) == (j & 1))) {
           const float* a = st.o[2 * j];
           const float* b = st.o[2 * j + 1];
@@ -584,7 +598,9 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
         int4_store_out<T>(p, r, h, q, d + 2, O.z, lse);
         int4_store_out<T>(p, r, h, q, d + 3, O.w, lse);
       } else {
-        const int64_t base = static_cast<int64_t>(index) * p.group + q;
+        const int64_t base =
+            static_cast<int64_t>(p.item_slots != nullptr ? p.item_slots[index] : index) * p.group +
+            q;
         *reinterpret_cast<float4*>(p.part_o + base * kHeadDim + d) = O;
         if (d == 0) p.part_lse[base] = lse;
       }
@@ -592,7 +608,6 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
     if (!more) break;
     index = next_index;
     next_index = s_next[parity];  // stored ahead of the two barriers above
-    item = next;
   }
 }
 

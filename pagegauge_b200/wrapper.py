@@ -85,7 +85,7 @@ class _Workspace:
             raise ValueError("workspace must be a contiguous CUDA uint8 tensor")
         self.buffer = buffer
 
-    def layout(self, num_items: int, num_offsets: int, group: int):
+    def layout(self, num_items: int, num_offsets: int, group: int, slots: bool = False):
         def align(x: int) -> int:
             return (x + 255) // 256 * 256
 
@@ -94,7 +94,8 @@ class _Workspace:
         sem_b = align(num_offsets * 4)
         lse_b = align(max(num_items, 1) * group * 4)
         o_b = align(max(num_items, 1) * group * HEAD_DIM * 4)
-        total = items_b + off_b + sem_b + lse_b + o_b
+        used = items_b + off_b + sem_b + lse_b + o_b
+        total = used + (align(max(num_items, 1) * 4) if slots else 0)
         if total > self.buffer.numel():
             raise RuntimeError(
                 f"workspace of {self.buffer.numel()} bytes is too small for {num_items} work items "
@@ -104,22 +105,32 @@ class _Workspace:
         off = base[items_b:items_b + off_b]
         sem = base[items_b + off_b:items_b + off_b + sem_b]
         lse = base[items_b + off_b + sem_b:items_b + off_b + sem_b + lse_b]
-        part_o = base[items_b + off_b + sem_b + lse_b:total]
-        return items, off, sem, lse, part_o
+        part_o = base[items_b + off_b + sem_b + lse_b:used]
+        return items, off, sem, lse, part_o, base[used:total]
 
 
 class PagedDecodePlan:
     """Device-resident work list of one plan."""
 
     def __init__(self, ws: _Workspace, items: np.ndarray, off: np.ndarray, info, batch: int,
-                 kv_heads: int, group: int):
+                 kv_heads: int, group: int, largest_first: bool = False):
+        """``largest_first`` lists the items by falling page count, with each
+        item's place in the planner's order beside it (``slots_ptr``)."""
         self.num_items = int(info.num_items)
         self.single = bool(info.single_item_per_head)
         self.split_pages = (int(info.split_pages[0]), int(info.split_pages[1]))
         self.warps = int(info.warps_per_cta)
         self.batch, self.kv_heads, self.group = batch, kv_heads, group
-        d_items, d_off, d_sem, d_lse, d_o = ws.layout(self.num_items, off.size, group)
+        d_items, d_off, d_sem, d_lse, d_o, d_slots = ws.layout(self.num_items, off.size, group,
+                                                               largest_first)
         d_sem.zero_()  # per-head arrival counters of the fused merge
+        self.slots_ptr = 0
+        if largest_first and self.num_items:
+            order = np.argsort(-(items[:, 3] & 0x7FFFFFFF), kind="stable").astype(np.int32)
+            items = np.ascontiguousarray(items[order])
+            d_slots[:order.size * 4].copy_(torch.from_numpy(order.view(np.uint8)),
+                                           non_blocking=False)
+            self.slots_ptr = d_slots.data_ptr()
         if self.num_items:
             src = torch.from_numpy(items.view(np.uint8).reshape(-1))
             d_items[:src.numel()].copy_(src, non_blocking=False)
@@ -216,6 +227,7 @@ class BatchDecodeWithPagedKVCacheWrapper:
     """
 
     _split_multiple = 1  # of an automatic split, in pages
+    _largest_first = False  # the order of the work items
 
     def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD",
                  use_cuda_graph: bool = False, use_tensor_cores: bool = True,
@@ -305,7 +317,7 @@ class BatchDecodeWithPagedKVCacheWrapper:
             split = -(-info.split_pages[0] // self._split_multiple) * self._split_multiple
             items, off, info = plan_items(batch, num_kv_heads, seg0, seg1, split, split, sms)
         self._plan = PagedDecodePlan(self._ws, items, off, info, batch, num_kv_heads,
-                                     num_qo_heads // num_kv_heads)
+                                     num_qo_heads // num_kv_heads, self._largest_first)
         self._indices = dev_indices
         self._last_len = dev_last
         self._num_qo_heads = num_qo_heads
@@ -384,6 +396,7 @@ class Int4DecodeWrapper(BatchDecodeWithPagedKVCacheWrapper):
     # rounded up to whole pairs (4,096 tokens: 5 pages 7.9 us, 8 pages 7.1 us;
     # 16,384: 19 pages 11.5 us, 24 pages 10.7 us).
     _split_multiple = 8
+    _largest_first = True
 
     def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD", **kwargs):
         super().__init__(float_workspace_buffer, kv_layout, **kwargs)
@@ -448,8 +461,8 @@ class Int4DecodeWrapper(BatchDecodeWithPagedKVCacheWrapper):
         _lib.launch("pg_decode_int4_run", device, _PACK_INT4_DECODE(
             q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], lse_ptr, vc_ptr,
             kv_heads * HEAD_DIM, records_ptr, pages, self._indices.data_ptr(),
-            self._last_len.data_ptr(), plan.items_ptr, plan.off_ptr, plan.o_ptr, plan.lse_ptr,
-            plan.sem_ptr, plan.num_items, plan.batch, kv_heads, plan.group,
+            self._last_len.data_ptr(), plan.items_ptr, plan.slots_ptr, plan.off_ptr, plan.o_ptr,
+            plan.lse_ptr, plan.sem_ptr, plan.num_items, plan.batch, kv_heads, plan.group,
             plan.single and plan.num_items > 0, DTYPES[dtype],
             self._sm_scale if sm_scale is None else sm_scale, 0))
         return (out, lse) if return_lse else out

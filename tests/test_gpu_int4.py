@@ -2,9 +2,9 @@
 FP32 steps, decode attention against float64 from the values held.
 
 Attention bound.  With weights p (float64) over tokens, the kernel rounds
-P * s and P to FP16 (2^-11 relative, and half a subnormal step 2^-25) before
-the tensor-core products, so an output dim is off by at most
-  2^-11 sum p (|z - 8| s + |m|) + 2^-25 sum (|z - 8| + |m|) / l,
+P * s to FP16 (2^-11 relative, and half a subnormal step 2^-25) before the
+tensor-core products, so an output dim is off by at most
+  2^-11 sum p |z - 8| s + 2^-25 sum |z - 8| / l,
 l >= 1/4 the sum of the unnormalised weights (a weight of 1/4 is the least
 the largest has).  A score's FP32 sums (at most 2^5 roundings of partial sums
 that do not pass S = scale sum |q| (|z - 8| s + |m|)) move p by the relative
@@ -319,11 +319,11 @@ class Attend:
                 size = scale * (np.abs(q[r, heads]) @ (np.abs(ka) + np.abs(km)).T).max(-1)
                 e = 2.0 ** -19 * size + 2.0 ** -18
                 big = np.abs(va) + np.abs(vm)
-                bound = 2.0 ** -11 * (p @ big) + 2 * e[:, None] * (p @ big)
+                bound = 2.0 ** -11 * (p @ np.abs(va)) + 2 * e[:, None] * (p @ big)
                 # a subnormal step of each weight, over a sum of weights that
                 # is at least a quarter of (sum p) / (max p)
                 least = 1 / p.max(-1, keepdims=True) / 4
-                bound += 2.0 ** -25 * (8 * n + np.abs(vm).sum(0)) / np.maximum(least, 0.25)
+                bound += 2.0 ** -25 * 8 * n / np.maximum(least, 0.25)
                 if c is not None:
                     exp = exp + c[r, h]
                 bound = bound + eps * (np.abs(exp) + bound) + 2.0 ** -25 + 2.0 ** -23 * np.abs(exp)
