@@ -99,12 +99,13 @@ _PACK_ROTARY = _lib.packer(_lib.PgRotaryArgs).pack
 def check_tables(cosine: torch.Tensor, sine: torch.Tensor, device: torch.device,
                  head_dim: int) -> tuple[int, int, int]:
     """(rows, row stride, pairs) of a table pair [positions, pairs]."""
+    shape = cosine.shape
     if (cosine.dtype is not torch.float32 or sine.dtype is not torch.float32
-            or cosine.dim() != 2 or cosine.shape != sine.shape):
+            or len(shape) != 2 or shape != sine.shape):
         raise ValueError("cosine and sine must be matching float32 [positions, pairs] tables")
     if cosine.device != device or sine.device != device:
         raise ValueError("rotary tables must be on the rows' device")
-    rows, pairs = cosine.shape
+    rows, pairs = shape
     strides = cosine.stride()
     if strides != sine.stride() or strides[1] != 1 or strides[0] < pairs:
         raise ValueError("rotary tables must have equal strides and contiguous rows")
@@ -123,12 +124,13 @@ def check_token_index(t: torch.Tensor, name: str, tokens: int, device: torch.dev
 
 def check_output(out: torch.Tensor, like: torch.Tensor, name: str) -> tuple[int, ...]:
     """The strides of an output that takes ``like``'s rows."""
-    if out.shape != like.shape or out.dtype is not like.dtype or out.device != like.device:
+    shape = out.shape
+    if shape != like.shape or out.dtype is not like.dtype or out.device != like.device:
         raise ValueError(f"{name} must have its input's shape, dtype and device")
     strides = out.stride()
     if strides[2] != 1:
         raise ValueError(f"{name} must have a contiguous last dimension")
-    if strides[0] <= 0 < out.size(0) - 1 or strides[1] <= 0 < out.size(1) - 1:
+    if (strides[0] <= 0 and shape[0] > 1) or (strides[1] <= 0 and shape[1] > 1):
         raise ValueError(f"{name} must not be expanded")
     return strides
 
@@ -136,13 +138,13 @@ def check_output(out: torch.Tensor, like: torch.Tensor, name: str) -> tuple[int,
 def check_rows(x: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device,
                tokens: int, head_dim: int) -> tuple[int, tuple[int, ...]]:
     """(heads, strides) of rows [tokens, heads, head_dim]."""
-    if x.dtype is not dtype or x.device != device or not x.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor of the query's device and dtype")
     shape = x.shape
+    if x.dtype is not dtype or x.device != device:
+        raise ValueError(f"{name} must have the query's device and dtype")
     if len(shape) != 3 or shape[0] != tokens or shape[2] != head_dim:
         raise ValueError(f"{name} must be [{tokens}, heads, {head_dim}]")
     strides = x.stride()
-    if strides[2] != 1 and x.numel():
+    if strides[2] != 1 and tokens:
         raise ValueError(f"{name} must have a contiguous last dimension")
     return shape[1], strides
 
@@ -165,8 +167,8 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, cosine: torch.Te
     dtype, device = query.dtype, query.device
     if dtype not in DTYPES:
         raise ValueError("rows must be float16, bfloat16 or float32")
-    if query.dim() != 3:
-        raise ValueError("query must be [tokens, heads, head_dim]")
+    if not query.is_cuda or query.dim() != 3:
+        raise ValueError("query must be a CUDA tensor [tokens, heads, head_dim]")
     tokens, _, head_dim = query.shape
     hq, qs = check_rows(query, "query", dtype, device, tokens, head_dim)
     if query_out is None:

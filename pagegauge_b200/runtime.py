@@ -315,8 +315,8 @@ class AppendExtension:
         dtype, device = query.dtype, query.device
         _require(dtype is torch.float16 or dtype is torch.bfloat16,
                  "query must be float16 or bfloat16")
-        _require(query.dim() == 3, "query must have rank three")
-        tokens = query.size(0)
+        _require(query.is_cuda and query.dim() == 3, "query must be CUDA of rank three")
+        tokens = query.shape[0]
         hq, qs = check_rows(query, "query", dtype, device, tokens, HEAD_DIM)
         kv_heads, ks = check_rows(key, "key", dtype, device, tokens, HEAD_DIM)
         v_heads, vs = check_rows(value, "value", dtype, device, tokens, HEAD_DIM)
@@ -335,15 +335,15 @@ class AppendExtension:
             rk_ptr = rotated_key.data_ptr()
         kc_ptr = vc_ptr = row_ptr = centers = 0
         if key_center is not None and value_center is not None:
-            for name, t in (("key_center", key_center), ("value_center", value_center)):
-                shape = t.shape
-                _require(t.device == device and t.dtype is dtype and t.is_contiguous()
-                         and len(shape) == 3 and shape[0] > 0 and shape[1] == kv_heads
-                         and shape[2] == HEAD_DIM,
-                         f"{name} must be contiguous [rows,{kv_heads},{HEAD_DIM}] of the "
-                         "query's dtype")
-            centers = key_center.size(0)
-            _require(centers == value_center.size(0), "center row counts must match")
+            shape = key_center.shape
+            if (len(shape) != 3 or shape[0] == 0 or shape[1] != kv_heads or shape[2] != HEAD_DIM
+                    or value_center.shape != shape):
+                raise RuntimeError(f"centers must both be [rows,{kv_heads},{HEAD_DIM}]")
+            for t in (key_center, value_center):
+                if t.dtype is not dtype or t.device != device or not t.is_contiguous():
+                    raise RuntimeError("centers must be contiguous, of the query's dtype and "
+                                       "device")
+            centers = shape[0]
             kc_ptr, vc_ptr = key_center.data_ptr(), value_center.data_ptr()
             if center_rows is not None:
                 row_ptr = check_token_index(center_rows, "center_rows", tokens, device)
