@@ -212,9 +212,9 @@ __device__ __forceinline__ void load_query_int4(const Int4DecodeParams& p, int r
   for (int i = 0; i < 2; ++i) iq.cr[i] = __shfl_sync(0xffffffffu, down, 4 * (2 * t + i));
 }
 
-// Two pages at rec and rec + kInt4Record in shared memory, of which the first
-// valid[i] tokens count (the others' scales may hold anything).
-template <bool NARROW>
+// Two pages at rec and rec + kInt4Record in shared memory.  MASKED: only the
+// first valid[i] tokens count (the others' scales may hold anything).
+template <bool NARROW, bool MASKED>
 __device__ __forceinline__ void pages_int4(const uint8_t* rec, const Int4Query& iq, Int4State& st,
                                            const int* valid, int g, int t) {
   const int lane = 4 * g + t;
@@ -249,8 +249,7 @@ __device__ __forceinline__ void pages_int4(const uint8_t* rec, const Int4Query& 
       s[i][3] = fmaf(wb, acc[3], s[i][3]);
     }
   }
-  const bool masked = valid[0] + valid[1] != 2 * kPage;
-  if (masked) {
+  if constexpr (MASKED) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (g >= valid[i]) s[i][0] = s[i][1] = kNegInf;
@@ -317,7 +316,7 @@ __device__ __forceinline__ void pages_int4(const uint8_t* rec, const Int4Query& 
         wb[0] = b0.x; wb[1] = b0.y; wb[kParts - 2] = b1.x; wb[kParts - 1] = b1.y;
         mb[0] = b2.x; mb[1] = b2.y; mb[kParts - 2] = b3.x; mb[kParts - 1] = b3.y;
       }
-      if (masked) {
+      if constexpr (MASKED) {
 #pragma unroll
         for (int k = 0; k < kParts; ++k) {
           if (g >= valid[i]) wa[k] = ma[k] = 0.f;
@@ -494,6 +493,9 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
 #pragma unroll
     for (int i = 0; i < 4; ++i) st.sums[i] = st.mid[i][0] = st.mid[i][1] = 0.f;
 
+    // Pairs of whole pages; the others (the last pair at most, unless ids were
+    // bad) are masked.
+    const int n_whole = bad_pages != 0u ? 0 : (n_w - (tail != kPage)) >> 1;
     for (int u = 0; u < n_pairs && ok; ++u) {
       const bool waited = mbar_wait_bounded(bars + slot, phase);
       if (!__all_sync(0xffffffffu, waited)) {
@@ -511,17 +513,17 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
         ok = false;
         break;
       }
-      int valid[2] = {kPage, kPage};
-      if (u == n_pairs - 1) {
-        const bool two = (n_w & 1) == 0;
-        valid[0] = two ? kPage : tail;
-        valid[1] = two ? tail : 0;
-      }
-      if (bad_pages != 0u) {
+      const uint8_t* pages = ring + 2 * slot * kInt4Record;
+      if (u < n_whole) {
+        pages_int4<NARROW, false>(pages, iq, st, nullptr, g, t);
+      } else {
+        int valid[2] = {kPage, kPage};
+        if (u == n_pairs - 1) valid[n_w & 1 ? 0 : 1] = tail;
+        if (u == n_pairs - 1 && (n_w & 1)) valid[1] = 0;
         if ((bad_pages >> (2 * u)) & 1u) valid[0] = 0;
         if ((bad_pages >> (2 * u)) & 2u) valid[1] = 0;
+        pages_int4<NARROW, true>(pages, iq, st, valid, g, t);
       }
-      pages_int4<NARROW>(ring + 2 * slot * kInt4Record, iq, st, valid, g, t);
       __syncwarp();
       if (u + kInt4Slots < n_pairs) issue(u + kInt4Slots, slot);
       if (++slot == kInt4Slots) {
