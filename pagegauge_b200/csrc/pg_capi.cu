@@ -1234,12 +1234,16 @@ int32_t pg_rope_append_int4(const pg_int4_append_args* a, void* stream) {
   const bool table16 = aligned(a->cosine, 16) && aligned(a->sine, 16) &&
                        a->table_stride % 4 == 0 && a->pairs % (p.interleaved ? 4 : 8) == 0;
   const bool fast = rows16 && table16;
-  // Few tokens: a warp per row pair.  Else four query row pairs (or a key and
-  // a value row pair) at a time, a token's groups over as many warps as fill
+  const int turn = !fast           ? pg::kTurnAny
+                   : p.interleaved ? pg::kTurnInterleaved
+                   : p.pairs == 64 ? pg::kTurnHalf
+                                   : pg::kTurnPart;
+  // Few tokens: a warp per four rows.  Else eight query rows (or four key and
+  // four value rows) at a time, a token's groups over as many warps as fill
   // the GPU.
-  const int64_t pairs_of_rows = (p.hq + 1) / 2 + 2 * ((p.hkv + 1) / 2);
-  const bool wide = a->tokens * pairs_of_rows > 148 * 32;
-  const int64_t units = wide ? (p.hq + 7) / 8 + (p.hkv + 1) / 2 : pairs_of_rows;
+  const int64_t fours = (p.hq + 3) / 4 + 2 * ((p.hkv + 3) / 4);
+  const bool wide = a->tokens * fours > 148 * 16;
+  const int64_t units = wide ? (p.hq + 7) / 8 + (p.hkv + 3) / 4 : fours;
   p.split = static_cast<int32_t>(
       std::min<int64_t>(units, std::max<int64_t>(1, 148 * 64 / a->tokens)));
   const int64_t warps = a->tokens * p.split;
@@ -1248,16 +1252,15 @@ int32_t pg_rope_append_int4(const pg_int4_append_args* a, void* stream) {
   const int block = wide ? 8 : 2;
   const dim3 grid(static_cast<unsigned>((warps + block - 1) / block));
   using Kernel = void (*)(pg::Int4AppendParams);
-  const Kernel kernels[2][2][2] = {
-      {{pg::pg_rope_append_int4_kernel<__half, false, 1>,
-        pg::pg_rope_append_int4_kernel<__half, false, 4>},
-       {pg::pg_rope_append_int4_kernel<__half, true, 1>,
-        pg::pg_rope_append_int4_kernel<__half, true, 4>}},
-      {{pg::pg_rope_append_int4_kernel<__nv_bfloat16, false, 1>,
-        pg::pg_rope_append_int4_kernel<__nv_bfloat16, false, 4>},
-       {pg::pg_rope_append_int4_kernel<__nv_bfloat16, true, 1>,
-        pg::pg_rope_append_int4_kernel<__nv_bfloat16, true, 4>}}};
-  return launch_pdl(kernels[a->dtype == PG_DTYPE_BF16][fast][wide], grid, dim3(block * 32), 0,
+#define PG_APPEND(T, TURN) \
+  {pg::pg_rope_append_int4_kernel<T, TURN, 1>, pg::pg_rope_append_int4_kernel<T, TURN, 2>}
+#define PG_APPEND_TURNS(T) \
+  {PG_APPEND(T, pg::kTurnAny), PG_APPEND(T, pg::kTurnHalf), \
+   PG_APPEND(T, pg::kTurnInterleaved), PG_APPEND(T, pg::kTurnPart)}
+  const Kernel kernels[2][4][2] = {PG_APPEND_TURNS(__half), PG_APPEND_TURNS(__nv_bfloat16)};
+#undef PG_APPEND_TURNS
+#undef PG_APPEND
+  return launch_pdl(kernels[a->dtype == PG_DTYPE_BF16][turn][wide], grid, dim3(block * 32), 0,
                     static_cast<cudaStream_t>(stream), "rope_append_int4 launch", p);
 }
 

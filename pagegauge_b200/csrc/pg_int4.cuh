@@ -142,33 +142,19 @@ __host__ __device__ constexpr int value_code_row(int tok) {
   return (tok & 8) + 4 * (tok & 1) + ((tok >> 1) & 3);
 }
 
-// Quantise lane m's 8 dims 8m .. 8m+7 of one row (16 lanes per row; lanes
-// 4j .. 4j+3 hold group j).  Returns the 8 codes, dim 8m + i in nibble i.
-// Bound by the ALU pipe (minima, selections, logic run at half rate), so the
-// clamps are taken only by warps that need them, and rounding and packing are
-// FP32 additions: r + 1.5 2^23 has rint(r) in its low bits, and four codes
-// c0 + 16 c1 + 256 c2 + 4096 c3 are exact.  (57,304 tokens of 32 + 16 rows:
-// 321 us with a clamp, a conversion and a shift per element, 222 us so.)
-__device__ __forceinline__ uint32_t int4_quantize8(float* x, __half& scale, __half& mid) {
-  float lo = min3_nan(x[0], x[1], x[2]), hi = max3_nan(x[0], x[1], x[2]);
-  lo = min3_nan(min3_nan(lo, x[3], x[4]), x[5], min_nan(x[6], x[7]));
-  hi = max3_nan(max3_nan(hi, x[3], x[4]), x[5], max_nan(x[6], x[7]));
-#pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
-  if (__any_sync(0xffffffffu, !(hi <= 65504.f && lo >= -65504.f))) {
-    lo = min_nan(max_nan(lo, -65504.f), 65504.f);
-    hi = min_nan(max_nan(hi, -65504.f), 65504.f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = min_nan(max_nan(x[i], -65504.f), 65504.f);
-  }
-  scale = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
+// Scale, midpoint and codes of one lane's 8 dims of a group, four lanes (l & 3)
+// to a group.  Returns the 8 codes, the first dim in nibble 0; meta: the
+// scale's bits and, in the upper half, the midpoint's.  lo, hi: the group's
+// extremes, which the caller has clamped with x.
+__device__ __forceinline__ uint32_t int4_codes8(float* x, float lo, float hi, bool& clamped,
+                                                uint32_t& meta) {
+  const __half scale = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
   const float s = __half2float(scale);
-  mid = __float2half_rn(__fadd_rn(lo, 8.f * s));
+  const __half mid = __float2half_rn(__fadd_rn(lo, 8.f * s));
   const float m = __half2float(mid);
   const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+  meta = static_cast<uint32_t>(__half_as_ushort(scale)) |
+         (static_cast<uint32_t>(__half_as_ushort(mid)) << 16);
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
     const float2 r = mul2(add2(make_float2(x[i], x[i + 1]), make_float2(-m, -m)),
@@ -179,9 +165,9 @@ __device__ __forceinline__ uint32_t int4_quantize8(float* x, __half& scale, __ha
   // The map is monotonic, so its extremes say whether any code needs a clamp
   // (where the midpoint's rounding is a large part of a step, or for a NaN,
   // which keeps code 0: its group's scale and midpoint are NaN).
-  const bool inside = __fmul_rn(__fsub_rn(lo, m), inv) >= -8.5f &&
-                      __fmul_rn(__fsub_rn(hi, m), inv) < 7.5f;
-  if (__any_sync(0xffffffffu, !inside)) {
+  clamped = !(__fmul_rn(__fsub_rn(lo, m), inv) >= -8.5f &&
+              __fmul_rn(__fsub_rn(hi, m), inv) < 7.5f);
+  if (__any_sync(0xffffffffu, clamped)) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = fminf(fmaxf(x[i], -8.f), 7.f);
   }
@@ -201,6 +187,44 @@ __device__ __forceinline__ uint32_t int4_quantize8(float* x, __half& scale, __ha
     half[i] = __float_as_uint(__fadd_rn(sum, 8388608.f));
   }
   return prmt(half[0], half[1], 0x5410u);
+}
+
+// Quantise one row of 8 lanes: lane l holds dims 8l .. 8l+7 (a) and
+// 64 + 8l .. (b), so lanes 0-3 and 4-7 hold groups 0, 1 (a) and 2, 3 (b).
+// Bound by the ALU pipe (minima, selections, logic run at half rate), so the
+// clamps are taken only by warps that need them, and rounding and packing are
+// FP32 additions: r + 1.5 2^23 has rint(r) in its low bits, and four codes
+// c0 + 16 c1 + 256 c2 + 4096 c3 are exact.
+__device__ __forceinline__ void int4_quantize16(float* a, float* b, uint32_t* codes,
+                                                uint32_t* meta) {
+  float lo[2], hi[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const float* x = k == 0 ? a : b;
+    lo[k] = min3_nan(min3_nan(x[0], x[1], x[2]), min3_nan(x[3], x[4], x[5]), min_nan(x[6], x[7]));
+    hi[k] = max3_nan(max3_nan(x[0], x[1], x[2]), max3_nan(x[3], x[4], x[5]), max_nan(x[6], x[7]));
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      lo[k] = min_nan(lo[k], __shfl_xor_sync(0xffffffffu, lo[k], o));
+      hi[k] = max_nan(hi[k], __shfl_xor_sync(0xffffffffu, hi[k], o));
+    }
+  }
+  const bool fits = max_nan(hi[0], hi[1]) <= 65504.f && min_nan(lo[0], lo[1]) >= -65504.f;
+  if (__any_sync(0xffffffffu, !fits)) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      lo[k] = min_nan(max_nan(lo[k], -65504.f), 65504.f);
+      hi[k] = min_nan(max_nan(hi[k], -65504.f), 65504.f);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      a[i] = min_nan(max_nan(a[i], -65504.f), 65504.f);
+      b[i] = min_nan(max_nan(b[i], -65504.f), 65504.f);
+    }
+  }
+  bool clamped;
+  codes[0] = int4_codes8(a, lo[0], hi[0], clamped, meta[0]);
+  codes[1] = int4_codes8(b, lo[1], hi[1], clamped, meta[1]);
 }
 
 struct Int4AppendParams {
@@ -230,60 +254,114 @@ struct Int4AppendParams {
   int* error_flag;
 };
 
-// Lane m's 8 dims of a row, rotated (raw: the row's elements 8m .. 8m + 7,
-// base: its element 0).  Half layout: dims (d, d + pairs) turn together;
-// interleaved: (2j, 2j + 1).  c, s: this lane's table entries, or read from
-// the rows here if !FAST.
-template <typename T, bool FAST>
-__device__ __forceinline__ void rotate8(float* x, const uint4& raw, const T* base, int m,
-                                        int pairs, bool interleaved, const float* c,
-                                        const float* s, const float* cos_row,
-                                        const float* sin_row) {
-  unpack8<T>(raw, x);
-  if (interleaved) {
+// How an append rotates: rows and tables that are not 16-byte aligned, or
+// parts that are not whole 16-byte chunks (kTurnAny); the whole head in half
+// layout, whose partner dims lie in one lane (kTurnHalf); neighbouring pairs
+// (kTurnInterleaved); part of the head in half layout (kTurnPart).
+constexpr int kTurnAny = 0, kTurnHalf = 1, kTurnInterleaved = 2, kTurnPart = 3;
+
+// A token's table rows and lane l's entries of them: kTurnHalf 8l .. 8l+7,
+// kTurnInterleaved 4l .. 4l+3 and 32 + 4l ..
+struct Int4Turn {
+  const float* cos_row;
+  const float* sin_row;
+  float c[8], s[8];
+  int pairs, l;
+  bool interleaved;  // kTurnAny
+};
+
+// 8 dims d .. d + 7 (a chunk) of a row with partner dims o.
+template <bool FIRST>
+__device__ __forceinline__ void turn_half(float* x, const float* o, const float* c,
+                                          const float* s) {
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      const int j = 4 * m + (i >> 1);
-      if (j >= pairs) continue;
-      const float cj = FAST ? c[i >> 1] : cos_row[j], sj = FAST ? s[i >> 1] : sin_row[j];
-      const float a = x[i], b = x[i + 1];
-      x[i] = __fsub_rn(__fmul_rn(a, cj), __fmul_rn(b, sj));
-      x[i + 1] = __fadd_rn(__fmul_rn(b, cj), __fmul_rn(a, sj));
-    }
-    return;
+  for (int i = 0; i < 8; ++i) {
+    const float a = __fmul_rn(x[i], c[i]), b = __fmul_rn(o[i], s[i]);
+    x[i] = FIRST ? __fsub_rn(a, b) : __fadd_rn(a, b);
   }
-  if constexpr (FAST) {
-    // pairs is a multiple of 8: a lane's partner dims are one lane's.  The
-    // first half's lanes hold -s, so both halves add.
-    const int step = pairs >> 3;
-    const bool turns = m < 2 * step;
-    const int peer = !turns ? m : m < step ? m + step : m - step;
-    uint4 other;
-    other.x = __shfl_sync(0xffffffffu, raw.x, peer, 16);
-    other.y = __shfl_sync(0xffffffffu, raw.y, peer, 16);
-    other.z = __shfl_sync(0xffffffffu, raw.z, peer, 16);
-    other.w = __shfl_sync(0xffffffffu, raw.w, peer, 16);
-    float o[8];
-    unpack8<T>(other, o);
-    if (turns) {
+}
+
+__device__ __forceinline__ void turn_interleaved(float* x, const float* c, const float* s) {
 #pragma unroll
-      for (int i = 0; i < 8; i += 2) {
-        const float2 r = add2(
-            make_float2(__fmul_rn(x[i], c[i]), __fmul_rn(x[i + 1], c[i + 1])),
-            make_float2(__fmul_rn(o[i], s[i]), __fmul_rn(o[i + 1], s[i + 1])));
-        x[i] = r.x;
-        x[i + 1] = r.y;
+  for (int i = 0; i < 4; ++i) {
+    const float a = x[2 * i], b = x[2 * i + 1];
+    x[2 * i] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i]));
+    x[2 * i + 1] = __fadd_rn(__fmul_rn(b, c[i]), __fmul_rn(a, s[i]));
+  }
+}
+
+// Lane l's two chunks of a row (ra, rb as loaded), rotated into a and b.
+template <typename T, int TURN>
+__device__ __forceinline__ void rotate16(float* a, float* b, const uint4& ra, const uint4& rb,
+                                         const T* row, const Int4Turn& t) {
+  unpack8<T>(ra, a);
+  unpack8<T>(rb, b);
+  const int l = t.l, pairs = t.pairs;
+  if constexpr (TURN == kTurnHalf) {
+    float o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = a[i];
+    turn_half<true>(a, b, t.c, t.s);
+    turn_half<false>(b, o, t.c, t.s);
+  } else if constexpr (TURN == kTurnInterleaved) {
+    if (4 * l < pairs) turn_interleaved(a, t.c, t.s);
+    if (32 + 4 * l < pairs) turn_interleaved(b, t.c + 4, t.s + 4);
+  } else if constexpr (TURN == kTurnPart) {
+    // Chunks c < n = pairs / 8 turn with c + n, n < 8: the partner of a first
+    // chunk (a) may be either one of another lane's, that of b is an a.
+    const int n = pairs >> 3;
+    const bool turns_a = l < 2 * n, turns_b = 8 + l < 2 * n;
+    const int peer = !turns_a ? l : l < n ? l + n : l - n;
+    const int peer_b = turns_b ? 8 + l - n : l;
+    uint4 oa, ob;
+    const uint32_t* wa = reinterpret_cast<const uint32_t*>(&ra);
+    const uint32_t* wb = reinterpret_cast<const uint32_t*>(&rb);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t x = __shfl_sync(0xffffffffu, wa[i], peer & 7, 8);
+      const uint32_t y = __shfl_sync(0xffffffffu, wb[i], peer & 7, 8);
+      reinterpret_cast<uint32_t*>(&oa)[i] = peer >= 8 ? y : x;
+      reinterpret_cast<uint32_t*>(&ob)[i] = __shfl_sync(0xffffffffu, wa[i], peer_b, 8);
+    }
+    float o[8], c[8], s[8];
+    auto entries = [&](int j) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        const float4 x = __ldg(reinterpret_cast<const float4*>(t.cos_row + j + i));
+        const float4 y = __ldg(reinterpret_cast<const float4*>(t.sin_row + j + i));
+        c[i] = x.x; c[i + 1] = x.y; c[i + 2] = x.z; c[i + 3] = x.w;
+        s[i] = y.x; s[i + 1] = y.y; s[i + 2] = y.z; s[i + 3] = y.w;
       }
+    };
+    if (turns_a) {
+      entries(8 * (l < n ? l : l - n));
+      unpack8<T>(oa, o);
+      if (l < n)
+        turn_half<true>(a, o, c, s);
+      else
+        turn_half<false>(a, o, c, s);
+    }
+    if (turns_b) {
+      entries(8 * peer_b);
+      unpack8<T>(ob, o);
+      turn_half<false>(b, o, c, s);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int d = 8 * m + i;
-      if (d >= 2 * pairs) continue;
-      const int j = d < pairs ? d : d - pairs;
-      const float o = to_float<T>(base[d < pairs ? d + pairs : j]);
-      const float a = __fmul_rn(x[i], cos_row[j]), b = __fmul_rn(o, sin_row[j]);
-      x[i] = d < pairs ? __fsub_rn(a, b) : __fadd_rn(a, b);
+    for (int k = 0; k < 2; ++k) {
+      float* x = k == 0 ? a : b;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int d = 64 * k + 8 * l + i;
+        if (d >= 2 * pairs) continue;
+        // The partner dim, read from the row (loaded whole before any store).
+        const bool first = t.interleaved ? (d & 1) == 0 : d < pairs;
+        const int j = t.interleaved ? d >> 1 : first ? d : d - pairs;
+        const int other = t.interleaved ? d ^ 1 : first ? d + pairs : j;
+        const float u = __fmul_rn(x[i], t.cos_row[j]);
+        const float w = __fmul_rn(to_float<T>(row[other]), t.sin_row[j]);
+        x[i] = first ? __fsub_rn(u, w) : __fadd_rn(u, w);
+      }
     }
   }
 }
@@ -292,67 +370,77 @@ __device__ __forceinline__ void rotate8(float* x, const uint4& raw, const T* bas
 struct Int4Token {
   int64_t token, page, center;
   int tok;
-  const float* cos_row;
-  const float* sin_row;
 };
 
-// Quantise and store lane m's 8 dims of one row of KV head h (the two halves
-// of a warp hold two rows; a row past the last stores nothing).
+// Quantise and store lane l's two chunks of one row of KV head h (a warp
+// holds four rows; a row past the last stores nothing).
 __device__ __forceinline__ void store_int4_row(const Int4AppendParams& p, const Int4Token& k,
-                                               bool is_key, int h, int m, float* x) {
-  __half scale, mid;
-  const uint32_t codes = int4_quantize8(x, scale, mid);
+                                               bool is_key, int h, int l, float* a, float* b) {
+  uint32_t codes[2], meta[2];
+  int4_quantize16(a, b, codes, meta);
   uint8_t* rec = p.records + (k.page * p.hkv + (h < p.hkv ? h : 0)) * kInt4Record;
-  const int grp = m >> 2;
+  const bool store = h < p.hkv;
   if (is_key) {
-    if (h < p.hkv)
-      *reinterpret_cast<uint32_t*>(rec + k.tok * 64 + (m & 3) * 16 + grp * 4) = codes;
+    uint8_t* at = rec + k.tok * 64 + (l & 3) * 16 + (l >> 2) * 4;
+    if (store) {
+      *reinterpret_cast<uint32_t*>(at) = codes[0];
+      *reinterpret_cast<uint32_t*>(at + 8) = codes[1];
+    }
   } else {
-    // Dims 4a .. 4a+3 of groups 2i and 2i+1 are one word: lanes of an even
-    // group take their first four dims' word, of an odd one the other.
-    const uint32_t other = __shfl_xor_sync(0xffffffffu, codes, 4);
-    const uint32_t word = (grp & 1) ? prmt(other, codes, 0x7632u) : prmt(codes, other, 0x5410u);
-    if (h < p.hkv)
-      *reinterpret_cast<uint32_t*>(rec + kInt4Value + value_code_row(k.tok) * 64 + (m & 3) * 16 +
-                                   (grp & 1) * 8 + (grp >> 1) * 4) = word;
+    // Dims 4e .. 4e+3 of the four groups are 8 bytes: lanes 0-3 take those of
+    // their chunks' first four dims, lanes 4-7 the other four.
+    const uint32_t x = __shfl_xor_sync(0xffffffffu, codes[0], 4);
+    const uint32_t y = __shfl_xor_sync(0xffffffffu, codes[1], 4);
+    const uint2 w = l < 4 ? make_uint2(prmt(codes[0], x, 0x5410u), prmt(codes[1], y, 0x5410u))
+                          : make_uint2(prmt(x, codes[0], 0x7632u), prmt(y, codes[1], 0x7632u));
+    if (store)
+      *reinterpret_cast<uint2*>(rec + kInt4Value + value_code_row(k.tok) * 64 + (l & 3) * 16 +
+                                (l >> 2) * 8) = w;
   }
   // The token's four scales and midpoints as one 16-byte store.
-  const uint32_t sm = static_cast<uint32_t>(__half_as_ushort(scale)) |
-                      (static_cast<uint32_t>(__half_as_ushort(mid)) << 16);
-  const uint32_t s1 = __shfl_down_sync(0xffffffffu, sm, 4, 16);
-  const uint32_t s2 = __shfl_down_sync(0xffffffffu, sm, 8, 16);
-  const uint32_t s3 = __shfl_down_sync(0xffffffffu, sm, 12, 16);
-  if (m == 0 && h < p.hkv)
+  const uint32_t m1 = __shfl_down_sync(0xffffffffu, meta[0], 4, 8);
+  const uint32_t m3 = __shfl_down_sync(0xffffffffu, meta[1], 4, 8);
+  if (l == 0 && store)
     *reinterpret_cast<uint4*>(rec + (is_key ? kInt4KeyMeta : kInt4ValueMeta) + k.tok * 16) =
-        make_uint4(prmt(sm, s1, 0x5410u), prmt(s2, s3, 0x5410u), prmt(sm, s1, 0x7632u),
-                   prmt(s2, s3, 0x7632u));
+        make_uint4(prmt(meta[0], m1, 0x5410u), prmt(meta[1], m3, 0x5410u),
+                   prmt(meta[0], m1, 0x7632u), prmt(meta[1], m3, 0x7632u));
 }
 
 template <typename T>
 __device__ __forceinline__ void subtract_center(const Int4AppendParams& p, const Int4Token& k,
-                                                const void* centers, int h, int m, float* x) {
+                                                const void* centers, int h, int l, float* a,
+                                                float* b) {
   if (centers == nullptr) return;
-  float y[8];
-  unpack8<T>(load8<T, true>(static_cast<const T*>(centers) +
-                            (k.center * p.hkv + h) * kHeadDim + 8 * m), y);
+  const T* row = static_cast<const T*>(centers) + (k.center * p.hkv + h) * kHeadDim + 8 * l;
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    const float2 r = add2(make_float2(x[i], x[i + 1]), make_float2(-y[i], -y[i + 1]));
-    x[i] = r.x;
-    x[i + 1] = r.y;
+  for (int j = 0; j < 2; ++j) {
+    float* x = j == 0 ? a : b;
+    float y[8];
+    unpack8<T>(load8<T, true>(row + 64 * j), y);
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const float2 r = add2(make_float2(x[i], x[i + 1]), make_float2(-y[i], -y[i + 1]));
+      x[i] = r.x;
+      x[i + 1] = r.y;
+    }
   }
 }
 
-// `split` warps share one token.  A warp takes two rows at a time (16 lanes of
-// 8 dims each) and requests U query row pairs, or a key and a value row pair,
-// before it uses the first.  U = 4 where tokens alone fill the GPU: the
-// table entries, slot and position are then read once per token; U = 1 with
-// a warp per row pair for few tokens, where latency is all.
-template <typename T, bool FAST, int U>
-__global__ void __launch_bounds__(256, 4)
+// `split` warps share one token.  A warp takes four rows at a time (8 lanes
+// of two 8-dim chunks each: the partners of the half layout in one lane, so
+// nothing is computed twice) and requests U times four query rows, or four
+// key and four value rows, before it uses the first.  U = 2 where tokens
+// alone fill the GPU: the table entries, slot and position are then read once
+// per token; U = 1 with a warp per four rows for few tokens, where latency is
+// all.  Bound by HBM: 57,304 tokens of 32 + 16 FP16 rows (1.277 GB) take
+// 206 us, 6.2 TB/s; with 16 lanes of one chunk per row, partners by shuffles,
+// 241 us; with a clamp, a conversion and a shift per code, 321 us.
+template <typename T, int TURN, int U>
+__global__ void __launch_bounds__(256, TURN == kTurnAny ? 2 : 4)
     pg_rope_append_int4_kernel(const __grid_constant__ Int4AppendParams p) {
+  constexpr bool FAST = TURN != kTurnAny;
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31, half = lane >> 4, m = lane & 15;
+  const int lane = threadIdx.x & 31, sub = lane >> 3, l = lane & 7;
   const int64_t w = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
   Int4Token k;
   k.token = p.split == 1 ? w : static_cast<uint32_t>(w) / p.split;  // w is small if split
@@ -363,15 +451,18 @@ __global__ void __launch_bounds__(256, 4)
   const int pos = p.positions[k.token];
   k.center = p.center_rows != nullptr ? p.center_rows[k.token] : 0;
   // The first query rows are asked for along with the token's indices.
-  const T* q = static_cast<const T*>(p.q) + k.token * p.q_stride_t + 8 * m;
-  const int nq = (p.hq + 2 * U - 1) / (2 * U), nk = (p.hkv + 1) >> 1;
-  uint4 raw[U];
+  const T* q = static_cast<const T*>(p.q) + k.token * p.q_stride_t;
+  const int nq = (p.hq + 4 * U - 1) / (4 * U), nk = (p.hkv + 3) >> 2;
+  uint4 ra[U], rb[U];
+  auto load_rows = [&](const T* base, int stride, int heads, int unit, uint4& x, uint4& y) {
+    const int h = 4 * unit + sub;
+    const T* row = base + (h < heads ? h : heads - 1) * stride + 8 * l;
+    x = load8<T, FAST>(row);
+    y = load8<T, FAST>(row + 64);
+  };
   auto load_queries = [&](int u) {
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int h = 2 * (u * U + i) + half;
-      raw[i] = load8<T, FAST>(q + (h < p.hq ? h : p.hq - 1) * p.q_stride_h);
-    }
+    for (int i = 0; i < U; ++i) load_rows(q, p.q_stride_h, p.hq, u * U + i, ra[i], rb[i]);
   };
   if (part < nq) load_queries(part);
   if (slot < 0) return;
@@ -386,75 +477,79 @@ __global__ void __launch_bounds__(256, 4)
     record_error(p.error_flag, kDevBadPosition);
     return;
   }
-  k.cos_row = p.cos + pos * p.table_stride;
-  k.sin_row = p.sin + pos * p.table_stride;
-  float c[8], s[8];
-  if constexpr (FAST) {
-    // The lane's entries: half layout 8 of them, interleaved 4.
-    const int step = p.pairs >> 3;
-    const int j = p.interleaved ? 4 * m : 8 * (m < step ? m : m - step);
+  Int4Turn t;
+  t.cos_row = p.cos + pos * p.table_stride;
+  t.sin_row = p.sin + pos * p.table_stride;
+  t.pairs = p.pairs;
+  t.l = l;
+  t.interleaved = p.interleaved != 0;
+  if constexpr (TURN == kTurnHalf || TURN == kTurnInterleaved) {
 #pragma unroll
     for (int i = 0; i < 8; i += 4) {
-      const bool in = (p.interleaved ? i == 0 : m < 2 * step) && j + i < p.pairs;
+      const int j = TURN == kTurnHalf ? 8 * l + i : 4 * l + 8 * i;
       const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-      const float4 a = in ? __ldg(reinterpret_cast<const float4*>(k.cos_row + j + i)) : z;
-      const float4 b = in ? __ldg(reinterpret_cast<const float4*>(k.sin_row + j + i)) : z;
-      c[i] = a.x; c[i + 1] = a.y; c[i + 2] = a.z; c[i + 3] = a.w;
-      const float sign = !p.interleaved && m < step ? -1.f : 1.f;
-      s[i] = sign * b.x; s[i + 1] = sign * b.y; s[i + 2] = sign * b.z; s[i + 3] = sign * b.w;
+      const float4 c = j < p.pairs ? __ldg(reinterpret_cast<const float4*>(t.cos_row + j)) : z;
+      const float4 s = j < p.pairs ? __ldg(reinterpret_cast<const float4*>(t.sin_row + j)) : z;
+      t.c[i] = c.x; t.c[i + 1] = c.y; t.c[i + 2] = c.z; t.c[i + 3] = c.w;
+      t.s[i] = s.x; t.s[i + 1] = s.y; t.s[i + 2] = s.z; t.s[i + 3] = s.w;
     }
   }
   const T* kr = static_cast<const T*>(p.k) + k.token * p.k_stride_t;
   const T* vr = static_cast<const T*>(p.v) + k.token * p.v_stride_t;
-  T* rq = static_cast<T*>(p.rotated_q) + k.token * p.rq_stride_t;
-  // Row h of two halves; an odd last row is loaded by both, stored by one.
-  auto turn_and_store = [&](float* x, const uint4& raw, const T* row, T* out, bool store) {
-    rotate8<T, FAST>(x, raw, row, m, p.pairs, p.interleaved, c, s, k.cos_row, k.sin_row);
+  // A last unit's missing rows repeat the last row and store nothing.
+  auto turn_and_store = [&](float* a, float* b, const uint4& x, const uint4& y, const T* row,
+                            T* out, bool store) {
+    rotate16<T, TURN>(a, b, x, y, row, t);
     // In place, other lanes' partner dims are this lane's.
     if constexpr (!FAST) __syncwarp();
-    if (store) store8<T, FAST>(out + 8 * m, x);
+    if (store) {
+      store8<T, FAST>(out + 8 * l, a);
+      store8<T, FAST>(out + 64 + 8 * l, b);
+    }
   };
-  auto append_row = [&](const uint4& raw, bool is_key, int h, const T* row) {
-    const int hc = h < p.hkv ? h : p.hkv - 1;
-    float x[8];
-    if (is_key)
-      turn_and_store(x, raw, row,
+  auto append_rows = [&](const uint4& x, const uint4& y, bool is_key, int unit) {
+    const int h = 4 * unit + sub, hc = h < p.hkv ? h : p.hkv - 1;
+    float a[8], b[8];
+    if (is_key) {
+      turn_and_store(a, b, x, y, kr + hc * p.k_stride_h,
                      static_cast<T*>(p.rotated_k) + k.token * p.rk_stride_t + hc * p.rk_stride_h,
                      p.rotated_k != nullptr && h < p.hkv);
-    else
-      unpack8<T>(raw, x);
-    subtract_center<T>(p, k, is_key ? p.key_center : p.value_center, hc, m, x);
-    store_int4_row(p, k, is_key, h, m, x);
+    } else {
+      unpack8<T>(x, a);
+      unpack8<T>(y, b);
+    }
+    subtract_center<T>(p, k, is_key ? p.key_center : p.value_center, hc, l, a, b);
+    store_int4_row(p, k, is_key, h, l, a, b);
   };
+  T* rq = static_cast<T*>(p.rotated_q) + k.token * p.rq_stride_t;
   for (int u = part; u < nq; u += p.split) {
     if (u != part) load_queries(u);
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int h = 2 * (u * U + i) + half;
-      if (2 * (u * U + i) >= p.hq) break;
+      const int h = 4 * (u * U + i) + sub;
+      if (4 * (u * U + i) >= p.hq) break;
       const int hc = h < p.hq ? h : p.hq - 1;
-      float x[8];
-      turn_and_store(x, raw[i], q - 8 * m + hc * p.q_stride_h, rq + hc * p.rq_stride_h, h < p.hq);
+      float a[8], b[8];
+      turn_and_store(a, b, ra[i], rb[i], q + hc * p.q_stride_h, rq + hc * p.rq_stride_h,
+                     h < p.hq);
     }
   }
   // This warp's first unit past the query rows.
   const int first = part >= nq ? part - nq : (p.split - (nq - part) % p.split) % p.split;
   if constexpr (U > 1) {
     for (int u = first; u < nk; u += p.split) {
-      const int h = 2 * u + half;
-      const int hc = h < p.hkv ? h : p.hkv - 1;
-      const uint4 x = load8<T, FAST>(kr + hc * p.k_stride_h + 8 * m);
-      const uint4 y = load8<T, FAST>(vr + hc * p.v_stride_h + 8 * m);
-      append_row(x, true, h, kr + hc * p.k_stride_h);
-      append_row(y, false, h, nullptr);
+      load_rows(kr, p.k_stride_h, p.hkv, u, ra[0], rb[0]);
+      load_rows(vr, p.v_stride_h, p.hkv, u, ra[1], rb[1]);
+      append_rows(ra[0], rb[0], true, u);
+      append_rows(ra[1], rb[1], false, u);
     }
   } else {
     for (int u = first; u < 2 * nk; u += p.split) {
       const bool is_key = u < nk;
-      const int h = 2 * (u - (is_key ? 0 : nk)) + half;
-      const int hc = h < p.hkv ? h : p.hkv - 1;
-      const T* row = is_key ? kr + hc * p.k_stride_h : vr + hc * p.v_stride_h;
-      append_row(load8<T, FAST>(row + 8 * m), is_key, h, row);
+      const int unit = u - (is_key ? 0 : nk);
+      load_rows(is_key ? kr : vr, is_key ? p.k_stride_h : p.v_stride_h, p.hkv, unit, ra[0],
+                rb[0]);
+      append_rows(ra[0], rb[0], is_key, unit);
     }
   }
 }
@@ -507,7 +602,7 @@ __global__ void __launch_bounds__(256)
       const __half* km = reinterpret_cast<const __half*>(rec + kInt4KeyMeta + tok * 16) + grp;
       const __half* vm = reinterpret_cast<const __half*>(rec + kInt4ValueMeta + tok * 16) + grp;
       codes[i][0] = *reinterpret_cast<const uint32_t*>(rec + tok * 64 + (m & 3) * 16 + grp * 4);
-      // The word of store_int4_row; its other lane's makes the two halves.
+      // One word of two groups' four dims; another lane's makes both halves.
       codes[i][1] = *reinterpret_cast<const uint32_t*>(
           rec + kInt4Value + value_code_row(tok) * 64 + (m & 3) * 16 + (grp & 1) * 8 +
           (grp >> 1) * 4);

@@ -98,7 +98,7 @@ def same_rounded(got, exp):
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("pairs,offset", [(64, 0), (32, 0), (8, 8), (29, 0), (64, 3), (1, 0),
-                                          (63, 8)])
+                                          (63, 8), (40, 0), (56, 0), (48, 8), (36, 0), (4, 0)])
 def test_append_is_bit_exact(cuda_lib, dtype, interleaved, pairs, offset):
     a = Append(77, hq=5, hkv=3, dtype=dtype, pairs=pairs, pad=5, offset=offset)
     q, k, records = a.expected(interleaved)
