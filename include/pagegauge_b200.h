@@ -483,8 +483,8 @@ int32_t pg_int4_read(const void* records, int64_t num_pages, int32_t kv_heads,
  *   out = softmax(sm_scale q K^T) V (+ value_center), lse_out = base-2
  * log-sum-exp of the scores.  The page table and its plan are those of
  * pg_decode_plan with one segment (indptr0); last_page_len counts the valid
- * tokens of a request's last page.  Requests without pages give zeros (no
- * centre) and -inf.  Pages may have been written by the kernel just before
+ * tokens of a request's last page (0..16; values outside are clamped).
+ * Requests without tokens give zeros (no centre) and -inf.  Pages may have been written by the kernel just before
  * in the stream: they are read after it completes.  A page id outside the
  * pool is left out and reported (PG_DEV_BAD_PAGE_ID).                      */
 typedef struct pg_int4_decode_args {

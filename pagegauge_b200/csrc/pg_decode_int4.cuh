@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
     int tail = kPage;
     if (item.count < 0 && n_w > 0 && warp + kInt4Warps * (n_w - 1) == n_pages - 1) {
       const int lv = __ldg(p.last_len + r);
-      tail = lv < 1 ? 1 : (lv > kPage ? kPage : lv);
+      tail = lv < 0 ? 0 : (lv > kPage ? kPage : lv);
     }
     Int4Query iq;
     load_query_int4<T, NARROW>(p, r, h, g, t, iq);

@@ -388,8 +388,9 @@ class Int4DecodeWrapper(BatchDecodeWithPagedKVCacheWrapper):
     """Decode over a 4-bit pool (``int4.Int4PagePool``): ``plan`` as the other
     wrappers' (``kv_data_type`` torch.uint8), ``run(q, records, sm_scale,
     value_center=, out=, lse=, return_lse=)`` with ``q`` and ``out`` float16
-    or bfloat16 [B,Hq,128].  Requests without pages give zeros and -inf.  One
-    wrapper's workspace serves one run at a time: concurrent streams (or
+    or bfloat16 [B,Hq,128]; ``q`` is 4-byte aligned with even strides.  Of a
+    request's last page ``last_page_len`` (0..16) tokens count; requests
+    without tokens give zeros and -inf.  One wrapper's workspace serves one run at a time: concurrent streams (or
     graphs replayed concurrently) need a wrapper each."""
 
     # The kernel's four warps take pages in pairs: an automatic split is

@@ -375,6 +375,51 @@ def test_attention_long_context(cuda_lib):
     a.check(*a.run(sm_scale=0.02), scale=float(np.float32(0.02)))
 
 
+@pytest.mark.parametrize("split,group", [(1, 4), (1, 8), (128, 4)])
+def test_attention_more_items_than_blocks(cuda_lib, split, group):
+    """More work items than resident blocks: items are handed out by a counter
+    that every run leaves at zero (run again, and replayed in a graph)."""
+    rng = np.random.default_rng(14)
+    lengths = [int(n) for n in rng.integers(1, 129, 70)]
+    a = Attend(lengths, hkv=8, group=group, split=split, seed=15)
+    assert a.wrapper._plan.num_items > 3 * 148
+    assert a.wrapper._plan.single == (split == 128)
+    out, lse = a.run()
+    a.check(out, lse)
+    graph = torch.cuda.CUDAGraph()
+    again, lse2 = torch.empty_like(out), torch.empty_like(lse)
+    with torch.cuda.graph(graph):
+        for _ in range(3):
+            a.run(out=again, lse=lse2)
+    for _ in range(2):
+        again.zero_()
+        graph.replay()
+        assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+def test_attention_last_page_without_tokens(cuda_lib):
+    a = Attend([33, 16], seed=16)
+    a.last[:] = 0  # 32 tokens, and none
+    a.lengths = [32, 0]
+    a.check(*a.run())
+
+
+def test_two_wrappers_on_two_streams(cuda_lib):
+    both = [Attend([3000, 100], hkv=4, seed=17), Attend([700, 2500], hkv=4, seed=18)]
+    exp = [tuple(t.clone() for t in a.run()) for a in both]
+    streams = [torch.cuda.Stream() for _ in both]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, (a, s) in enumerate(zip(both, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(a.run())
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out, lse in got[i]:
+            assert torch.equal(out, exp[i][0]) and torch.equal(lse, exp[i][1])
+
+
 def test_attention_strides_and_outputs(cuda_lib):
     a = Attend([100, 37, 250], seed=6)
     exp, exp_lse = (t.clone() for t in a.run())
