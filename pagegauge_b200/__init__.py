@@ -13,6 +13,10 @@ Public surface (mirrors the reference's operator surface):
   heterogeneous.run_decode()          the single-page-table ABI
   quantize.quantize_page_gauge() / quantize_completed_kv_pages()
   quantize.quantize_pages()           the affine_group16 representation
+  int4.Int4PagePool                   a paged cache in 4 bits, and its read-back
+  runtime ... .rope_append_int4()     rotation + append of any number of tokens to it
+  wrapper.make_int4_wrapper()         decode attention over it, plan/run
+  rotary.apply_rotary()               rotary positions; rotary_tables() scaled tables
   page_table.*                        request-major page-table helpers
   serving.*                           paged serving pool (vLLM-side layout)
   decoder.PageGaugeDecoder            Mistral-shaped decoder on these kernels

@@ -1114,7 +1114,7 @@ int32_t pg_rotary(const pg_rotary_args* a, void* stream) {
   p.positions = a->positions;
   p.error_flag = device_error_ptr();
   // Whole 16-byte chunks: the vector kernel.  (49,152 tokens of 40 FP16 rows:
-  // 168 us against 734 us one pair per thread.)
+  // 174 us against 734 us one pair per thread.)
   const int size = a->dtype == PG_DTYPE_F32 ? 4 : 2, v = 16 / size;
   const int table_floats = p.interleaved && v == 4 ? 2 : 4;
   bool fast = (p.interleaved ? 2 * a->pairs : a->pairs) % v == 0 &&
