@@ -11,8 +11,6 @@ import os
 import struct
 from pathlib import Path
 
-import torch
-
 LIB_NAME = "libpagegauge_b200.so"
 LIB_PATH = Path(__file__).resolve().parent / LIB_NAME
 
@@ -238,18 +236,27 @@ def packer(structure) -> struct.Struct:
     return struct.Struct("=" + out + "x" * (ctypes.sizeof(structure) - at))
 
 
-def launch(name: str, device, *args) -> None:
-    """Call entry ``name`` with ``args`` and the current stream of ``device``,
-    which is made the current device for the call."""
-    index = device.index
-    fn = getattr(_lib or load(), name)
-    if torch._C._cuda_getDevice() == index:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    if rc != 0:
-        check(rc)
+_ops = None
+
+
+def torch_ops():
+    """The torch binding of the rotary and 4-bit operators (csrc/pg_torch.cpp),
+    bound to the loaded library's entry points."""
+    global _ops
+    if _ops is None:
+        lib = load()
+        import torch  # noqa: F401  (the binding links against its libraries)
+        try:
+            from . import _torch_ops as ops
+        except ImportError as e:
+            raise RuntimeError(
+                "the torch binding could not be loaded; build it with "
+                "`python -m pagegauge_b200.build` (no fallback exists)") from e
+        ops.bind(*(ctypes.cast(getattr(lib, name), c_vp).value for name in (
+            "pg_last_error", "pg_rotary", "pg_rope_append_int4", "pg_int4_read",
+            "pg_decode_int4_run")))
+        _ops = ops
+    return _ops
 
 
 def kernel_pointer(t, name: str) -> int:

@@ -15,7 +15,6 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .rotary import DTYPES, check_token_index
 
 PAGE = 16
 HEAD_DIM = 128
@@ -23,18 +22,14 @@ GROUP = 32
 RECORD_BYTES = 2560
 
 
-def check_records(records: torch.Tensor) -> tuple[int, int, int]:
-    """(address, pages, KV heads) of a pool's records."""
-    shape = records.shape
-    address = records.data_ptr()
-    if (not records.is_cuda or records.dtype is not torch.uint8 or len(shape) != 3
-            or shape[0] == 0 or shape[1] == 0 or shape[2] != RECORD_BYTES
-            or not records.is_contiguous() or address % 16):
+def check_records(records: torch.Tensor) -> None:
+    if (not records.is_cuda or records.dtype != torch.uint8 or records.dim() != 3
+            or records.size(0) == 0 or records.size(1) == 0 or records.size(2) != RECORD_BYTES
+            or not records.is_contiguous() or records.data_ptr() % 16):
         raise ValueError(f"records must be contiguous 16-byte aligned CUDA uint8 "
                          f"[pages,Hkv,{RECORD_BYTES}]")
-    if shape[0] >= 1 << 27:
+    if records.size(0) >= 1 << 27:
         raise ValueError("a pool holds fewer than 2^27 pages")
-    return address, shape[0], shape[1]
 
 
 class Int4PagePool:
@@ -64,22 +59,5 @@ class Int4PagePool:
         16 + token), [T, Hkv, 128] each, without the centres that an append
         subtracted.  Negative slots give zeros; slots outside the pool give
         zeros and set the device guard word."""
-        if dtype not in DTYPES:
-            raise ValueError("values are read as float16, bfloat16 or float32")
-        records = self.records
-        device, tokens, kv_heads = records.device, slots.numel(), self.kv_heads
-        slot_ptr = check_token_index(slots, "slots", tokens, device)
-        if key_out is None and value_out is None:
-            shape, strides = (tokens, kv_heads, HEAD_DIM), (kv_heads * HEAD_DIM, HEAD_DIM, 1)
-            key_out = torch.empty_strided(shape, strides, dtype=dtype, device=device)
-            value_out = torch.empty_strided(shape, strides, dtype=dtype, device=device)
-        else:
-            shape = (tokens, kv_heads, HEAD_DIM)
-            for name, t in (("key_out", key_out), ("value_out", value_out)):
-                if (t is None or t.shape != shape or t.dtype is not dtype or t.device != device
-                        or not t.is_contiguous() or t.data_ptr() % 16):
-                    raise ValueError(f"{name} must be contiguous 16-byte aligned "
-                                     f"[T,{kv_heads},{HEAD_DIM}] {dtype} (both outputs or none)")
-        _lib.launch("pg_int4_read", device, records.data_ptr(), self.num_pages, kv_heads,
-                    slot_ptr, tokens, key_out.data_ptr(), value_out.data_ptr(), DTYPES[dtype])
-        return key_out, value_out
+        return (_lib._ops or _lib.torch_ops()).int4_read(self.records, slots, dtype, key_out,
+                                                         value_out)

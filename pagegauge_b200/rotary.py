@@ -16,9 +16,6 @@ import torch
 
 from . import _lib
 
-DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
-
-
 @dataclass(frozen=True)
 class RotaryScaling:
     """How the frequencies of a model trained on ``trained_positions`` are
@@ -93,62 +90,6 @@ def rotary_tables(positions: int, rotary_dim: int = 128, theta: float = 1.0e6,
     return (angle.cos() * scale).float(), (angle.sin() * scale).float()
 
 
-_PACK_ROTARY = _lib.packer(_lib.PgRotaryArgs).pack
-
-
-def check_tables(cosine: torch.Tensor, sine: torch.Tensor, device: torch.device,
-                 head_dim: int) -> tuple[int, int, int]:
-    """(rows, row stride, pairs) of a table pair [positions, pairs]."""
-    shape = cosine.shape
-    if (cosine.dtype is not torch.float32 or sine.dtype is not torch.float32
-            or len(shape) != 2 or shape != sine.shape):
-        raise ValueError("cosine and sine must be matching float32 [positions, pairs] tables")
-    if cosine.device != device or sine.device != device:
-        raise ValueError("rotary tables must be on the rows' device")
-    rows, pairs = shape
-    strides = cosine.stride()
-    if strides != sine.stride() or strides[1] != 1 or strides[0] < pairs:
-        raise ValueError("rotary tables must have equal strides and contiguous rows")
-    if rows == 0 or not 1 <= pairs <= head_dim // 2:
-        raise ValueError("the tables must have rows and rotate no more dims than a head has")
-    return rows, strides[0], pairs
-
-
-def check_token_index(t: torch.Tensor, name: str, tokens: int, device: torch.device) -> int:
-    """The address of an int32 index per token."""
-    if (t.dtype is not torch.int32 or t.shape != (tokens,) or t.device != device
-            or not t.is_contiguous()):
-        raise ValueError(f"{name} must be contiguous int32 [{tokens}] on the rows' device")
-    return t.data_ptr()
-
-
-def check_output(out: torch.Tensor, like: torch.Tensor, name: str) -> tuple[int, ...]:
-    """The strides of an output that takes ``like``'s rows."""
-    shape = out.shape
-    if shape != like.shape or out.dtype is not like.dtype or out.device != like.device:
-        raise ValueError(f"{name} must have its input's shape, dtype and device")
-    strides = out.stride()
-    if strides[2] != 1:
-        raise ValueError(f"{name} must have a contiguous last dimension")
-    if (strides[0] <= 0 and shape[0] > 1) or (strides[1] <= 0 and shape[1] > 1):
-        raise ValueError(f"{name} must not be expanded")
-    return strides
-
-
-def check_rows(x: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device,
-               tokens: int, head_dim: int) -> tuple[int, tuple[int, ...]]:
-    """(heads, strides) of rows [tokens, heads, head_dim]."""
-    shape = x.shape
-    if x.dtype is not dtype or x.device != device:
-        raise ValueError(f"{name} must have the query's device and dtype")
-    if len(shape) != 3 or shape[0] != tokens or shape[2] != head_dim:
-        raise ValueError(f"{name} must be [{tokens}, heads, {head_dim}]")
-    strides = x.stride()
-    if strides[2] != 1 and tokens:
-        raise ValueError(f"{name} must have a contiguous last dimension")
-    return shape[1], strides
-
-
 def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, cosine: torch.Tensor,
                  sine: torch.Tensor, positions: torch.Tensor, *, interleaved: bool = False,
                  adjoint: bool = False, query_out: torch.Tensor | None = None,
@@ -164,34 +105,5 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, cosine: torch.Te
     other strides.  The outputs may be the inputs (in place); they must not
     overlap them in any other way.  Rows of a token whose position is outside
     the tables are not written (``runtime.read_device_error`` reports it)."""
-    dtype, device = query.dtype, query.device
-    if dtype not in DTYPES:
-        raise ValueError("rows must be float16, bfloat16 or float32")
-    if not query.is_cuda or query.dim() != 3:
-        raise ValueError("query must be a CUDA tensor [tokens, heads, head_dim]")
-    tokens, _, head_dim = query.shape
-    hq, qs = check_rows(query, "query", dtype, device, tokens, head_dim)
-    if query_out is None:
-        query_out = torch.empty(query.shape, dtype=dtype, device=device)
-        qos = (hq * head_dim, head_dim)
-    else:
-        qos = check_output(query_out, query, "query_out")
-    hkv, ks, kos, k_ptr, ko_ptr = 0, (0, 0), (0, 0), 0, 0
-    if key is not None:
-        hkv, ks = check_rows(key, "key", dtype, device, tokens, head_dim)
-        if key_out is None:
-            key_out = torch.empty(key.shape, dtype=dtype, device=device)
-            kos = (hkv * head_dim, head_dim)
-        else:
-            kos = check_output(key_out, key, "key_out")
-        k_ptr, ko_ptr = key.data_ptr(), key_out.data_ptr()
-    elif key_out is not None:
-        raise ValueError("key_out without key")
-    rows, row_stride, pairs = check_tables(cosine, sine, device, head_dim)
-    pos_ptr = check_token_index(positions, "positions", tokens, device)
-    _lib.launch("pg_rotary", device, _PACK_ROTARY(
-        query.data_ptr(), k_ptr, query_out.data_ptr(), ko_ptr, qs[0], ks[0], qs[1], ks[1],
-        qos[0], kos[0], qos[1], kos[1], tokens, row_stride, rows, cosine.data_ptr(),
-        sine.data_ptr(), pos_ptr, hq, hkv, head_dim, pairs, bool(interleaved), bool(adjoint),
-        DTYPES[dtype]))
-    return query_out, key_out
+    return (_lib._ops or _lib.torch_ops()).rotary(
+        query, key, cosine, sine, positions, interleaved, adjoint, query_out, key_out)

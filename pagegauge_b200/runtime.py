@@ -14,12 +14,9 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .int4 import check_records
-from .rotary import DTYPES, check_output, check_rows, check_tables, check_token_index
 
 HEAD_DIM = 128
 PAGE = 16
-_PACK_INT4_APPEND = _lib.packer(_lib.PgInt4AppendArgs).pack
 
 
 def _stream(tensor: torch.Tensor) -> int:
@@ -312,51 +309,9 @@ class AppendExtension:
         ``center_rows[t]``, or row 0) are subtracted before quantising; the
         decode adds the value centre back.  ``rotated_query`` and the optional
         ``rotated_key`` take the rotated rows and may be the inputs."""
-        dtype, device = query.dtype, query.device
-        _require(dtype is torch.float16 or dtype is torch.bfloat16,
-                 "query must be float16 or bfloat16")
-        _require(query.is_cuda and query.dim() == 3, "query must be CUDA of rank three")
-        tokens = query.shape[0]
-        hq, qs = check_rows(query, "query", dtype, device, tokens, HEAD_DIM)
-        kv_heads, ks = check_rows(key, "key", dtype, device, tokens, HEAD_DIM)
-        v_heads, vs = check_rows(value, "value", dtype, device, tokens, HEAD_DIM)
-        _require(kv_heads == v_heads, "K/V input shapes must match")
-        _require(hq > 0 and kv_heads > 0, "head counts must be positive")
-        rqs = check_output(rotated_query, query, "rotated_query")
-        rows, row_stride, pairs = check_tables(cosine, sine, device, HEAD_DIM)
-        pos_ptr = check_token_index(positions, "positions", tokens, device)
-        slot_ptr = check_token_index(token_slots, "token_slots", tokens, device)
-        records_ptr, pages, heads = check_records(records)
-        _require(records.device == device and heads == kv_heads,
-                 "records must be [pages,Hkv,2560] on the rows' device")
-        rk_ptr, rks = 0, (0, 0)
-        if rotated_key is not None:
-            rks = check_output(rotated_key, key, "rotated_key")
-            rk_ptr = rotated_key.data_ptr()
-        kc_ptr = vc_ptr = row_ptr = centers = 0
-        if key_center is not None and value_center is not None:
-            shape = key_center.shape
-            if (len(shape) != 3 or shape[0] == 0 or shape[1] != kv_heads or shape[2] != HEAD_DIM
-                    or value_center.shape != shape):
-                raise RuntimeError(f"centers must both be [rows,{kv_heads},{HEAD_DIM}]")
-            for t in (key_center, value_center):
-                if t.dtype is not dtype or t.device != device or not t.is_contiguous():
-                    raise RuntimeError("centers must be contiguous, of the query's dtype and "
-                                       "device")
-            centers = shape[0]
-            kc_ptr, vc_ptr = key_center.data_ptr(), value_center.data_ptr()
-            if center_rows is not None:
-                row_ptr = check_token_index(center_rows, "center_rows", tokens, device)
-        else:
-            _require(key_center is None and value_center is None,
-                     "key and value centers are both given or both None")
-            _require(center_rows is None, "center_rows without centers")
-        _lib.launch("pg_rope_append_int4", device, _PACK_INT4_APPEND(
-            query.data_ptr(), key.data_ptr(), value.data_ptr(), rotated_query.data_ptr(), rk_ptr,
-            qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], rqs[0], rqs[1], rks[0], rks[1],
-            cosine.data_ptr(), sine.data_ptr(), row_stride, rows, pos_ptr, slot_ptr, records_ptr,
-            pages, kc_ptr, vc_ptr, row_ptr, centers, tokens, hq, kv_heads, pairs,
-            bool(interleaved), DTYPES[dtype], 0))
+        (_lib._ops or _lib.torch_ops()).rope_append_int4(
+            query, key, value, cosine, sine, positions, token_slots, rotated_query, records,
+            key_center, value_center, center_rows, rotated_key, interleaved)
 
     def exact_tail_merge_center(self, query, exact_key_pages, exact_value_pages,
                                 exact_page_indices, exact_last_page_len, old_output, old_lse,

@@ -33,8 +33,6 @@ import numpy as np
 import torch
 
 from . import _lib
-from .int4 import check_records
-from .rotary import DTYPES, check_output
 
 HEAD_DIM = 128
 PAGE = 16
@@ -416,57 +414,24 @@ class Int4DecodeWrapper(BatchDecodeWithPagedKVCacheWrapper):
             raise ValueError("indptr counts more pages than indices has")
         with torch.cuda.device(device):
             super().plan(indptr, indices, last_page_len, *args, **kwargs)
+        plan = self._plan
+        self._block = _PACK_INT4_DECODE(
+            0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, self._indices.data_ptr(), self._last_len.data_ptr(),
+            plan.items_ptr, plan.slots_ptr, plan.off_ptr, plan.o_ptr, plan.lse_ptr, plan.sem_ptr,
+            plan.num_items, plan.batch, plan.kv_heads, plan.group,
+            plan.single and plan.num_items > 0, 0, 0.0, 0)
+        self._device_index = device.index
 
     begin_forward = plan
 
     def run(self, q: torch.Tensor, records, sm_scale: float | None = None, *,
             value_center: torch.Tensor | None = None, out: torch.Tensor | None = None,
             lse: torch.Tensor | None = None, return_lse: bool = False):
-        plan = self._plan
-        if plan is None:
+        if self._plan is None:
             raise RuntimeError("plan() must be called before run()")
-        records = getattr(records, "records", records)
-        device = self._ws.buffer.device
-        kv_heads, hq = plan.kv_heads, self._num_qo_heads
-        records_ptr, pages, heads = check_records(records)
-        if records.device != device or heads != kv_heads:
-            raise ValueError(f"records must be [pages,{kv_heads},2560] on the workspace's device")
-        dtype = q.dtype
-        if ((dtype is not torch.float16 and dtype is not torch.bfloat16) or q.device != device
-                or q.shape != (plan.batch, hq, HEAD_DIM)):
-            raise ValueError(f"q must be float16 or bfloat16 [{plan.batch},{hq},{HEAD_DIM}] on "
-                             "the workspace's device")
-        qs = q.stride()
-        if qs[2] != 1:
-            raise ValueError("q must have a contiguous last dimension")
-        if out is None:
-            out = torch.empty(q.shape, dtype=dtype, device=device)
-        os = check_output(out, q, "out")
-        if lse is None and return_lse:
-            lse = torch.empty((plan.batch, hq), dtype=torch.float32, device=device)
-        lse_ptr = 0
-        if lse is not None:
-            if (lse.dtype is not torch.float32 or lse.shape != (plan.batch, hq)
-                    or lse.device != device or not lse.is_contiguous()):
-                raise ValueError(f"lse must be contiguous float32 [{plan.batch},{hq}] on the "
-                                 "workspace's device")
-            lse_ptr = lse.data_ptr()
-        vc_ptr = 0
-        if value_center is not None:
-            if (value_center.dtype is not dtype or value_center.device != device
-                    or not value_center.is_contiguous()
-                    or value_center.shape != (plan.batch, kv_heads, HEAD_DIM)):
-                raise ValueError(f"value_center must be contiguous [{plan.batch},{kv_heads},"
-                                 f"{HEAD_DIM}] of q's dtype")
-            vc_ptr = value_center.data_ptr()
-        _lib.launch("pg_decode_int4_run", device, _PACK_INT4_DECODE(
-            q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], lse_ptr, vc_ptr,
-            kv_heads * HEAD_DIM, records_ptr, pages, self._indices.data_ptr(),
-            self._last_len.data_ptr(), plan.items_ptr, plan.slots_ptr, plan.off_ptr, plan.o_ptr,
-            plan.lse_ptr, plan.sem_ptr, plan.num_items, plan.batch, kv_heads, plan.group,
-            plan.single and plan.num_items > 0, DTYPES[dtype],
-            self._sm_scale if sm_scale is None else sm_scale, 0))
-        return (out, lse) if return_lse else out
+        return (_lib._ops or _lib.torch_ops()).decode_int4(
+            self._block, self._device_index, q, getattr(records, "records", records),
+            self._sm_scale if sm_scale is None else sm_scale, value_center, out, lse, return_lse)
 
     forward = run
 

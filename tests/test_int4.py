@@ -149,3 +149,21 @@ def test_automatic_splits_are_whole_pairs_of_four_warps():
     split = -(-info.split_pages[0] // 8) * 8
     items, off, info = plan_items(1, 8, indptr, None, split, split, 148)
     assert info.split_pages[0] == split == 8 and off[-1] == 8 * 32
+
+
+def test_binding_refuses_what_is_not_a_cuda_tensor():
+    ops = _lib.torch_ops()
+    q = torch.zeros(2, 4, 128, dtype=torch.float16)
+    k = torch.zeros(2, 1, 128, dtype=torch.float16)
+    with pytest.raises(ValueError, match="query must be a tensor"):
+        ops.rope_append_int4(*([None] * 13), False)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.rope_append_int4(q, k, k, q, q, q, q, q, q, None, None, None, None, False)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.rotary(q, k, q, q, q, False, False, None, None)
+    with pytest.raises(ValueError, match="dtype"):
+        ops.int4_read(q, q, "half", None, None)
+    with pytest.raises(ValueError, match="argument block"):
+        ops.decode_int4(b"", 0, q, q, 1.0, None, None, None, False)
+    with pytest.raises(TypeError, match="arguments"):
+        ops.rotary(q)
