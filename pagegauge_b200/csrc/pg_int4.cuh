@@ -33,11 +33,6 @@ constexpr int kInt4KeyMeta = 2048;  // key scales and midpoints
 constexpr int kInt4ValueMeta = 2304;
 constexpr int kInt4Group = 32;  // dims that share a scale and a midpoint
 
-// Element types of q/k/v rows (the C ABI's PG_DTYPE_*).
-constexpr int kDtypeF16 = 0;
-constexpr int kDtypeBf16 = 1;
-constexpr int kDtypeF32 = 2;
-
 template <typename T>
 __device__ __forceinline__ float to_float(T x);
 template <>
