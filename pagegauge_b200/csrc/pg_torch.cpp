@@ -1,7 +1,7 @@
 // The torch side of the rotary and 4-bit cache operators: argument checks and
 // argument blocks in C++, so that a call costs little more than its launch
-// (from Python with ctypes the checks alone took 5-9 us: one decode token's
-// append 12.3 us, its read-back 9.3 us; here APPEND_US and READ_US).
+// (one decode token's append and read-back take 8.5 us; with the checks in
+// Python and ctypes 21.6 us, 5 to 9 us of it per call).
 //
 // The kernels are reached through the C ABI (include/pagegauge_b200.h), whose
 // entry points bind() takes from the loaded library.
@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -18,6 +19,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 
 #include "pagegauge_b200.h"
 
@@ -56,6 +58,20 @@ const Tensor* arg(PyObject* o, const char* name, bool optional = false) {
   if (optional && o == Py_None) return nullptr;
   if (!THPVariable_Check(o)) refuse("%s must be a tensor", name);
   return &THPVariable_Unpack(o);
+}
+
+// Rows and tables whose gradient a call would lose.
+void check_no_grad(std::initializer_list<const Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : tensors)
+    if (t != nullptr && t->requires_grad())
+      refuse("this operator has no gradient: detach its inputs or call it under no_grad");
+}
+
+// Written in place: a graph that saved the tensor for its backward must know.
+void wrote(std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    if (t != nullptr && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
 }
 
 bool flag(PyObject* o) {
@@ -164,7 +180,8 @@ PyObject* wrap_pair(const Tensor& a, const Tensor* b) {
 }
 
 // (query, key | None, cosine, sine, positions, interleaved, adjoint,
-//  query_out | None, key_out | None) -> (query_out, key_out | None)
+//  query_out | None, key_out | None) -> (query_out, key_out | None), or None,
+// with nothing done, for rows that require gradients
 PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!expect(n, 9)) return nullptr;
   return guarded([&]() -> PyObject* {
@@ -175,6 +192,10 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor& positions = *arg(a[4], "positions");
     const Tensor* query_out = arg(a[7], "query_out", true);
     const Tensor* key_out = arg(a[8], "key_out", true);
+    if (at::GradMode::is_enabled() &&
+        (query.requires_grad() || (key != nullptr && key->requires_grad())))
+      Py_RETURN_NONE;
+    check_no_grad({&cosine, &sine, query_out, key_out});
     const ScalarType dtype = query.scalar_type();
     if (dtype != at::kHalf && dtype != at::kBFloat16 && dtype != at::kFloat)
       refuse("rows must be float16, bfloat16 or float32");
@@ -223,6 +244,7 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.adjoint = flag(a[6]);
     p.dtype = dtype_code(dtype);
     launch(query.device(), [&](void* stream) { return entry.rotary(&p, stream); });
+    wrote({query_out, key_out});
     return wrap_pair(*outs[0], outs[1]);
   });
 }
@@ -246,6 +268,8 @@ PyObject* rope_append_int4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor* value_center = arg(a[10], "value_center", true);
     const Tensor* center_rows = arg(a[11], "center_rows", true);
     const Tensor* rotated_key = arg(a[12], "rotated_key", true);
+    check_no_grad({&query, &key, &value, &cosine, &sine, key_center, value_center, &rotated,
+                   rotated_key});
     const ScalarType dtype = query.scalar_type();
     if (dtype != at::kHalf && dtype != at::kBFloat16)
       refuse("query must be float16 or bfloat16");
@@ -315,6 +339,7 @@ PyObject* rope_append_int4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.interleaved = flag(a[13]);
     p.dtype = dtype_code(dtype);
     launch(query.device(), [&](void* stream) { return entry.append(&p, stream); });
+    wrote({&rotated, &records, rotated_key});
     Py_RETURN_NONE;
   });
 }
@@ -330,6 +355,7 @@ PyObject* int4_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (dtype != at::kHalf && dtype != at::kBFloat16 && dtype != at::kFloat)
       refuse("values are read as float16, bfloat16 or float32");
     const Tensor* outs[2] = {arg(a[3], "key_out", true), arg(a[4], "value_out", true)};
+    check_no_grad({outs[0], outs[1]});
     check_records(records);
     const int64_t tokens = slots.numel(), heads = records.size(1);
     const int32_t* at_slots = token_index(slots, "slots", tokens, records.device());
@@ -351,6 +377,7 @@ PyObject* int4_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
       return entry.read(pointer(records), records.size(0), static_cast<int32_t>(heads), at_slots,
                         tokens, pointer(*outs[0]), pointer(*outs[1]), dtype_code(dtype), stream);
     });
+    wrote({outs[0], outs[1]});
     return wrap_pair(*outs[0], outs[1]);
   });
 }
@@ -376,6 +403,7 @@ PyObject* decode_int4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor* out = arg(a[6], "out", true);
     const Tensor* lse = arg(a[7], "lse", true);
     const bool return_lse = flag(a[8]);
+    check_no_grad({&q, center, out, lse});
     const int64_t batch = p.batch, kv_heads = p.kv_heads, heads = kv_heads * p.group;
     check_records(records);
     if (records.device() != device || records.size(1) != kv_heads)
@@ -425,6 +453,7 @@ PyObject* decode_int4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.dtype = dtype_code(dtype);
     p.sm_scale = static_cast<float>(scale);
     launch(device, [&](void* stream) { return entry.decode(&p, stream); });
+    wrote({out, lse});
     return return_lse ? wrap_pair(*out, lse) : THPVariable_Wrap(*out);
   });
 }

@@ -16,6 +16,7 @@ import torch
 
 from . import _lib
 
+
 @dataclass(frozen=True)
 class RotaryScaling:
     """How the frequencies of a model trained on ``trained_positions`` are
@@ -90,6 +91,50 @@ def rotary_tables(positions: int, rotary_dim: int = 128, theta: float = 1.0e6,
     return (angle.cos() * scale).float(), (angle.sin() * scale).float()
 
 
+class _Rotate(torch.autograd.Function):
+    """The rotation, whose gradient is its transpose.  Rows that the kernel
+    leaves (a position outside the tables) are zero, and so are their
+    gradients."""
+
+    @staticmethod
+    def forward(ctx, query, key, cosine, sine, positions, interleaved, adjoint):
+        ctx.save_for_backward(cosine, sine, positions)
+        ctx.set_materialize_grads(False)
+        ctx.mode = (interleaved, not adjoint)
+        out = _lib.torch_ops().rotary(
+            query, key, cosine, sine, positions, interleaved, adjoint,
+            torch.zeros(query.shape, dtype=query.dtype, device=query.device),
+            None if key is None else torch.zeros(key.shape, dtype=key.dtype, device=key.device))
+        ctx.mark_non_differentiable(
+            *(y for y, need in zip(out, ctx.needs_input_grad) if y is not None and not need))
+        return out
+
+    @staticmethod
+    def backward(ctx, *grads):
+        needed = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[i]]
+        # A sum's gradient is one value expanded over the rows.
+        rows = [grads[i] if grads[i].stride(-1) == 1 else grads[i].contiguous() for i in needed]
+        result = [None] * 7
+        if rows:
+            turned = _Rotate.apply(rows[0], rows[1] if len(rows) == 2 else None,
+                                   *ctx.saved_tensors, *ctx.mode)
+            for i, y in zip(needed, turned):
+                result[i] = y
+        return tuple(result)
+
+
+def _rotate_with_gradient(query, key, cosine, sine, positions, interleaved, adjoint, query_out,
+                          key_out):
+    if query_out is not None or key_out is not None:
+        raise ValueError("rows that require gradients are rotated into new tensors")
+    if cosine.requires_grad or sine.requires_grad:
+        raise ValueError("the rotary tables have no gradient")
+    if torch.cuda.is_current_stream_capturing():
+        raise ValueError("a rotation with a gradient cannot be captured; capture the rotation "
+                         "and its adjoint under no_grad")
+    return _Rotate.apply(query, key, cosine, sine, positions, bool(interleaved), bool(adjoint))
+
+
 def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, cosine: torch.Tensor,
                  sine: torch.Tensor, positions: torch.Tensor, *, interleaved: bool = False,
                  adjoint: bool = False, query_out: torch.Tensor | None = None,
@@ -100,10 +145,16 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, cosine: torch.Te
     ``cosine``/``sine`` are FP32 [positions, pairs] (``rotary_tables``); the
     first ``2 * pairs`` dims turn, the others are copied.  Half layout pairs
     dim j with j + pairs, ``interleaved`` 2j with 2j + 1.  ``adjoint`` turns
-    back (the gradient of the rotation with respect to its rows).  Rows are
+    back (the gradient of the rotation with respect to its rows, which autograd
+    takes for rows that require one; the call then makes its outputs and is
+    not captured into a graph).  Rows are
     float16, bfloat16 or float32 with a contiguous last dimension and any
     other strides.  The outputs may be the inputs (in place); they must not
     overlap them in any other way.  Rows of a token whose position is outside
     the tables are not written (``runtime.read_device_error`` reports it)."""
-    return (_lib._ops or _lib.torch_ops()).rotary(
+    out = (_lib._ops or _lib.torch_ops()).rotary(
         query, key, cosine, sine, positions, interleaved, adjoint, query_out, key_out)
+    if out is None:  # rows that require gradients
+        out = _rotate_with_gradient(query, key, cosine, sine, positions, interleaved, adjoint,
+                                    query_out, key_out)
+    return out

@@ -458,6 +458,35 @@ def test_attention_reports_bad_pages(cuda_lib):
         a.check(out, lse, requests=[1])
 
 
+def test_attention_cuts_items_past_the_limit(cuda_lib):
+    """An item of more pages than the four warps hold (a plan for eight warps)
+    is cut at 128 pages and reported; the call ends and the others are whole."""
+    import ctypes
+
+    from pagegauge_b200 import _lib
+    from pagegauge_b200.wrapper import PagedDecodePlan, _Workspace, plan_items
+
+    a = Attend([16 * 200, 100], hkv=1, seed=19, center=False)
+    items, off, info = plan_items(2, 1, a.indptr.numpy(), None, 200, 0, 148, 8)
+    assert info.split_pages[0] == 200
+    p = PagedDecodePlan(_Workspace(torch.empty(8 << 20, dtype=torch.uint8, device="cuda")), items,
+                        off, info, 2, 1, 4)
+    out, lse = torch.empty_like(a.q), torch.empty(2, 4, device="cuda")
+    x = _lib.PgInt4DecodeArgs(
+        q=a.q.data_ptr(), q_stride_b=512, q_stride_h=128, out=out.data_ptr(), out_stride_b=512,
+        out_stride_h=128, lse_out=lse.data_ptr(), records=a.records.data_ptr(),
+        num_pages=a.records.size(0), indices=a.indices.data_ptr(),
+        last_page_len=a.last.data_ptr(), items=p.items_ptr, item_off=p.off_ptr, part_o=p.o_ptr,
+        part_lse=p.lse_ptr, work_counter=p.sem_ptr, num_items=p.num_items, batch=2, kv_heads=1,
+        group=4, final_mode=int(p.single), sm_scale=128 ** -0.5)
+    _lib.check(cuda_lib.pg_decode_int4_run(ctypes.byref(x),
+                                           torch.cuda.current_stream().cuda_stream))
+    assert read_device_error() == 3
+    a.check(out, lse, requests=[1])
+    a.lengths = [16 * 128, 100]
+    a.check(out, lse)
+
+
 def test_attention_merges_with_an_exact_tail(cuda_lib):
     """The (out, lse) state joins an FP16 segment's through
     merge_state_in_place, as the INT8 wrapper's does."""
@@ -540,6 +569,28 @@ def test_attention_refusals(cuda_lib):
 
 
 # ------------------------------------------------------------- as one path
+def test_inputs_that_require_gradients_are_refused(cuda_lib):
+    """And what a call writes carries a new version."""
+    a = Attend([33], hkv=2, seed=23)
+    w = a.wrapper
+    with pytest.raises(ValueError, match="no gradient"):
+        w.run(a.q.clone().requires_grad_(), a.records)
+    with torch.no_grad():
+        got = w.run(a.q.clone().requires_grad_(), a.records)
+    assert torch.equal(got, w.run(a.q, a.records)) and not got.requires_grad
+    out = torch.zeros_like(a.q)
+    version = out._version
+    w.run(a.q, a.records, out=out)
+    assert out._version > version
+    b = Append(3, 4, 2)
+    version = b.pool.records._version
+    b.run()
+    assert b.pool.records._version > version
+    b.k = b.k.clone().requires_grad_()
+    with pytest.raises(ValueError, match="no gradient"):
+        b.run()
+
+
 def test_prompt_then_decode_steps(cuda_lib):
     """A prompt appended in one call, then tokens one by one, attending after
     each: records equal the oracle's, outputs the attention over them."""

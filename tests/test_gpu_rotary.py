@@ -124,6 +124,98 @@ def test_adjoint_is_the_gradient(cuda_lib):
             assert abs((f(up) - f(down)) / 2 - float(grad[i])) < 256 * 2.0 ** -22 * 40
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_gradients(cuda_lib, dtype, interleaved):
+    """Autograd's gradients are the rotation's transpose applied to those of
+    the outputs (one rounding, as a rotation's), for strided rows, expanded
+    gradients, either input alone, and twice."""
+    flat = rows(9, 7, 64, dtype, 20).cuda().requires_grad_()
+    q, k = flat[:, :4], flat[:, 4:6]
+    cos, sin = rotary_tables(64, 48, scaling=RotaryScaling("parts", 4.0), device="cuda")
+    pos = torch.arange(5, 14, dtype=torch.int32, device="cuda")
+    at = pos.long()
+    qo, ko = apply_rotary(q, k, cos, sin, pos, interleaved=interleaved)
+    check(qo.detach(), q.detach(), cos[at], sin[at], interleaved)
+    check(ko.detach(), k.detach(), cos[at], sin[at], interleaved)
+    gq, gk = rows(9, 4, 64, dtype, 21).cuda(), rows(9, 2, 64, dtype, 22).cuda()
+    (grad,) = torch.autograd.grad((qo, ko), flat, (gq, gk), retain_graph=True)
+    check(grad[:, :4], gq, cos[at], sin[at], interleaved, adjoint=True)
+    check(grad[:, 4:6], gk, cos[at], sin[at], interleaved, adjoint=True)
+    assert (grad[:, 6] == 0).all()
+    # The sum's gradient is one expanded value; the key's output is unused.
+    (grad,) = torch.autograd.grad(qo.sum(), flat, retain_graph=True)
+    check(grad[:, :4], torch.ones_like(gq), cos[at], sin[at], interleaved, adjoint=True)
+    assert (grad[:, 4:] == 0).all()
+    (grad,) = torch.autograd.grad(ko, flat, gk)
+    check(grad[:, 4:6], gk, cos[at], sin[at], interleaved, adjoint=True)
+    # Only the key requires a gradient.
+    leaf = k.detach().clone().requires_grad_()
+    qo, ko = apply_rotary(q.detach(), leaf, cos, sin, pos, interleaved=interleaved)
+    assert not qo.requires_grad and ko.requires_grad
+    ko.backward(gk)
+    check(leaf.grad, gk, cos[at], sin[at], interleaved, adjoint=True)
+    # The gradient's gradient is the rotation again.
+    leaf = q.detach().clone().requires_grad_()
+    qo, none = apply_rotary(leaf, None, cos, sin, pos, interleaved=interleaved)
+    assert none is None
+    weight = gq.clone().requires_grad_()
+    (grad,) = torch.autograd.grad(qo, leaf, weight, create_graph=True)
+    (second,) = torch.autograd.grad(grad, weight, gq)
+    check(second, gq, cos[at], sin[at], interleaved)
+
+
+def test_gradients_of_rows_outside_the_tables_are_zero(cuda_lib):
+    x = rows(4, 2, 64, torch.float32, 23).cuda().requires_grad_()
+    cos, sin = rotary_tables(8, 64, device="cuda")
+    pos = torch.tensor([1, -1, 7, 8], dtype=torch.int32, device="cuda")
+    y, _ = apply_rotary(x, None, cos, sin, pos)
+    (grad,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    assert read_device_error() == 2
+    for t in (y, grad):
+        assert (t[[1, 3]] == 0).all() and (t[[0, 2]] != 0).any()
+
+
+def test_gradient_refusals_and_in_place_writes(cuda_lib):
+    q = rows(4, 2, 64, torch.float16, 24).cuda()
+    cos, sin = rotary_tables(8, 64, device="cuda")
+    pos = torch.zeros(4, dtype=torch.int32, device="cuda")
+    leaf = q.clone().requires_grad_()
+    for kw in (dict(query_out=torch.empty_like(q)), dict(query_out=leaf)):
+        with pytest.raises(ValueError, match="new tensors"):
+            apply_rotary(leaf, None, cos, sin, pos, **kw)
+    with pytest.raises(ValueError, match="no gradient"):
+        apply_rotary(leaf, None, cos.clone().requires_grad_(), sin, pos)
+    with pytest.raises(ValueError, match="no gradient"):
+        apply_rotary(q, None, cos.clone().requires_grad_(), sin, pos)
+    with pytest.raises(ValueError, match="no gradient"):
+        apply_rotary(q, None, cos, sin, pos, query_out=leaf)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pos.add_(1)
+        with pytest.raises(ValueError, match="captured"):
+            apply_rotary(leaf, None, cos, sin, pos)
+    with torch.no_grad():
+        out, _ = apply_rotary(leaf, None, cos, sin, pos)
+    assert not out.requires_grad
+    # What a graph saved and a rotation in place then changed is refused.
+    hidden = q.float().requires_grad_() * 2
+    loss = (hidden * hidden).sum()
+    with torch.no_grad():
+        apply_rotary(hidden, None, cos, sin, pos, query_out=hidden)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    # Tables and positions that changed between forward and backward, too.
+    y, _ = apply_rotary(leaf, None, cos, sin, pos)
+    pos.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.float().sum().backward()
+    with torch.inference_mode():
+        x = q.clone()
+        apply_rotary(x, None, cos, sin, pos, query_out=x)
+    assert torch.equal(x, apply_rotary(q, None, cos, sin, pos)[0])
+
+
 def test_capture_and_another_stream(cuda_lib):
     q, k = rows(33, 4, 128, torch.bfloat16, 10).cuda(), rows(33, 2, 128, torch.bfloat16,
                                                              11).cuda()
