@@ -1113,22 +1113,31 @@ int32_t pg_rotary(const pg_rotary_args* a, void* stream) {
   p.table_rows = a->table_rows;
   p.positions = a->positions;
   p.error_flag = device_error_ptr();
-  // Whole 16-byte chunks: the vector kernel.  (49,152 tokens of 40 FP16 rows:
-  // 174 us against 734 us one pair per thread.)
   const int size = a->dtype == PG_DTYPE_F32 ? 4 : 2, v = 16 / size;
+  bool rows16 = true;
+  for (int i = 0; i < 2; ++i) {
+    rows16 = rows16 &&
+             (p.heads[i] == 0 ||
+              (aligned(p.x[i], 16) && aligned(p.y[i], 16) &&
+               (p.x_stride_t[i] | p.x_stride_h[i] | p.y_stride_t[i] | p.y_stride_h[i]) % v == 0));
+    p.in_place[i] = p.x[i] == p.y[i] && p.x_stride_t[i] == p.y_stride_t[i] &&
+                    p.x_stride_h[i] == p.y_stride_h[i];
+  }
   const int table_floats = p.interleaved && v == 4 ? 2 : 4;
-  bool fast = (p.interleaved ? 2 * a->pairs : a->pairs) % v == 0 &&
-              (a->head_dim - 2 * a->pairs) % v == 0 && aligned(a->cosine, 4 * table_floats) &&
-              aligned(a->sine, 4 * table_floats) && a->table_stride % table_floats == 0;
-  for (int i = 0; i < 2 && fast; ++i)
-    fast = p.heads[i] == 0 ||
-           (aligned(p.x[i], 16) && aligned(p.y[i], 16) &&
-            (p.x_stride_t[i] | p.x_stride_h[i] | p.y_stride_t[i] | p.y_stride_h[i]) % v == 0);
+  const bool chunks16 = rows16 && (p.interleaved ? 2 * a->pairs : a->pairs) % v == 0 &&
+                        (a->head_dim - 2 * a->pairs) % v == 0 &&
+                        aligned(a->cosine, 4 * table_floats) &&
+                        aligned(a->sine, 4 * table_floats) && a->table_stride % table_floats == 0;
+  // Whole 16-byte chunks of turning dims need no shared memory, which is
+  // faster where the call stays in the L2 (1,000 tokens of 40 FP16 rows of 128
+  // dims: 5.7 against 6.8 us; interleaved 6.9 / 7.1) and for 16-bit heads that
+  // turn whole in half layout (16,000 tokens: 61.1 / 62.8 us; interleaved 66.8
+  // / 63.6, half of the head 66.0 / 54.1, FP32 108.9 / 104.7 us).
+  const bool large = a->tokens * rows * a->head_dim * size * 2 > int64_t(100) << 20;
+  const bool whole_head = size == 2 && !p.interleaved && 2 * a->pairs == a->head_dim;
+  using Kernel = void (*)(pg::RotaryParams);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (fast) {
-    for (int i = 0; i < 2; ++i)
-      p.in_place[i] = p.x[i] == p.y[i] && p.x_stride_t[i] == p.y_stride_t[i] &&
-                      p.x_stride_h[i] == p.y_stride_h[i];
+  if (chunks16 && (!large || whole_head)) {
     p.chunks = p.interleaved ? 2 * a->pairs / v : a->pairs / v;
     // Rows per thread once there are rows enough for every thread slot four
     // times over, else one: more rows per thread read fewer table entries.
@@ -1143,7 +1152,6 @@ int32_t pg_rotary(const pg_rotary_args* a, void* stream) {
     const int block = units > 148 * 256 ? 256 : 64;
     PG_REQUIRE((units + block - 1) / block < (int64_t(1) << 31), "too many rows or tokens");
     const dim3 grid(static_cast<unsigned>((units + block - 1) / block));
-    using Kernel = void (*)(pg::RotaryParams);
     const Kernel kernels[3][2] = {
         {pg::pg_rotary_kernel<__half, false>, pg::pg_rotary_kernel<__half, true>},
         {pg::pg_rotary_kernel<__nv_bfloat16, false>, pg::pg_rotary_kernel<__nv_bfloat16, true>},
@@ -1151,15 +1159,40 @@ int32_t pg_rotary(const pg_rotary_args* a, void* stream) {
     return launch_pdl(kernels[a->dtype][p.interleaved], grid, dim3(block), 0, st,
                       "rotary launch", p);
   }
-  const int64_t total = a->tokens * rows * (a->head_dim - a->pairs);
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>((total + 255) / 256, 148 * 64)));
-  if (a->dtype == PG_DTYPE_F16)
-    return launch_pdl(pg::pg_rotary_any_kernel<__half>, grid, dim3(256), 0, st, "rotary launch",
-                      p);
-  if (a->dtype == PG_DTYPE_BF16)
-    return launch_pdl(pg::pg_rotary_any_kernel<__nv_bfloat16>, grid, dim3(256), 0, st,
-                      "rotary launch", p);
-  return launch_pdl(pg::pg_rotary_any_kernel<float>, grid, dim3(256), 0, st, "rotary launch", p);
+  // Tiles of up to 26 KB (16,000 tokens of 10 KB: tiles of 10 KB 70.7, 20 KB
+  // 62.8, 40 KB 66.2 us), of few tokens no more rows than occupy the GPU.
+  const bool vec = rows16 && a->head_dim % v == 0;
+  p.pitch = vec ? a->head_dim : (a->head_dim + 1) & ~1;
+  const int64_t row_bytes = static_cast<int64_t>(p.pitch) * size, most = 26 << 10;
+  p.block_tokens = 1;
+  while (p.block_tokens < 8 && 2 * p.block_tokens * rows * row_bytes <= most &&
+         2 * p.block_tokens * 148 * 8 <= a->tokens)
+    p.block_tokens *= 2;
+  const int64_t spread = std::max<int64_t>(1, 148 * 8 / a->tokens);
+  const int64_t fit = std::max<int64_t>(1, std::min(most / row_bytes, (rows + spread - 1) / spread));
+  const int64_t tiles = p.block_tokens > 1 ? 1 : (rows + fit - 1) / fit;
+  PG_REQUIRE(tiles < 65536, "too many rows");
+  p.tile_rows = static_cast<int32_t>((rows + tiles - 1) / tiles);
+  // Two pairs per access for 16-bit rows (half layout 62.8 us; one 69.7, four
+  // 65.8 us; interleaved 59.5 / 62.7 / 68 us), one for FP32 (100 / 110 us).
+  const bool two = vec && size == 2 && a->pairs % 2 == 0;
+  const int threads = 256 / p.block_tokens;
+  p.over_cols = pg::over_n(std::min(vec ? a->head_dim / v : a->head_dim, threads));
+  p.over_pairs = pg::over_n(std::min(two ? a->pairs / 2 : a->pairs, threads));
+  const dim3 grid(
+      static_cast<unsigned>((a->tokens + p.block_tokens - 1) / p.block_tokens),
+      static_cast<unsigned>(tiles));
+  const size_t smem = static_cast<size_t>(p.block_tokens * p.tile_rows * row_bytes);
+#define PG_ROTARY_ROWS(T, TWO)                                                               \
+  {pg::pg_rotary_rows_kernel<T, false, false, 1>, pg::pg_rotary_rows_kernel<T, true, false, 1>, \
+   pg::pg_rotary_rows_kernel<T, false, true, 1>, pg::pg_rotary_rows_kernel<T, true, true, 1>,   \
+   pg::pg_rotary_rows_kernel<T, false, true, TWO>,                                            \
+   pg::pg_rotary_rows_kernel<T, true, true, TWO>}
+  const Kernel kernels[3][6] = {PG_ROTARY_ROWS(__half, 2), PG_ROTARY_ROWS(__nv_bfloat16, 2),
+                                PG_ROTARY_ROWS(float, 1)};
+#undef PG_ROTARY_ROWS
+  return launch_pdl(kernels[a->dtype][two ? 4 + p.interleaved : 2 * vec + p.interleaved], grid, dim3(256), smem,
+                    st, "rotary launch", p);
 }
 
 int32_t pg_rope_append_int4(const pg_int4_append_args* a, void* stream) {
@@ -1234,10 +1267,12 @@ int32_t pg_rope_append_int4(const pg_int4_append_args* a, void* stream) {
   const bool table16 = aligned(a->cosine, 16) && aligned(a->sine, 16) &&
                        a->table_stride % 4 == 0 && a->pairs % (p.interleaved ? 4 : 8) == 0;
   const bool fast = rows16 && table16;
-  const int turn = !fast           ? pg::kTurnAny
+  const int turn = !rows16         ? pg::kTurnAny
+                   : !fast         ? (p.interleaved ? pg::kTurnOddInterleaved : pg::kTurnOdd)
                    : p.interleaved ? pg::kTurnInterleaved
                    : p.pairs == 64 ? pg::kTurnHalf
-                                   : pg::kTurnPart;
+                   : p.pairs <= 32 ? pg::kTurnPart
+                                   : pg::kTurnOdd;
   // Few tokens: a warp per four rows.  Else eight query rows (or four key and
   // four value rows) at a time, a token's groups over as many warps as fill
   // the GPU.
@@ -1256,8 +1291,9 @@ int32_t pg_rope_append_int4(const pg_int4_append_args* a, void* stream) {
   {pg::pg_rope_append_int4_kernel<T, TURN, 1>, pg::pg_rope_append_int4_kernel<T, TURN, 2>}
 #define PG_APPEND_TURNS(T) \
   {PG_APPEND(T, pg::kTurnAny), PG_APPEND(T, pg::kTurnHalf), \
-   PG_APPEND(T, pg::kTurnInterleaved), PG_APPEND(T, pg::kTurnPart)}
-  const Kernel kernels[2][4][2] = {PG_APPEND_TURNS(__half), PG_APPEND_TURNS(__nv_bfloat16)};
+   PG_APPEND(T, pg::kTurnInterleaved), PG_APPEND(T, pg::kTurnPart), PG_APPEND(T, pg::kTurnOdd), \
+   PG_APPEND(T, pg::kTurnOddInterleaved)}
+  const Kernel kernels[2][6][2] = {PG_APPEND_TURNS(__half), PG_APPEND_TURNS(__nv_bfloat16)};
 #undef PG_APPEND_TURNS
 #undef PG_APPEND
   return launch_pdl(kernels[a->dtype == PG_DTYPE_BF16][turn][wide], grid, dim3(block * 32), 0,

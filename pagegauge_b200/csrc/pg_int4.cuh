@@ -249,20 +249,27 @@ struct Int4AppendParams {
   int* error_flag;
 };
 
-// How an append rotates: rows and tables that are not 16-byte aligned, or
-// parts that are not whole 16-byte chunks (kTurnAny); the whole head in half
-// layout, whose partner dims lie in one lane (kTurnHalf); neighbouring pairs
-// (kTurnInterleaved); part of the head in half layout (kTurnPart).
-constexpr int kTurnAny = 0, kTurnHalf = 1, kTurnInterleaved = 2, kTurnPart = 3;
+// How an append rotates: the whole head in half layout, whose partner dims lie
+// in one lane (kTurnHalf); up to half of the head in half layout (kTurnPart);
+// neighbouring pairs (kTurnInterleaved); parts that are not whole 16-byte
+// chunks, or tables that are not aligned, in half layout, through shared
+// memory (kTurnOdd), and interleaved (kTurnOddInterleaved); and rows that are
+// not 16-byte aligned (kTurnAny).  8,000 tokens of 32 + 16 FP16 rows with 58
+// turning dims, append and read: 56.4 us in half layout, 46.3 us
+// interleaved (128 dims: 45.2 / 46.2 us); with the partners read one by one
+// from the rows 138.8 / 118.7 us.
+constexpr int kTurnAny = 0, kTurnHalf = 1, kTurnInterleaved = 2, kTurnPart = 3, kTurnOdd = 4,
+              kTurnOddInterleaved = 5;
 
 // A token's table rows and lane l's entries of them: kTurnHalf 8l .. 8l+7,
-// kTurnInterleaved 4l .. 4l+3 and 32 + 4l ..
+// kTurnPart those of its first chunk, interleaved 4l .. 4l+3 and 32 + 4l ..,
+// others l, l + 8, ...
 struct Int4Turn {
   const float* cos_row;
   const float* sin_row;
   float c[8], s[8];
   int pairs, l;
-  bool interleaved;  // kTurnAny
+  bool interleaved;
 };
 
 // 8 dims d .. d + 7 (a chunk) of a row with partner dims o.
@@ -276,19 +283,26 @@ __device__ __forceinline__ void turn_half(float* x, const float* o, const float*
   }
 }
 
-__device__ __forceinline__ void turn_interleaved(float* x, const float* c, const float* s) {
+// The first n pairs.
+__device__ __forceinline__ void turn_interleaved(float* x, const float* c, const float* s,
+                                                 int n = 4) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
+    if (i >= n) break;
     const float a = x[2 * i], b = x[2 * i + 1];
     x[2 * i] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i]));
     x[2 * i + 1] = __fadd_rn(__fmul_rn(b, c[i]), __fmul_rn(a, s[i]));
   }
 }
 
+// A row in shared memory: rows of a warp start eight banks apart.
+constexpr int kTurnPitch = kHeadDim + 8;
+
 // Lane l's two chunks of a row (ra, rb as loaded), rotated into a and b.
+// tile: the row's floats in shared memory (kTurnOdd, kTurnAny).
 template <typename T, int TURN>
 __device__ __forceinline__ void rotate16(float* a, float* b, const uint4& ra, const uint4& rb,
-                                         const T* row, const Int4Turn& t) {
+                                         const Int4Turn& t, float* tile) {
   unpack8<T>(ra, a);
   unpack8<T>(rb, b);
   const int l = t.l, pairs = t.pairs;
@@ -302,61 +316,51 @@ __device__ __forceinline__ void rotate16(float* a, float* b, const uint4& ra, co
     if (4 * l < pairs) turn_interleaved(a, t.c, t.s);
     if (32 + 4 * l < pairs) turn_interleaved(b, t.c + 4, t.s + 4);
   } else if constexpr (TURN == kTurnPart) {
-    // Chunks c < n = pairs / 8 turn with c + n, n < 8: the partner of a first
-    // chunk (a) may be either one of another lane's, that of b is an a.
+    // Chunks c < n = pairs / 8 turn with c + n, n <= 4: all of them in a.
     const int n = pairs >> 3;
-    const bool turns_a = l < 2 * n, turns_b = 8 + l < 2 * n;
-    const int peer = !turns_a ? l : l < n ? l + n : l - n;
-    const int peer_b = turns_b ? 8 + l - n : l;
-    uint4 oa, ob;
+    const int peer = l < n ? l + n : l - n;
+    uint4 oa;
     const uint32_t* wa = reinterpret_cast<const uint32_t*>(&ra);
-    const uint32_t* wb = reinterpret_cast<const uint32_t*>(&rb);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t x = __shfl_sync(0xffffffffu, wa[i], peer & 7, 8);
-      const uint32_t y = __shfl_sync(0xffffffffu, wb[i], peer & 7, 8);
-      reinterpret_cast<uint32_t*>(&oa)[i] = peer >= 8 ? y : x;
-      reinterpret_cast<uint32_t*>(&ob)[i] = __shfl_sync(0xffffffffu, wa[i], peer_b, 8);
-    }
-    float o[8], c[8], s[8];
-    auto entries = [&](int j) {
-#pragma unroll
-      for (int i = 0; i < 8; i += 4) {
-        const float4 x = __ldg(reinterpret_cast<const float4*>(t.cos_row + j + i));
-        const float4 y = __ldg(reinterpret_cast<const float4*>(t.sin_row + j + i));
-        c[i] = x.x; c[i + 1] = x.y; c[i + 2] = x.z; c[i + 3] = x.w;
-        s[i] = y.x; s[i + 1] = y.y; s[i + 2] = y.z; s[i + 3] = y.w;
-      }
-    };
-    if (turns_a) {
-      entries(8 * (l < n ? l : l - n));
+    for (int i = 0; i < 4; ++i)
+      reinterpret_cast<uint32_t*>(&oa)[i] = __shfl_sync(0xffffffffu, wa[i], peer & 7, 8);
+    if (l < 2 * n) {
+      float o[8];
       unpack8<T>(oa, o);
       if (l < n)
-        turn_half<true>(a, o, c, s);
+        turn_half<true>(a, o, t.c, t.s);
       else
-        turn_half<false>(a, o, c, s);
+        turn_half<false>(a, o, t.c, t.s);
     }
-    if (turns_b) {
-      entries(8 * peer_b);
-      unpack8<T>(ob, o);
-      turn_half<false>(b, o, c, s);
-    }
+  } else if (TURN == kTurnOddInterleaved || (TURN == kTurnAny && t.interleaved)) {
+    turn_interleaved(a, t.c, t.s, pairs - 4 * l);
+    turn_interleaved(b, t.c + 4, t.s + 4, pairs - 32 - 4 * l);
   } else {
+    static_assert(TURN == kTurnAny || TURN == kTurnOdd || TURN == kTurnOddInterleaved,
+                  "the others have no tile");
+    // Lane l turns pairs l, l + 8, ... of its row.
+    float4* mine = reinterpret_cast<float4*>(tile + 8 * l);
+    mine[0] = make_float4(a[0], a[1], a[2], a[3]);
+    mine[1] = make_float4(a[4], a[5], a[6], a[7]);
+    mine[16] = make_float4(b[0], b[1], b[2], b[3]);
+    mine[17] = make_float4(b[4], b[5], b[6], b[7]);
+    __syncwarp();
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      float* x = k == 0 ? a : b;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int d = 64 * k + 8 * l + i;
-        if (d >= 2 * pairs) continue;
-        // The partner dim, read from the row (loaded whole before any store).
-        const bool first = t.interleaved ? (d & 1) == 0 : d < pairs;
-        const int j = t.interleaved ? d >> 1 : first ? d : d - pairs;
-        const int other = t.interleaved ? d ^ 1 : first ? d + pairs : j;
-        const float u = __fmul_rn(x[i], t.cos_row[j]);
-        const float w = __fmul_rn(to_float<T>(row[other]), t.sin_row[j]);
-        x[i] = first ? __fsub_rn(u, w) : __fadd_rn(u, w);
+    for (int i = 0; i < 8; ++i) {
+      const int j = l + 8 * i;
+      if (8 * i >= pairs) break;
+      if (j < pairs) {
+        const float x = tile[j], y = tile[j + pairs];
+        tile[j] = __fsub_rn(__fmul_rn(x, t.c[i]), __fmul_rn(y, t.s[i]));
+        tile[j + pairs] = __fadd_rn(__fmul_rn(y, t.c[i]), __fmul_rn(x, t.s[i]));
       }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float4 x = mine[i], y = mine[16 + i];
+      a[4 * i] = x.x; a[4 * i + 1] = x.y; a[4 * i + 2] = x.z; a[4 * i + 3] = x.w;
+      b[4 * i] = y.x; b[4 * i + 1] = y.y; b[4 * i + 2] = y.z; b[4 * i + 3] = y.w;
     }
   }
 }
@@ -431,7 +435,7 @@ __device__ __forceinline__ void subtract_center(const Int4AppendParams& p, const
 // 206 us, 6.2 TB/s; with 16 lanes of one chunk per row, partners by shuffles,
 // 241 us; with a clamp, a conversion and a shift per code, 321 us.
 template <typename T, int TURN, int U>
-__global__ void __launch_bounds__(256, TURN == kTurnAny ? 2 : 4)
+__global__ void __launch_bounds__(256, 4)
     pg_rope_append_int4_kernel(const __grid_constant__ Int4AppendParams p) {
   constexpr bool FAST = TURN != kTurnAny;
   pdl_launch_dependents();
@@ -478,10 +482,11 @@ __global__ void __launch_bounds__(256, TURN == kTurnAny ? 2 : 4)
   t.pairs = p.pairs;
   t.l = l;
   t.interleaved = p.interleaved != 0;
-  if constexpr (TURN == kTurnHalf || TURN == kTurnInterleaved) {
+  if constexpr (TURN == kTurnHalf || TURN == kTurnInterleaved || TURN == kTurnPart) {
+    const int first = TURN == kTurnPart && 8 * l >= p.pairs ? 8 * l - p.pairs : 8 * l;
 #pragma unroll
     for (int i = 0; i < 8; i += 4) {
-      const int j = TURN == kTurnHalf ? 8 * l + i : 4 * l + 8 * i;
+      const int j = TURN == kTurnInterleaved ? 4 * l + 8 * i : first + i;
       const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
       const float4 c = j < p.pairs ? __ldg(reinterpret_cast<const float4*>(t.cos_row + j)) : z;
       const float4 s = j < p.pairs ? __ldg(reinterpret_cast<const float4*>(t.sin_row + j)) : z;
@@ -489,14 +494,24 @@ __global__ void __launch_bounds__(256, TURN == kTurnAny ? 2 : 4)
       t.s[i] = s.x; t.s[i + 1] = s.y; t.s[i + 2] = s.z; t.s[i + 3] = s.w;
     }
   }
+  if constexpr (TURN == kTurnAny || TURN == kTurnOdd || TURN == kTurnOddInterleaved) {
+    const bool quads = TURN == kTurnOddInterleaved || (TURN == kTurnAny && t.interleaved);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int j = quads ? 4 * l + 8 * (i & 4) + (i & 3) : l + 8 * i;
+      t.c[i] = j < p.pairs ? __ldg(t.cos_row + j) : 0.f;
+      t.s[i] = j < p.pairs ? __ldg(t.sin_row + j) : 0.f;
+    }
+  }
+  constexpr bool kTile = TURN == kTurnAny || TURN == kTurnOdd;
+  __shared__ __align__(16) float s_rows[kTile ? 8 : 1][kTile ? 4 * kTurnPitch : 4];
+  float* tile = kTile ? &s_rows[threadIdx.x >> 5][sub * kTurnPitch] : nullptr;
   const T* kr = static_cast<const T*>(p.k) + k.token * p.k_stride_t;
   const T* vr = static_cast<const T*>(p.v) + k.token * p.v_stride_t;
   // A last unit's missing rows repeat the last row and store nothing.
-  auto turn_and_store = [&](float* a, float* b, const uint4& x, const uint4& y, const T* row,
-                            T* out, bool store) {
-    rotate16<T, TURN>(a, b, x, y, row, t);
-    // In place, other lanes' partner dims are this lane's.
-    if constexpr (!FAST) __syncwarp();
+  auto turn_and_store = [&](float* a, float* b, const uint4& x, const uint4& y, T* out,
+                            bool store) {
+    rotate16<T, TURN>(a, b, x, y, t, tile);
     if (store) {
       store8<T, FAST>(out + 8 * l, a);
       store8<T, FAST>(out + 64 + 8 * l, b);
@@ -506,7 +521,7 @@ __global__ void __launch_bounds__(256, TURN == kTurnAny ? 2 : 4)
     const int h = 4 * unit + sub, hc = h < p.hkv ? h : p.hkv - 1;
     float a[8], b[8];
     if (is_key) {
-      turn_and_store(a, b, x, y, kr + hc * p.k_stride_h,
+      turn_and_store(a, b, x, y,
                      static_cast<T*>(p.rotated_k) + k.token * p.rk_stride_t + hc * p.rk_stride_h,
                      p.rotated_k != nullptr && h < p.hkv);
     } else {
@@ -525,8 +540,7 @@ __global__ void __launch_bounds__(256, TURN == kTurnAny ? 2 : 4)
       if (4 * (u * U + i) >= p.hq) break;
       const int hc = h < p.hq ? h : p.hq - 1;
       float a[8], b[8];
-      turn_and_store(a, b, ra[i], rb[i], q + hc * p.q_stride_h, rq + hc * p.rq_stride_h,
-                     h < p.hq);
+      turn_and_store(a, b, ra[i], rb[i], rq + hc * p.rq_stride_h, h < p.hq);
     }
   }
   // This warp's first unit past the query rows.

@@ -124,6 +124,18 @@ def test_append_sizes(cuda_lib, tokens, hq, hkv):
     assert np.array_equal(cpu(a.pool.records), records)
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("pairs,offset", [(29, 0), (32, 0), (16, 8), (47, 0), (64, 3), (45, 1)])
+def test_append_many_tokens_of_partial_heads(cuda_lib, pairs, offset, interleaved):
+    a = Append(1203, hq=5, hkv=3, dtype=BF16, pairs=pairs, pad=7, offset=offset, seed=pairs)
+    q, k, records = a.expected(interleaved)
+    a.run(interleaved=interleaved, rotated_key=a.k, rotated_query=a.q)
+    keep = (a.slots >= 0).cpu()
+    same_rounded(a.q[keep.cuda()], q[keep.numpy()])
+    same_rounded(a.k[keep.cuda()], k[keep.numpy()])
+    assert np.array_equal(cpu(a.pool.records), records)
+
+
 def test_append_in_place_and_shared_center(cuda_lib):
     for offset in (0, 3):
         a = Append(50, hq=3, hkv=1, offset=offset)

@@ -69,6 +69,63 @@ def test_token_counts(cuda_lib, tokens):
         check(ko, k, cos[pos.long()], sin[pos.long()])
 
 
+@pytest.mark.parametrize("tokens,hq,hkv,dim,rotary_dim", [
+    (9473, 2, 1, 64, 26), (9473, 1, 1, 24, 24), (4740, 7, 2, 48, 44), (2369, 20, 4, 80, 34),
+    (3, 3, 1, 4096, 4090), (2, 3, 1, 4096, 4096), (3, 2, 1, 1000, 998), (2, 2, 1, 2050, 2050),
+    (1, 700, 300, 32, 30), (3, 40, 8, 256, 122), (1, 1, 0, 128, 58)])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_tiles_of_rows(cuda_lib, tokens, hq, hkv, dim, rotary_dim, interleaved, dtype):
+    """Several tokens to a block, a part of a token's rows, rows and pairs
+    wider than a block; in place as out of place."""
+    q, k = rows(tokens, hq, dim, dtype, 14).cuda(), rows(tokens, hkv, dim, dtype, 15).cuda()
+    cos, sin = rotary_tables(300, rotary_dim, device="cuda")
+    pos = (torch.arange(tokens, dtype=torch.int32, device="cuda") * 7) % 300
+    qo, ko = apply_rotary(q, k, cos, sin, pos, interleaved=interleaved)
+    at = pos.long()
+    check(qo, q, cos[at], sin[at], interleaved)
+    check(ko, k, cos[at], sin[at], interleaved)
+    apply_rotary(q, k, cos, sin, pos, interleaved=interleaved, query_out=q, key_out=k)
+    assert torch.equal(q, qo) and torch.equal(k, ko)
+
+
+@pytest.mark.parametrize("dim,rotary_dim,dtype", [
+    (128, 128, torch.float16), (128, 64, torch.bfloat16), (128, 128, torch.float32),
+    (64, 32, torch.float32), (80, 80, torch.float16)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_large_calls_equal_small_ones(cuda_lib, dim, rotary_dim, dtype, interleaved):
+    """More than 100 MB, and the same tokens some hundred at a time, bit for
+    bit; bad positions are left there too."""
+    size = torch.finfo(dtype).bits // 8
+    tokens = (105 << 20) // (2 * size * dim * 10) + 5
+    g = torch.Generator(device="cuda").manual_seed(16)
+    q = torch.randn(tokens, 8, dim, generator=g, device="cuda").to(dtype)
+    k = torch.randn(tokens, 2, dim, generator=g, device="cuda").to(dtype)
+    cos, sin = rotary_tables(4096, rotary_dim, device="cuda")
+    pos = torch.randint(0, 4096, (tokens,), generator=g, device="cuda").int()
+    pos[5] = -1
+    pos[tokens - 2] = 4096
+    out = torch.full_like(q, 7.0), torch.full_like(k, 7.0)
+    apply_rotary(q, k, cos, sin, pos, interleaved=interleaved, query_out=out[0], key_out=out[1])
+    assert read_device_error() == 2
+    for t in out:
+        assert (t[5] == 7).all() and (t[tokens - 2] == 7).all()
+    pos[5] = pos[tokens - 2] = 0
+    step = 997
+    for t0 in range(0, tokens, step):
+        some = slice(t0, t0 + step)
+        a, b = apply_rotary(q[some], k[some], cos, sin, pos[some], interleaved=interleaved)
+        for got, exp in ((out[0][some], a), (out[1][some], b)):
+            for bad in (5, tokens - 2):
+                if t0 <= bad < t0 + step:
+                    exp[bad - t0] = 7.0
+            assert torch.equal(got, exp)
+    apply_rotary(q, k, cos, sin, pos, interleaved=interleaved, query_out=q, key_out=k)
+    keep = torch.ones(tokens, dtype=torch.bool, device="cuda")
+    keep[5] = keep[tokens - 2] = False
+    assert torch.equal(q[keep], out[0][keep]) and torch.equal(k[keep], out[1][keep])
+
+
 @pytest.mark.parametrize("offset", [0, 1, 4, 8])
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
