@@ -440,7 +440,7 @@ enum { PG_INT4_RECORD_BYTES = 2560 };
 /* Rotation (as pg_rotary, pairs in 1..64) of query and key rows, then the
  * keys and values of any number of tokens, less their centres, written in 4
  * bits at slots[t] = physical page * 16 + token.  A negative slot skips its
- * token: nothing of it is read or written.  Every other slot may occur once
+ * token: nothing is written for it.  Every other slot may occur once
  * per call (with two tokens at one slot the slot's contents are undefined).
  * A slot outside the pool, a centre row outside the centres
  * (PG_DEV_BAD_PAGE_ID) or a position outside the table

@@ -1275,28 +1275,35 @@ int32_t pg_rope_append_int4(const pg_int4_append_args* a, void* stream) {
                                    : pg::kTurnOdd;
   // Few tokens: a warp per four rows.  Else eight query rows (or four key and
   // four value rows) at a time, a token's groups over as many warps as fill
-  // the GPU.
+  // the GPU; with one or two KV heads, the rows of four or two tokens.
   const int64_t fours = (p.hq + 3) / 4 + 2 * ((p.hkv + 3) / 4);
   const bool wide = a->tokens * fours > 148 * 16;
-  const int64_t units = wide ? (p.hq + 7) / 8 + (p.hkv + 3) / 4 : fours;
-  p.split = static_cast<int32_t>(
-      std::min<int64_t>(units, std::max<int64_t>(1, 148 * 64 / a->tokens)));
-  const int64_t warps = a->tokens * p.split;
+  p.row_shift = !wide || p.hkv > 2 ? 2 : p.hkv - 1;
+  const int64_t groups = (a->tokens + (4 >> p.row_shift) - 1) >> (2 - p.row_shift);
+  const int each = 1 << p.row_shift;
+  const int64_t units =
+      wide ? (p.hq + 2 * each - 1) / (2 * each) + (p.hkv + each - 1) / each : fours;
+  p.split =
+      static_cast<int32_t>(std::min<int64_t>(units, std::max<int64_t>(1, 148 * 64 / groups)));
+  const int64_t warps = groups * p.split;
   PG_REQUIRE((warps + 7) / 8 < (int64_t(1) << 31), "too many tokens");
   // Small blocks spread few warps over the SMs.
   const int block = wide ? 8 : 2;
   const dim3 grid(static_cast<unsigned>((warps + block - 1) / block));
   using Kernel = void (*)(pg::Int4AppendParams);
 #define PG_APPEND(T, TURN) \
-  {pg::pg_rope_append_int4_kernel<T, TURN, 1>, pg::pg_rope_append_int4_kernel<T, TURN, 2>}
+  {pg::pg_rope_append_int4_kernel<T, TURN, 1, false>, \
+   pg::pg_rope_append_int4_kernel<T, TURN, 2, false>, \
+   pg::pg_rope_append_int4_kernel<T, TURN, 2, true>}
 #define PG_APPEND_TURNS(T) \
   {PG_APPEND(T, pg::kTurnAny), PG_APPEND(T, pg::kTurnHalf), \
    PG_APPEND(T, pg::kTurnInterleaved), PG_APPEND(T, pg::kTurnPart), PG_APPEND(T, pg::kTurnOdd), \
    PG_APPEND(T, pg::kTurnOddInterleaved)}
-  const Kernel kernels[2][6][2] = {PG_APPEND_TURNS(__half), PG_APPEND_TURNS(__nv_bfloat16)};
+  const Kernel kernels[2][6][3] = {PG_APPEND_TURNS(__half), PG_APPEND_TURNS(__nv_bfloat16)};
 #undef PG_APPEND_TURNS
 #undef PG_APPEND
-  return launch_pdl(kernels[a->dtype == PG_DTYPE_BF16][turn][wide], grid, dim3(block * 32), 0,
+  const int form = !wide ? 0 : p.row_shift == 2 ? 1 : 2;
+  return launch_pdl(kernels[a->dtype == PG_DTYPE_BF16][turn][form], grid, dim3(block * 32), 0,
                     static_cast<cudaStream_t>(stream), "rope_append_int4 launch", p);
 }
 
@@ -1322,18 +1329,18 @@ int32_t pg_int4_read(const void* records, int64_t num_pages, int32_t kv_heads,
   p.value = value;
   p.error_flag = device_error_ptr();
   const bool wide = tokens * kv_heads > 148 * 64;
-  p.split = wide ? (kv_heads + 7) / 8 : (kv_heads + 1) / 2;
-  const int64_t warps = tokens * p.split;
+  const int64_t warps = (tokens * kv_heads + (wide ? 7 : 1)) / (wide ? 8 : 2);
   PG_REQUIRE((warps + 7) / 8 < (int64_t(1) << 31), "too many tokens");
   const int block = wide ? 8 : 2;
   const dim3 grid(static_cast<unsigned>((warps + block - 1) / block));
   using Kernel = void (*)(pg::Int4ReadParams);
-  const Kernel kernels[3][2] = {
-      {pg::pg_int4_read_kernel<__half, 1>, pg::pg_int4_read_kernel<__half, 4>},
-      {pg::pg_int4_read_kernel<__nv_bfloat16, 1>, pg::pg_int4_read_kernel<__nv_bfloat16, 4>},
-      {pg::pg_int4_read_kernel<float, 1>, pg::pg_int4_read_kernel<float, 4>}};
-  return launch_pdl(kernels[dtype][wide], grid, dim3(block * 32), 0,
-                    static_cast<cudaStream_t>(stream), "int4 read launch", p);
+#define PG_READ(T)                                                            \
+  {pg::pg_int4_read_kernel<T, 1, false>, pg::pg_int4_read_kernel<T, 4, false>, \
+   pg::pg_int4_read_kernel<T, 4, true>}
+  const Kernel kernels[3][3] = {PG_READ(__half), PG_READ(__nv_bfloat16), PG_READ(float)};
+#undef PG_READ
+  return launch_pdl(kernels[dtype][!wide ? 0 : kv_heads % 8 == 0 ? 2 : 1], grid, dim3(block * 32),
+                    0, static_cast<cudaStream_t>(stream), "int4 read launch", p);
 }
 
 int32_t pg_decode_int4_run(const pg_int4_decode_args* a, void* stream) {

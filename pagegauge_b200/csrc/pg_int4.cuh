@@ -245,7 +245,8 @@ struct Int4AppendParams {
   int64_t num_centers;
   int64_t tokens;
   int32_t hq, hkv, pairs, interleaved;
-  int32_t split;  // warps that share one token's rows
+  int32_t split;      // warps that share one token's rows
+  int32_t row_shift;  // a warp's four rows are of 4 >> row_shift tokens (FEW)
   int* error_flag;
 };
 
@@ -430,31 +431,41 @@ __device__ __forceinline__ void subtract_center(const Int4AppendParams& p, const
 // nothing is computed twice) and requests U times four query rows, or four
 // key and four value rows, before it uses the first.  U = 2 where tokens
 // alone fill the GPU: the table entries, slot and position are then read once
-// per token; U = 1 with a warp per four rows for few tokens, where latency is
-// all.  Bound by HBM: 57,304 tokens of 32 + 16 FP16 rows (1.277 GB) take
-// 206 us, 6.2 TB/s; with 16 lanes of one chunk per row, partners by shuffles,
-// 241 us; with a clamp, a conversion and a shift per code, 321 us.
-template <typename T, int TURN, int U>
+// per token, and with one or two KV heads (FEW) the four rows are of four or two
+// tokens (42,000 tokens of 1 + 2 rows with the read: 65.8 -> 24.4 us); U = 1
+// with a warp per four rows for few tokens, where latency is all.  Bound by
+// HBM: 57,304 tokens of 32 + 16 FP16 rows (1.277 GB) take 206 us, 6.2 TB/s;
+// with 16 lanes of one chunk per row, partners by shuffles, 241 us; with a
+// clamp, a conversion and a shift per code, 321 us.
+template <typename T, int TURN, int U, bool FEW>
 __global__ void __launch_bounds__(256, 4)
     pg_rope_append_int4_kernel(const __grid_constant__ Int4AppendParams p) {
   constexpr bool FAST = TURN != kTurnAny;
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, sub = lane >> 3, l = lane & 7;
   const int64_t w = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+  const int shift = FEW ? p.row_shift : 2, step = 1 << shift, hs = sub & (step - 1);
+  const int64_t tokens = p.split == 1 ? w : static_cast<uint32_t>(w) / p.split;  // w is small then
+  const int part = static_cast<int>(w - tokens * p.split);
   Int4Token k;
-  k.token = p.split == 1 ? w : static_cast<uint32_t>(w) / p.split;  // w is small if split
-  const int part = static_cast<int>(w - k.token * p.split);
+  k.token = tokens << (2 - shift);
   if (k.token >= p.tokens) return;
+  k.token += sub >> shift;
+  bool live = true;
+  if (FEW && k.token >= p.tokens) {
+    k.token = p.tokens - 1;
+    live = false;
+  }
   pdl_wait_primary();
   const int slot = p.slots[k.token];
-  const int pos = p.positions[k.token];
+  int pos = p.positions[k.token];
   k.center = p.center_rows != nullptr ? p.center_rows[k.token] : 0;
   // The first query rows are asked for along with the token's indices.
   const T* q = static_cast<const T*>(p.q) + k.token * p.q_stride_t;
-  const int nq = (p.hq + 4 * U - 1) / (4 * U), nk = (p.hkv + 3) >> 2;
+  const int nq = (p.hq + U * step - 1) / (U * step), nk = (p.hkv + step - 1) >> shift;
   uint4 ra[U], rb[U];
   auto load_rows = [&](const T* base, int stride, int heads, int unit, uint4& x, uint4& y) {
-    const int h = 4 * unit + sub;
+    const int h = step * unit + hs;
     const T* row = base + (h < heads ? h : heads - 1) * stride + 8 * l;
     x = load8<T, FAST>(row);
     y = load8<T, FAST>(row + 64);
@@ -464,17 +475,23 @@ __global__ void __launch_bounds__(256, 4)
     for (int i = 0; i < U; ++i) load_rows(q, p.q_stride_h, p.hq, u * U + i, ra[i], rb[i]);
   };
   if (part < nq) load_queries(part);
-  if (slot < 0) return;
+  // Skipped tokens, and those that are reported, store nothing.
+  live = live && slot >= 0;
   k.page = slot >> 4;
   k.tok = slot & 15;
-  if (k.page >= p.num_pages ||
-      (p.key_center != nullptr && (k.center < 0 || k.center >= p.num_centers))) {
+  if (live && (k.page >= p.num_pages ||
+               (p.key_center != nullptr && (k.center < 0 || k.center >= p.num_centers)))) {
     record_error(p.error_flag, kDevBadPageId);
-    return;
+    live = false;
   }
-  if (pos < 0 || pos >= p.table_rows) {
+  if (live && (pos < 0 || pos >= p.table_rows)) {
     record_error(p.error_flag, kDevBadPosition);
-    return;
+    live = false;
+  }
+  if (FEW ? !__any_sync(0xffffffffu, live) : !live) return;
+  if (FEW && !live) {
+    pos = 0;
+    k.page = k.center = 0;
   }
   Int4Turn t;
   t.cos_row = p.cos + pos * p.table_stride;
@@ -518,29 +535,30 @@ __global__ void __launch_bounds__(256, 4)
     }
   };
   auto append_rows = [&](const uint4& x, const uint4& y, bool is_key, int unit) {
-    const int h = 4 * unit + sub, hc = h < p.hkv ? h : p.hkv - 1;
+    const int h = step * unit + hs, hc = h < p.hkv ? h : p.hkv - 1;
     float a[8], b[8];
     if (is_key) {
       turn_and_store(a, b, x, y,
                      static_cast<T*>(p.rotated_k) + k.token * p.rk_stride_t + hc * p.rk_stride_h,
-                     p.rotated_k != nullptr && h < p.hkv);
+                     p.rotated_k != nullptr && (!FEW || live) && h < p.hkv);
     } else {
       unpack8<T>(x, a);
       unpack8<T>(y, b);
     }
     subtract_center<T>(p, k, is_key ? p.key_center : p.value_center, hc, l, a, b);
-    store_int4_row(p, k, is_key, h, l, a, b);
+    store_int4_row(p, k, is_key, !FEW || live ? h : p.hkv, l, a, b);
   };
   T* rq = static_cast<T*>(p.rotated_q) + k.token * p.rq_stride_t;
   for (int u = part; u < nq; u += p.split) {
     if (u != part) load_queries(u);
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int h = 4 * (u * U + i) + sub;
-      if (4 * (u * U + i) >= p.hq) break;
+      const int h = step * (u * U + i) + hs;
+      if (step * (u * U + i) >= p.hq) break;
       const int hc = h < p.hq ? h : p.hq - 1;
       float a[8], b[8];
-      turn_and_store(a, b, ra[i], rb[i], rq + hc * p.rq_stride_h, h < p.hq);
+      turn_and_store(a, b, ra[i], rb[i], rq + hc * p.rq_stride_h,
+                     (!FEW || live) && h < p.hq);
     }
   }
   // This warp's first unit past the query rows.
@@ -569,31 +587,40 @@ struct Int4ReadParams {
   const int32_t* slots;
   int64_t tokens;
   int32_t hkv;
-  int32_t split;  // warps that share one token's heads
   void* key;      // [T, Hkv, 128]
   void* value;    // [T, Hkv, 128]
   int* error_flag;
 };
 
-// One warp per token and 2 U KV heads (16 lanes per head's key and value row),
-// with everything requested before it is used; skipped slots read as zeros.
-// U = 4 where tokens alone fill the GPU, as in the append.
-template <typename T, int U>
+// A warp reads 2 U rows (KV heads of consecutive tokens), 16 lanes per row's
+// key and value, with everything requested before it is used; skipped slots
+// read as zeros.  U = 4 where the rows alone fill the GPU, as in the append.
+// SAME: the KV heads are a multiple of 2 U, so a warp's rows are one token's
+// (57,304 tokens of 8 heads: 57 us, 63 us with the tokens followed).
+template <typename T, int U, bool SAME>
 __global__ void __launch_bounds__(256)
     pg_int4_read_kernel(const __grid_constant__ Int4ReadParams p) {
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, half = lane >> 4, m = lane & 15, grp = m >> 2;
   const int64_t w = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+  const int64_t end = p.tokens * p.hkv;
+  if (2 * U * w >= end) return;
+  const int64_t first = 2 * U * w + half;  // of this half warp
   // A 32-bit division where the index allows it.
-  const int64_t token = w < (int64_t(1) << 31)
-                            ? static_cast<int64_t>(static_cast<uint32_t>(w) / p.split)
-                            : w / p.split;
-  if (token >= p.tokens) return;
-  const int h0 = 2 * U * static_cast<int>(w - token * p.split) + half;
+  int64_t token = first < (int64_t(1) << 31)
+                      ? static_cast<int64_t>(static_cast<uint32_t>(first) / p.hkv)
+                      : first / p.hkv;
+  int h = static_cast<int>(first - token * p.hkv);
   pdl_wait_primary();
-  const int slot = p.slots[token];
-  const bool held = slot >= 0 && (slot >> 4) < p.num_pages;
-  if (slot >= 0 && !held) record_error(p.error_flag, kDevBadPageId);
+  int slot = -1;
+  auto load_slot = [&](bool held) {
+    slot = held ? p.slots[token] : -1;
+    if (slot >= 0 && (slot >> 4) >= p.num_pages) {
+      record_error(p.error_flag, kDevBadPageId);
+      slot = -1;
+    }
+  };
+  if constexpr (SAME) load_slot(true);
   uint32_t codes[U][2];
   __half s[U][2], mid[U][2];
 #pragma unroll
@@ -603,8 +630,8 @@ __global__ void __launch_bounds__(256)
       codes[i][kv] = 0u;
       s[i][kv] = mid[i][kv] = __ushort_as_half(0);
     }
-    const int h = h0 + 2 * i;
-    if (held && h < p.hkv) {
+    if constexpr (!SAME) load_slot(first + 2 * i < end);
+    if (slot >= 0) {
       const int tok = slot & 15;
       const uint8_t* rec =
           p.records + (static_cast<int64_t>(slot >> 4) * p.hkv + h) * kInt4Record;
@@ -620,16 +647,18 @@ __global__ void __launch_bounds__(256)
       s[i][1] = vm[0];
       mid[i][1] = vm[4];
     }
+    h += 2;
+    if constexpr (!SAME)
+      for (; h >= p.hkv; h -= p.hkv) ++token;
   }
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     const uint32_t other = __shfl_xor_sync(0xffffffffu, codes[i][1], 4);
     codes[i][1] = (grp & 1) ? prmt(other, codes[i][1], 0x7632u) : prmt(codes[i][1], other, 0x5410u);
-    const int h = h0 + 2 * i;
+    const int64_t row = first + 2 * i;
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
-      T* out = static_cast<T*>(kv == 0 ? p.key : p.value) +
-               (token * p.hkv + (h < p.hkv ? h : 0)) * kHeadDim + 8 * m;
+      T* out = static_cast<T*>(kv == 0 ? p.key : p.value) + row * kHeadDim + 8 * m;
       const float sc = __half2float(s[i][kv]), md = __half2float(mid[i][kv]);
       float x[8];
 #pragma unroll
@@ -641,7 +670,7 @@ __global__ void __launch_bounds__(256)
         x[j] = __fadd_rn(__fmul_rn(f.x, sc), md);
         x[j + 4] = __fadd_rn(__fmul_rn(f.y, sc), md);
       }
-      if (h >= p.hkv) continue;
+      if (!SAME && row >= end) continue;
       if constexpr (sizeof(T) == 2) {
         store8<T, true>(out, x);
       } else {

@@ -302,8 +302,8 @@ class AppendExtension:
         projection are fine); ``cosine``/``sine`` FP32 [positions,pairs] from
         ``rotary.rotary_tables`` (``pairs`` < 64 rotates part of the head);
         ``positions`` and ``token_slots`` (physical page * 16 + token) device
-        int32 [T].  A negative slot skips its token (padding): none of its
-        rows is read or written.  Every other slot may occur once per call.
+        int32 [T].  A negative slot skips its token (padding): nothing
+        is written for it.  Every other slot may occur once per call.
         ``records`` is the pool's [pages,Hkv,2560] uint8.  With
         ``key_center``/``value_center`` [C,Hkv,128] the rows' centres (row
         ``center_rows[t]``, or row 0) are subtracted before quantising; the

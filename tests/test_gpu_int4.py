@@ -201,6 +201,43 @@ def test_append_reports_bad_tokens_and_skips_them(cuda_lib):
             assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("tokens,hq,hkv", [(4003, 1, 1), (4001, 7, 1), (3001, 6, 2), (5002, 2, 2),
+                                           (3203, 5, 3), (2003, 7, 5), (1201, 8, 8)])
+@pytest.mark.parametrize("pairs", [64, 29])
+def test_append_and_read_of_many_tokens(cuda_lib, tokens, hq, hkv, pairs):
+    """Rows of several tokens in one warp; skipped, refused and last tokens
+    leave the others whole.  The read of many tokens is that of few."""
+    a = Append(tokens, hq=hq, hkv=hkv, pairs=pairs, pad=9, seed=tokens)
+    bad = torch.arange(3, tokens, 331)
+    a.positions[bad[0::2].cuda()] = 5000
+    a.kw["center_rows"][bad[1::2].cuda()] = -1
+    stored = torch.ones(tokens, dtype=torch.bool)
+    stored[bad] = False
+    given, slots = a.slots, a.slots.clone()
+    slots[bad.cuda()] = -1
+    safe = a.positions.clamp(max=4999), a.kw["center_rows"].clamp(min=0)
+    real = a.positions, a.kw["center_rows"]
+    a.slots, a.positions, a.kw["center_rows"] = slots, *safe
+    q, _, records = a.expected()
+    a.slots, a.positions, a.kw["center_rows"] = given, *real
+    a.run()
+    assert read_device_error() in (2, 3)
+    stored &= (given >= 0).cpu()
+    same_rounded(a.rotated[stored.cuda()], q[stored.numpy()])
+    assert (a.rotated[~stored.cuda()] == 9).all()
+    assert np.array_equal(cpu(a.pool.records), records)
+    slots[5] = 16 * a.pool.num_pages
+    slots[stored.nonzero()[-1].item()] = -1
+    key, value = a.pool.read(slots)
+    assert read_device_error() == 3
+    for t0 in range(0, tokens, 997):  # few rows each
+        few = a.pool.read(slots[t0:t0 + 997])
+        read_device_error()
+        assert torch.equal(key[t0:t0 + 997], few[0]) and torch.equal(value[t0:t0 + 997], few[1])
+    skipped = (slots < 0) | (slots >= 16 * a.pool.num_pages)
+    assert (key[skipped] == 0).all() and (value[skipped] == 0).all()
+
+
 def test_read_matches_the_records(cuda_lib):
     a = Append(40, hkv=3, pad=4)
     a.run()
