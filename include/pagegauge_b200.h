@@ -518,6 +518,13 @@ typedef struct pg_int4_decode_args {
 
 int32_t pg_decode_int4_run(const pg_int4_decode_args* args, void* stream);
 
+/* Host-only: the pages per work item (a multiple of `multiple`, at most 128)
+ * that pg_decode_int4_run is fastest with, for pg_decode_plan; indptr as
+ * there, group the query heads of a KV head.                              */
+int32_t pg_int4_split_pages(int32_t batch, int32_t kv_heads, int32_t group,
+                            const int32_t* indptr, int32_t num_sms,
+                            int32_t multiple, int32_t* split);
+
 /* ---------------------------------------------------------------------- */
 /* Decoder-layer element-wise steps around the attention path (the Mistral   */
 /* layer body of scripts/benchmark_page_gauge_transformer.py:2754-2804).    */

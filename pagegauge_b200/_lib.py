@@ -167,6 +167,7 @@ _SIGNATURES = {
     "pg_rope_append_int4": (c_i32, [c_vp, c_vp]),
     "pg_int4_read": (c_i32, [c_vp, c_i64, c_i32, c_vp, c_i64, c_vp, c_vp, c_i32, c_vp]),
     "pg_decode_int4_run": (c_i32, [c_vp, c_vp]),
+    "pg_int4_split_pages": (c_i32, [c_i32, c_i32, c_i32, c_vp, c_i32, c_i32, c_i32p]),
     "pg_quantize_affine_group16": (c_i32, [c_vp, c_i64, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp]),
 }
 

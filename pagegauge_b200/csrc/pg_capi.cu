@@ -1343,6 +1343,67 @@ int32_t pg_int4_read(const void* records, int64_t num_pages, int32_t kv_heads,
                     0, static_cast<cudaStream_t>(stream), "int4 read launch", p);
 }
 
+// The time of a split in microseconds: the pages of a block's items, round by
+// round, at a rate that falls with the blocks that still run, and a start-up
+// for every further item.  Fitted to sweeps of splits (one request of 49,152
+// tokens and 8 heads in items of 56 / 96 / 128 pages: 17.8 / 23.4 / 25.6 us;
+// four of 62,769 tokens and 4 heads in items of 64 / 72 / 80 / 96 / 128 pages,
+// 2.2 / 2.0 / 1.8 / 1.5 / 1.1 rounds of 444 blocks: 42.1 / 36.4 / 38.6 / 43.5
+// / 45.4 us; more than four heads to a group 15 % more).
+int32_t pg_int4_split_pages(int32_t batch, int32_t kv_heads, int32_t group, const int32_t* indptr,
+                            int32_t num_sms, int32_t multiple, int32_t* split) {
+  PG_REQUIRE(batch > 0 && kv_heads > 0 && kv_heads < 65536, "batch and kv heads must be positive");
+  PG_REQUIRE(indptr != nullptr && split != nullptr, "indptr and an output are required");
+  PG_REQUIRE(num_sms > 0 && multiple > 0, "SM count and multiple must be positive");
+  constexpr int kMost = 32 * pg::kInt4Warps;  // pages of an item
+  const int64_t blocks = static_cast<int64_t>(num_sms) * pg::kInt4CtasPerSm;
+  for (int r = 0; r < batch; ++r)
+    PG_REQUIRE(indptr[r] >= 0 && indptr[r + 1] >= indptr[r], "indptr must be non-decreasing");
+  *split = std::min(multiple, kMost);
+  double best = 1e300;
+  for (int s = *split; s <= kMost; s += multiple) {
+    int64_t with[kMost + 1] = {0};  // items of a size
+    int64_t items = 0, empty = 0;
+    for (int r = 0; r < batch; ++r) {
+      const int32_t n = indptr[r + 1] - indptr[r];
+      with[s] += static_cast<int64_t>(n / s) * kv_heads;
+      if (n % s != 0) with[n % s] += kv_heads;
+      if (n == 0) ++empty;
+      items += static_cast<int64_t>((n + s - 1) / s) * kv_heads;
+    }
+    if (items == 0) return PG_OK;
+    // Sizes by rank, largest first; a page's time in round k.
+    std::vector<int32_t> size;
+    size.reserve(static_cast<size_t>(std::min(items, 2 * blocks)));
+    std::vector<int32_t> later;  // the largest of every round after the second
+    int64_t rank = 0;
+    for (int x = s; x > 0; --x) {
+      const int64_t end = rank + with[x];
+      for (; rank < end && rank < 2 * blocks; ++rank) size.push_back(x);
+      for (int64_t k = 2 + static_cast<int64_t>(later.size()); k * blocks < end; ++k)
+        later.push_back(x);
+      rank = end;
+    }
+    const double head = group > 4 ? 1.15 : 1.0;
+    auto page = [&](int64_t round) {
+      const double running = static_cast<double>(items - round * blocks) / blocks;
+      return head * (0.12 + 0.06 * std::min(1.0, running));
+    };
+    double cost = size[0] * page(0);
+    for (int64_t i = blocks; i < static_cast<int64_t>(size.size()); ++i)
+      cost = std::max(cost, size[2 * blocks - 1 - i] * page(0) + size[i] * page(1));
+    for (size_t k = 0; k < later.size(); ++k) cost += later[k] * page(static_cast<int64_t>(k) + 2);
+    cost += 2.6 * static_cast<double>((items - 1) / blocks);
+    const bool join = empty != 0 || items != static_cast<int64_t>(batch) * kv_heads;
+    if (join) cost += 2.5;
+    if (cost < best - 1e-9) {
+      best = cost;
+      *split = s;
+    }
+  }
+  return PG_OK;
+}
+
 int32_t pg_decode_int4_run(const pg_int4_decode_args* a, void* stream) {
   PG_REQUIRE(a != nullptr, "null arguments");
   PG_REQUIRE(a->batch > 0 && a->kv_heads > 0, "batch and kv heads must be positive");

@@ -224,7 +224,6 @@ class BatchDecodeWithPagedKVCacheWrapper:
     (page, head, 16-dim group).
     """
 
-    _split_multiple = 1  # of an automatic split, in pages
     _largest_first = False  # the order of the work items
 
     def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD",
@@ -309,11 +308,10 @@ class BatchDecodeWithPagedKVCacheWrapper:
         sms = num_sms(self._ws.buffer.device)
         seg0 = ind if self._first_segment else None
         seg1 = None if self._first_segment else ind
+        if split == 0:
+            split = self._automatic_split(ind, num_kv_heads, num_qo_heads // num_kv_heads, sms)
         items, off, info = plan_items(batch, num_kv_heads, seg0, seg1,
                                       min(split, 1 << 30), min(split, 1 << 30), sms)
-        if split == 0 and info.split_pages[0] % self._split_multiple:
-            split = -(-info.split_pages[0] // self._split_multiple) * self._split_multiple
-            items, off, info = plan_items(batch, num_kv_heads, seg0, seg1, split, split, sms)
         self._plan = PagedDecodePlan(self._ws, items, off, info, batch, num_kv_heads,
                                      num_qo_heads // num_kv_heads, self._largest_first)
         self._indices = dev_indices
@@ -322,6 +320,9 @@ class BatchDecodeWithPagedKVCacheWrapper:
         self._num_kv_heads = num_kv_heads
 
     begin_forward = plan
+
+    def _automatic_split(self, indptr: np.ndarray, kv_heads: int, group: int, sms: int) -> int:
+        return 0  # the planner's
 
     @property
     def split_pages(self) -> int:
@@ -392,9 +393,9 @@ class Int4DecodeWrapper(BatchDecodeWithPagedKVCacheWrapper):
     at a time: concurrent streams (or graphs replayed concurrently) need a
     wrapper each."""
 
-    # The kernel's four warps take pages in pairs: an automatic split is
-    # rounded up to whole pairs (4,096 tokens: 5 pages 7.9 us, 8 pages 7.1 us;
-    # 16,384: 19 pages 11.5 us, 24 pages 10.7 us).
+    # The kernel's four warps take pages in pairs: an automatic split is of
+    # whole pairs (4,096 tokens: 5 pages 7.9 us, 8 pages 7.1 us; 16,384: 19
+    # pages 11.5 us, 24 pages 10.7 us).
     _split_multiple = 8
     _largest_first = True
 
@@ -404,6 +405,12 @@ class Int4DecodeWrapper(BatchDecodeWithPagedKVCacheWrapper):
             raise ValueError("choose one representation")
         self._kv_dtype = torch.uint8
         self._first_segment = True
+
+    def _automatic_split(self, indptr: np.ndarray, kv_heads: int, group: int, sms: int) -> int:
+        split = ctypes.c_int32()
+        _lib.call("pg_int4_split_pages", indptr.size - 1, kv_heads, group, indptr.ctypes.data, sms,
+                  self._split_multiple, ctypes.byref(split))
+        return split.value
 
     def plan(self, indptr: torch.Tensor, indices: torch.Tensor, last_page_len: torch.Tensor,
              *args, **kwargs) -> None:

@@ -446,6 +446,33 @@ def test_attention_more_items_than_blocks(cuda_lib, split, group):
         assert torch.equal(out, again) and torch.equal(lse, lse2)
 
 
+@pytest.mark.parametrize("rounds", [1.0, 1.01, 1.6, 2.0, 2.01, 2.5, 3.0, 3.01, 4.3])
+def test_attention_rounds_of_items(cuda_lib, rounds):
+    """Plans of just under and over whole rounds of items; every run leaves the
+    counter at zero, and splits agree within their bounds."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    items = int(rounds * 3 * sms)
+    rng = np.random.default_rng(items)
+    lengths = [int(n) for n in rng.integers(1, 129, 40)]
+    while sum(-(-n // 16) for n in lengths) < items:
+        lengths.append(int(rng.integers(1, 129)))
+    lengths[-1] -= 16 * (sum(-(-n // 16) for n in lengths) - items)
+    if lengths[-1] <= 0:
+        lengths[-1] = 16
+    a = Attend(lengths, hkv=1, group=3, split=1, seed=items)
+    assert a.wrapper._plan.num_items in (items, items + 1)
+    out, lse = a.run()
+    a.check(out, lse)
+    for _ in range(3):
+        again = a.run()
+        assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+    for split in (0, 3):
+        a.split = split
+        a.plan()
+        a.check(*a.run())
+    assert read_device_error() == 0
+
+
 def test_attention_last_page_without_tokens(cuda_lib):
     a = Attend([33, 16], seed=16)
     a.last[:] = 0  # 32 tokens, and none

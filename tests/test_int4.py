@@ -151,6 +151,41 @@ def test_automatic_splits_are_whole_pairs_of_four_warps():
     assert info.split_pages[0] == split == 8 and off[-1] == 8 * 32
 
 
+def split_pages(pages, kv_heads, group=4, sms=148, multiple=8):
+    indptr = np.concatenate([[0], np.cumsum(pages)]).astype(np.int32)
+    split = ctypes.c_int32()
+    _lib.call("pg_int4_split_pages", len(pages), kv_heads, group, indptr.ctypes.data, sms, multiple,
+              ctypes.byref(split))
+    return split.value
+
+
+@pytest.mark.parametrize("pages,kv_heads,group,best", [
+    # The fastest of measured splits, or one within 3 % of it.
+    ([3923] * 4, 4, 4, (72,)), ([3923] * 4, 4, 7, (72,)), ([3000], 8, 4, (56,)),
+    ([6250], 8, 4, (120,)), ([8192], 8, 4, (80,)), ([256], 8, 8, (8,)), ([63], 8, 4, (8,)),
+    ([53] * 22, 8, 5, (32,)), ([256] * 32, 8, 4, (88,)), ([13] * 64, 8, 4, (16,)),
+    ([713] * 12, 1, 8, (24,)), ([128] * 64, 8, 4, (64, 72, 48)), ([512] * 16, 8, 4, (80, 88))])
+def test_automatic_split_is_the_measured_one(pages, kv_heads, group, best):
+    assert split_pages(pages, kv_heads, group) in best
+
+
+def test_automatic_split_of_any_plan():
+    rng = np.random.default_rng(5)
+    assert split_pages([0, 0], 4) == 8
+    for _ in range(200):
+        pages = rng.integers(0, rng.integers(2, 5000), rng.integers(1, 80))
+        split = split_pages(list(pages), int(rng.integers(1, 9)), int(rng.integers(1, 9)),
+                            int(rng.integers(1, 200)))
+        assert split % 8 == 0 and 8 <= split <= 128
+    assert split_pages([100], 1, multiple=500) == 128
+    split, bad = ctypes.c_int32(), np.array([0, 4, 2], np.int32)
+    for args in ((0, 1, 4, bad.ctypes.data, 148, 8), (2, 0, 4, bad.ctypes.data, 148, 8),
+                 (2, 1, 4, bad.ctypes.data, 148, 8), (1, 1, 4, None, 148, 8),
+                 (1, 1, 4, bad.ctypes.data, 0, 8), (1, 1, 4, bad.ctypes.data, 148, 0)):
+        with pytest.raises((RuntimeError, ValueError)):
+            _lib.call("pg_int4_split_pages", *args, ctypes.byref(split))
+
+
 def test_binding_refuses_what_is_not_a_cuda_tensor():
     ops = _lib.torch_ops()
     q = torch.zeros(2, 4, 128, dtype=torch.float16)
