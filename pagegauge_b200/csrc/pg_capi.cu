@@ -1129,15 +1129,17 @@ int32_t pg_rotary(const pg_rotary_args* a, void* stream) {
                         aligned(a->cosine, 4 * table_floats) &&
                         aligned(a->sine, 4 * table_floats) && a->table_stride % table_floats == 0;
   // Whole 16-byte chunks of turning dims need no shared memory, which is
-  // faster where the call stays in the L2 (1,000 tokens of 40 FP16 rows of 128
-  // dims: 5.7 against 6.8 us; interleaved 6.9 / 7.1) and for 16-bit heads that
-  // turn whole in half layout (16,000 tokens: 61.1 / 62.8 us; interleaved 66.8
-  // / 63.6, half of the head 66.0 / 54.1, FP32 108.9 / 104.7 us).
-  const bool large = a->tokens * rows * a->head_dim * size * 2 > int64_t(100) << 20;
+  // faster for few bytes (40 FP16 rows of 128 dims, inputs not in the L2: 8 MB
+  // 2.9 against 4.8 us, 16 MB 6.3 / 7.0, 24 MB 9.5 / 8.7, 40 MB of which half
+  // turns 13.3 / 10.4, interleaved 12.7 / 10.2, FP32 13.3 / 10.1 us), and for
+  // 16-bit heads that turn whole in half layout again for many (150 MB 33.9 /
+  // 32.1, 328 MB 61.1 / 62.8, 1 GB 173 / 181 us).
+  const int64_t bytes = a->tokens * rows * a->head_dim * size * 2;
   const bool whole_head = size == 2 && !p.interleaved && 2 * a->pairs == a->head_dim;
+  const bool direct = bytes < int64_t(20) << 20 || (whole_head && bytes > int64_t(256) << 20);
   using Kernel = void (*)(pg::RotaryParams);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (chunks16 && (!large || whole_head)) {
+  if (chunks16 && direct) {
     p.chunks = p.interleaved ? 2 * a->pairs / v : a->pairs / v;
     // Rows per thread once there are rows enough for every thread slot four
     // times over, else one: more rows per thread read fewer table entries.

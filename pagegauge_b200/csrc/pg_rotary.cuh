@@ -34,10 +34,11 @@ struct RotaryParams {
 };
 
 // Rows that are 16-byte aligned and whose parts are whole 16-byte chunks, where
-// few tokens or whole heads make the copies through shared memory the slower
-// way.  A thread takes one turning chunk (half layout: of both halves) of every
-// row_groups-th row of one token, so it reads its table entries once, and the
-// rows' copied chunks with it, two rows requested before the first is used.
+// little data, or much of whole heads, makes the way through shared memory the
+// slower one.  A thread takes one turning chunk (half layout: of both halves)
+// of every row_groups-th row of one token, so it reads its table entries once,
+// and the rows' copied chunks with it, two rows requested before the first is
+// used.
 // Bound by HBM (each row is read and written once), so what counts is bytes in
 // flight against registers: interleaved rows hold half as much per thread and
 // run six blocks per SM (8,191 tokens: 32.9 us, 38.4 us with four rows in
