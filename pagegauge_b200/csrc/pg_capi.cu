@@ -1141,12 +1141,9 @@ int32_t pg_rotary(const pg_rotary_args* a, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (chunks16 && direct) {
     p.chunks = p.interleaved ? 2 * a->pairs / v : a->pairs / v;
-    // Rows per thread once there are rows enough for every thread slot four
-    // times over, else one: more rows per thread read fewer table entries.
-    // (49,152 tokens, half layout: 288 / 188 / 179 / 174 us at 1 / 2 / 4 / 8;
-    // 8,191 interleaved: 43.7 / 32.7 / 33.0 / 36.0 us.)
-    const int64_t threads = a->tokens * rows * p.chunks;
-    const int64_t each = threads < 148 * 2048 * 4 ? 1 : p.interleaved ? 4 : 8;
+    // Rows per thread: one for little data, else more read fewer table entries
+    // (49,152 tokens: 288 / 188 / 179 / 174 us at 1 / 2 / 4 / 8).
+    const int64_t each = whole_head && bytes > int64_t(256) << 20 ? 8 : 1;
     p.row_groups = static_cast<int32_t>((rows + each - 1) / each);
     const int64_t per_token = static_cast<int64_t>(p.chunks) * p.row_groups;
     PG_REQUIRE(per_token < (int64_t(1) << 30), "too many rows");

@@ -39,10 +39,11 @@ struct RotaryParams {
 // of every row_groups-th row of one token, so it reads its table entries once,
 // and the rows' copied chunks with it, two rows requested before the first is
 // used.
-// Bound by HBM (each row is read and written once), so what counts is bytes in
-// flight against registers: interleaved rows hold half as much per thread and
-// run six blocks per SM (8,191 tokens: 32.9 us, 38.4 us with four rows in
-// flight on four blocks), half-layout rows four.
+// Bound by latency where there is little data, by HBM where there is much (each
+// row is read and written once: 49,152 tokens of 40 FP16 rows, 1.03 GB, 174
+// us, 5.9 TB/s), so bytes in flight count against registers: interleaved rows
+// hold half as much per thread and run six blocks per SM, half-layout rows
+// four.
 template <typename T, bool INTERLEAVED>
 __global__ void __launch_bounds__(256, INTERLEAVED ? 6 : 4)
     pg_rotary_kernel(const __grid_constant__ RotaryParams p) {

@@ -126,6 +126,25 @@ def test_large_calls_equal_small_ones(cuda_lib, dim, rotary_dim, dtype, interlea
     assert torch.equal(q[keep], out[0][keep]) and torch.equal(k[keep], out[1][keep])
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_whole_heads_past_256_mb(cuda_lib, dtype):
+    tokens = (257 << 20) // (2 * 2 * 128 * 13) + 3
+    g = torch.Generator(device="cuda").manual_seed(17)
+    q = torch.randn(tokens, 10, 128, generator=g, device="cuda").to(dtype)
+    k = torch.randn(tokens, 3, 128, generator=g, device="cuda").to(dtype)
+    cos, sin = rotary_tables(4096, 128, device="cuda")
+    pos = torch.randint(0, 4096, (tokens,), generator=g, device="cuda").int()
+    for adjoint in (False, True):
+        qo, ko = apply_rotary(q, k, cos, sin, pos, adjoint=adjoint)
+        for t0 in range(0, tokens, 2999):
+            some = slice(t0, t0 + 2999)
+            a, b = apply_rotary(q[some], k[some], cos, sin, pos[some], adjoint=adjoint)
+            assert torch.equal(qo[some], a) and torch.equal(ko[some], b)
+    check(qo[-40:], q[-40:], cos[pos[-40:].long()], sin[pos[-40:].long()], adjoint=True)
+    apply_rotary(q, k, cos, sin, pos, adjoint=True, query_out=q, key_out=k)
+    assert torch.equal(q, qo) and torch.equal(k, ko)
+
+
 @pytest.mark.parametrize("offset", [0, 1, 4, 8])
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
