@@ -331,8 +331,8 @@ class PageGaugeDecoder:
             self.cos, self.sin = rotary_tables(self.max_context, HEAD_DIM, cfg.rope_theta,
                                                device=dev)
             # Request r's token at position p lies at slot r * capacity + p.
-            self.slots = torch.zeros(B, dtype=torch.int32, **z)
             self.center_rows = torch.arange(B, dtype=torch.int32, **z)
+            self.slots = self.center_rows * self.max_context
         else:
             self.cos, self.sin = rope_tables(self.max_context, cfg.rope_theta, device=dev)
         qkv_w = (self.hq + 2 * hkv) * HEAD_DIM

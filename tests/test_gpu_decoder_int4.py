@@ -142,3 +142,34 @@ def test_refusals(cuda_lib):
                dict(kv_cache="int4", ring_pages=4), dict(kv_cache="int4", suffix_pages=1)):
         with pytest.raises(ValueError):
             PageGaugeDecoder(weights, batch=1, max_context=64, **kw)
+
+
+def test_steps_without_a_prompt(cuda_lib):
+    """Decoding from an empty cache: every request appends to its own pages, so
+    each follows a decoder that runs it alone.  Their logits differ by the FP16
+    roundings of the projections' sums alone."""
+    weights = random_decoder_weights(SMALL, 8, device="cuda")
+    first = torch.tensor([3, 77, 400], device="cuda")
+    alone = []
+    steps = 18  # crosses a page
+    feed = torch.randint(0, SMALL.vocab, (steps, 3),
+                         generator=torch.Generator().manual_seed(9)).cuda()
+    feed[0] = first
+    for batch in (slice(0, 3), slice(0, 1), slice(1, 2), slice(2, 3)):
+        n = batch.stop - batch.start
+        dec = PageGaugeDecoder(weights, batch=n, max_context=40, kv_cache="int4", gemm="cublas")
+        logits = []
+        for i in range(steps):
+            dec.tokens.copy_(feed[i, batch])
+            dec.step(use_graph=i > 2)
+            logits.append(dec.logits.float().clone())
+        assert dec.slots.tolist() == [r * dec.max_context + steps for r in range(n)]
+        # Every request's pages hold its tokens.
+        for r in range(n):
+            at = torch.arange(steps, dtype=torch.int32, device="cuda") + r * dec.max_context
+            key, value = dec.pools[0].read(at, dtype=torch.float32)
+            assert (key.abs().amax((1, 2)) > 0).all() and (value.abs().amax((1, 2)) > 0).all()
+        alone.append(torch.stack(logits, 1))
+    together, single = alone[0], torch.cat(alone[1:])
+    cos = torch.nn.functional.cosine_similarity(together, single, dim=-1)
+    assert float(cos.min()) >= 0.999 and read_device_error() == 0
