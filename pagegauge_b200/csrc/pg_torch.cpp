@@ -10,6 +10,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -60,8 +61,17 @@ const Tensor* arg(PyObject* o, const char* name, bool optional = false) {
   return &THPVariable_Unpack(o);
 }
 
-// Rows and tables whose gradient a call would lose.
+// Forward-mode derivatives, which need no requires_grad and no grad mode.
+void check_no_tangent(std::initializer_list<const Tensor*> tensors) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : tensors)
+    if (t != nullptr && t->_fw_grad(0).defined())
+      refuse("this operator has no forward-mode derivative: unpack its inputs' duals");
+}
+
+// Rows, tables and outputs whose derivative a call would lose.
 void check_no_grad(std::initializer_list<const Tensor*> tensors) {
+  check_no_tangent(tensors);
   if (!at::GradMode::is_enabled()) return;
   for (const Tensor* t : tensors)
     if (t != nullptr && t->requires_grad())
@@ -192,6 +202,7 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor& positions = *arg(a[4], "positions");
     const Tensor* query_out = arg(a[7], "query_out", true);
     const Tensor* key_out = arg(a[8], "key_out", true);
+    check_no_tangent({&query, key});
     if (at::GradMode::is_enabled() &&
         (query.requires_grad() || (key != nullptr && key->requires_grad())))
       Py_RETURN_NONE;

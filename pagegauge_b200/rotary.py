@@ -147,7 +147,7 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, cosine: torch.Te
     dim j with j + pairs, ``interleaved`` 2j with 2j + 1.  ``adjoint`` turns
     back (the gradient of the rotation with respect to its rows, which autograd
     takes for rows that require one; the call then makes its outputs and is
-    not captured into a graph).  Rows are
+    not captured into a graph; forward-mode duals are refused).  Rows are
     float16, bfloat16 or float32 with a contiguous last dimension and any
     other strides.  The outputs may be the inputs (in place); they must not
     overlap them in any other way.  Rows of a token whose position is outside

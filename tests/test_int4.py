@@ -202,3 +202,40 @@ def test_binding_refuses_what_is_not_a_cuda_tensor():
         ops.decode_int4(b"", 0, q, q, 1.0, None, None, None, False)
     with pytest.raises(TypeError, match="arguments"):
         ops.rotary(q)
+
+
+def test_binding_refuses_forward_mode_duals():
+    """A dual tensor does not require a gradient; its tangent would be lost all
+    the same, with gradients recorded or not."""
+    import torch.autograd.forward_ad as forward
+
+    ops = _lib.torch_ops()
+    plain = torch.zeros(2, 4, 128)
+    plan = bytes(ctypes.sizeof(_lib.PgInt4DecodeArgs))
+    with forward.dual_level():
+        dual = forward.make_dual(plain, torch.ones_like(plain))
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode():
+                for at in (0, 1, 2, 3, 7, 8):
+                    args = [plain] * 9
+                    args[at], args[5], args[6] = dual, False, False
+                    with pytest.raises(ValueError, match="forward-mode"):
+                        ops.rotary(*args)
+                for at in (0, 1, 2, 3, 4, 7, 9, 10, 12):
+                    args = [plain] * 14
+                    args[at], args[13] = dual, False
+                    with pytest.raises(ValueError, match="forward-mode"):
+                        ops.rope_append_int4(*args)
+                for at in (3, 4):
+                    args = [plain, plain, torch.float16, plain, plain]
+                    args[at] = dual
+                    with pytest.raises(ValueError, match="forward-mode"):
+                        ops.int4_read(*args)
+                for at in (2, 5, 6, 7):
+                    args = [plan, 0, plain, plain, 1.0, plain, plain, plain, False]
+                    args[at] = dual
+                    with pytest.raises(ValueError, match="forward-mode"):
+                        ops.decode_int4(*args)
+        rows = forward.make_dual(plain.clone().requires_grad_(), torch.ones_like(plain))
+        with pytest.raises(ValueError, match="forward-mode"):
+            ops.rotary(rows, None, plain, plain, plain, False, False, None, None)
