@@ -1360,7 +1360,8 @@ int32_t pg_int4_split_pages(int32_t batch, int32_t kv_heads, int32_t group, cons
     PG_REQUIRE(indptr[r] >= 0 && indptr[r + 1] >= indptr[r], "indptr must be non-decreasing");
   *split = std::min(multiple, kMost);
   double best = 1e300;
-  for (int s = *split; s <= kMost; s += multiple) {
+  for (int64_t next = *split; next <= kMost; next += multiple) {
+    const int s = static_cast<int>(next);
     int64_t with[kMost + 1] = {0};  // items of a size
     int64_t items = 0, empty = 0;
     for (int r = 0; r < batch; ++r) {
@@ -1368,30 +1369,50 @@ int32_t pg_int4_split_pages(int32_t batch, int32_t kv_heads, int32_t group, cons
       with[s] += static_cast<int64_t>(n / s) * kv_heads;
       if (n % s != 0) with[n % s] += kv_heads;
       if (n == 0) ++empty;
-      items += static_cast<int64_t>((n + s - 1) / s) * kv_heads;
+      items += ((static_cast<int64_t>(n) + s - 1) / s) * kv_heads;
     }
     if (items == 0) return PG_OK;
-    // Sizes by rank, largest first; a page's time in round k.
-    std::vector<int32_t> size;
-    size.reserve(static_cast<size_t>(std::min(items, 2 * blocks)));
-    std::vector<int32_t> later;  // the largest of every round after the second
-    int64_t rank = 0;
-    for (int x = s; x > 0; --x) {
-      const int64_t end = rank + with[x];
-      for (; rank < end && rank < 2 * blocks; ++rank) size.push_back(x);
-      for (int64_t k = 2 + static_cast<int64_t>(later.size()); k * blocks < end; ++k)
-        later.push_back(x);
-      rank = end;
-    }
     const double head = group > 4 ? 1.15 : 1.0;
+    // A page's time in round k.
     auto page = [&](int64_t round) {
       const double running = static_cast<double>(items - round * blocks) / blocks;
       return head * (0.12 + 0.06 * std::min(1.0, running));
     };
-    double cost = size[0] * page(0);
-    for (int64_t i = blocks; i < static_cast<int64_t>(size.size()); ++i)
-      cost = std::max(cost, size[2 * blocks - 1 - i] * page(0) + size[i] * page(1));
-    for (size_t k = 0; k < later.size(); ++k) cost += later[k] * page(static_cast<int64_t>(k) + 2);
+    // Items lie by rank, largest first.  In the first two rounds block b has
+    // those of ranks b and 2 blocks - 1 - b: the longest pair counts, and
+    // pairs change only where a size ends on either side.
+    int64_t ends[kMost + 1], rank = 0;  // of the items of a size and larger ones
+    for (int x = s; x > 0; --x) ends[x] = rank += with[x];
+    auto largest = [&](int64_t i) {  // size of rank i < items
+      int x = s;
+      while (ends[x] <= i) --x;
+      return x;
+    };
+    double cost = largest(0) * page(0);
+    const int64_t second = std::min(items, 2 * blocks);
+    if (second > blocks) {
+      int here = largest(blocks), there = largest(blocks - 1);
+      for (int64_t i = blocks; i < second;) {
+        while (ends[here] <= i) --here;
+        while (there < s && ends[there + 1] > 2 * blocks - 1 - i) ++there;
+        cost = std::max(cost, there * page(0) + here * page(1));
+        // The next rank at which either size changes.
+        int64_t change = std::min(second, ends[here]);
+        if (there < s) change = std::min(change, 2 * blocks - ends[there + 1]);
+        i = std::max(change, i + 1);
+      }
+    }
+    // Every later round: its largest item.  All blocks run in all but the last.
+    const int64_t rounds = (items + blocks - 1) / blocks, whole = items / blocks;
+    int64_t k = 2;
+    for (int x = s; x > 0 && k < rounds; --x) {
+      const int64_t end = std::min(rounds, (ends[x] + blocks - 1) / blocks);
+      if (end <= k) continue;
+      const int64_t running = std::max<int64_t>(0, std::min(end, whole) - k);
+      cost += x * page(0) * static_cast<double>(running);
+      if (k + running < end) cost += x * page(k + running);
+      k = end;
+    }
     cost += 2.6 * static_cast<double>((items - 1) / blocks);
     const bool join = empty != 0 || items != static_cast<int64_t>(batch) * kv_heads;
     if (join) cost += 2.5;

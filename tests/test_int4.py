@@ -239,3 +239,44 @@ def test_binding_refuses_forward_mode_duals():
         rows = forward.make_dual(plain.clone().requires_grad_(), torch.ones_like(plain))
         with pytest.raises(ValueError, match="forward-mode"):
             ops.rotary(rows, None, plain, plain, plain, False, False, None, None)
+
+
+def test_automatic_split_at_the_ends_of_its_ranges():
+    """Page counts whose items pass 32 bits, as many heads as are taken, and a
+    multiple that has no second one: an answer within the range, at once."""
+    for pages in ([2 ** 31 - 1], [2 ** 30, 0, 2 ** 30 - 1], [2 ** 27 - 1]):
+        for kv_heads in (8, 65535):
+            for sms in (1, 148, 2 ** 31 - 1):
+                split = split_pages(pages, kv_heads, sms=sms)
+                assert split % 8 == 0 and 8 <= split <= 128
+    assert split_pages([200], 8, multiple=2 ** 31 - 1) == 128
+    assert split_pages([200], 8, multiple=127) == 127
+
+
+@pytest.mark.parametrize("sms,kv_heads,group", [(1, 1, 4), (2, 3, 8), (5, 2, 1)])
+def test_automatic_split_counts_rounds_as_handed_out(sms, kv_heads, group):
+    """The estimate against one that lists the items and their rounds one by one."""
+    rng = np.random.default_rng(sms)
+    for _ in range(40):
+        pages = [int(n) for n in rng.integers(0, rng.integers(2, 700), rng.integers(1, 12))]
+        blocks, costs = 3 * sms, {}
+        for s in range(8, 129, 8):
+            items = sorted((x for n in pages for x in [s] * (n // s) + [n % s] * (n % s > 0)
+                            for _ in range(kv_heads)), reverse=True)
+            if not items:
+                continue
+
+            def page(k):
+                return (1.15 if group > 4 else 1.0) * (
+                    0.12 + 0.06 * min(1.0, (len(items) - k * blocks) / blocks))
+
+            cost = items[0] * page(0)
+            for i in range(blocks, min(len(items), 2 * blocks)):
+                cost = max(cost, items[2 * blocks - 1 - i] * page(0) + items[i] * page(1))
+            for k in range(2, -(-len(items) // blocks)):
+                cost += items[k * blocks] * page(k)
+            cost += 2.6 * ((len(items) - 1) // blocks)
+            cost += 2.5 * (0 in pages or len(items) != len(pages) * kv_heads)
+            costs[s] = cost
+        split = split_pages(pages, kv_heads, group, sms=sms)
+        assert split == 8 if not costs else costs[split] <= min(costs.values()) * (1 + 1e-9)
