@@ -1102,6 +1102,12 @@ int32_t pg_rotary(const pg_rotary_args* a, void* stream) {
              "too many rows or tokens");
   PG_REQUIRE(a->cosine != nullptr && a->sine != nullptr && a->positions != nullptr,
              "rotary tables and device positions are required");
+  const int size = a->dtype == PG_DTYPE_F32 ? 4 : 2, v = 16 / size;
+  PG_REQUIRE(aligned(a->cosine, 4) && aligned(a->sine, 4) && aligned(a->positions, 4),
+             "rotary tables and positions must be 4-byte aligned");
+  for (int i = 0; i < 2; ++i)
+    PG_REQUIRE(p.heads[i] == 0 || (aligned(a->x[i], size) && aligned(a->y[i], size)),
+               "rows must be aligned to their elements");
   p.tokens = a->tokens;
   p.head_dim = a->head_dim;
   p.pairs = a->pairs;
@@ -1113,7 +1119,6 @@ int32_t pg_rotary(const pg_rotary_args* a, void* stream) {
   p.table_rows = a->table_rows;
   p.positions = a->positions;
   p.error_flag = device_error_ptr();
-  const int size = a->dtype == PG_DTYPE_F32 ? 4 : 2, v = 16 / size;
   bool rows16 = true;
   for (int i = 0; i < 2; ++i) {
     rows16 = rows16 &&
@@ -1217,6 +1222,11 @@ int32_t pg_rope_append_int4(const pg_int4_append_args* a, void* stream) {
              "rows, tables, positions, slots and records are required");
   PG_REQUIRE(aligned(a->records, 16) && aligned(a->key_center, 16) && aligned(a->value_center, 16),
              "records and centres must be 16-byte aligned");
+  PG_REQUIRE(aligned(a->query, 2) && aligned(a->key, 2) && aligned(a->value, 2) &&
+                 aligned(a->rotated_query, 2) && aligned(a->rotated_key, 2) &&
+                 aligned(a->cosine, 4) && aligned(a->sine, 4) && aligned(a->positions, 4) &&
+                 aligned(a->slots, 4) && aligned(a->center_rows, 4),
+             "rows must be 2-byte, tables, positions and slots 4-byte aligned");
   const int64_t head_stride[5] = {a->q_stride_h, a->rq_stride_h, a->k_stride_h, a->v_stride_h,
                                   a->rotated_key == nullptr ? 0 : a->rk_stride_h};
   for (int i = 0; i < 5; ++i)
@@ -1316,8 +1326,8 @@ int32_t pg_int4_read(const void* records, int64_t num_pages, int32_t kv_heads,
   if (tokens == 0) return PG_OK;
   PG_REQUIRE(records != nullptr && slots != nullptr && key != nullptr && value != nullptr,
              "records, slots and outputs are required");
-  PG_REQUIRE(aligned(records, 16) && aligned(key, 16) && aligned(value, 16),
-             "records and outputs must be 16-byte aligned");
+  PG_REQUIRE(aligned(records, 16) && aligned(key, 16) && aligned(value, 16) && aligned(slots, 4),
+             "records and outputs must be 16-byte aligned, slots 4-byte");
   pg::Int4ReadParams p{};
   p.records = static_cast<const uint8_t*>(records);
   p.num_pages = num_pages;
@@ -1445,6 +1455,17 @@ int32_t pg_decode_int4_run(const pg_int4_decode_args* a, void* stream) {
              "page table is incomplete");
   PG_REQUIRE(a->num_items == 0 || (a->items != nullptr && a->work_counter != nullptr),
              "work items and their counter are required");
+  for (const void* word : {static_cast<const void*>(a->indices),
+                           static_cast<const void*>(a->last_page_len),
+                           static_cast<const void*>(a->items),
+                           static_cast<const void*>(a->item_slots),
+                           static_cast<const void*>(a->item_off),
+                           static_cast<const void*>(a->part_lse),
+                           static_cast<const void*>(a->work_counter),
+                           static_cast<const void*>(a->lse_out)})
+    PG_REQUIRE(aligned(word, 4), "page tables, plan, workspace and lse must be 4-byte aligned");
+  PG_REQUIRE(aligned(a->out, 2) && aligned(a->value_center, 2),
+             "output and value centre must be 2-byte aligned");
   const bool final_mode = a->final_mode != 0 && a->num_items > 0;
   PG_REQUIRE(final_mode || a->item_off != nullptr, "item offsets are required for the merge");
   PG_REQUIRE(final_mode || a->num_items == 0 ||

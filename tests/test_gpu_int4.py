@@ -720,3 +720,14 @@ def test_plan_rounds_only_its_own_split(cuda_lib):
     a.plan()
     assert a.wrapper.split_pages == 5
     a.check(*a.run())
+
+
+@pytest.mark.parametrize("lengths", [[5], [300]])
+def test_a_workspace_at_an_odd_byte_is_refused(cuda_lib, lengths):
+    a = Attend(lengths, seed=2)
+    for skip in (1, 2):
+        a.wrapper = make_int4_wrapper(workspace=torch.empty(8 << 20, dtype=torch.uint8,
+                                                            device="cuda")[skip:])
+        a.plan()
+        with pytest.raises(RuntimeError, match="aligned"):
+            a.run()

@@ -280,3 +280,34 @@ def test_automatic_split_counts_rounds_as_handed_out(sms, kv_heads, group):
             costs[s] = cost
         split = split_pages(pages, kv_heads, group, sms=sms)
         assert split == 8 if not costs else costs[split] <= min(costs.values()) * (1 + 1e-9)
+
+
+@pytest.mark.parametrize("final_mode", [0, 1])
+def test_c_entries_refuse_misaligned_words(final_mode):
+    """A workspace that starts at an odd byte puts a plan's words there, and a
+    single-item plan needs no partial states whose alignment is looked at."""
+    lib = _lib.load()
+    for name in ("indices", "last_page_len", "items", "item_slots", "item_off", "part_lse",
+                 "work_counter", "lse_out", "out", "value_center"):
+        a = decode_args(final_mode=final_mode, **{name: 0x1001})
+        assert lib.pg_decode_int4_run(ctypes.byref(a), None) == 1, name
+        assert b"aligned" in lib.pg_last_error()
+    for name in ("query", "key", "value", "rotated_query", "rotated_key", "cosine", "sine",
+                 "positions", "slots"):
+        a = append_args(**{name: 0x1001})
+        assert lib.pg_rope_append_int4(ctypes.byref(a), None) == 1, name
+        assert b"aligned" in lib.pg_last_error()
+    assert lib.pg_int4_read(0x1000, 4, 1, 0x1002, 1, 0x1000, 0x1000, 0, None) == 1
+    for dtype, at in ((0, 1), (1, 1), (2, 2)):
+        for name in ("x", "y", "cosine", "sine", "positions"):
+            a = _lib.PgRotaryArgs()
+            a.x[0], a.y[0] = 0x1000, 0x2000
+            a.heads[0], a.tokens, a.head_dim, a.pairs = 4, 1, 128, 64
+            a.table_rows, a.table_stride, a.dtype = 8, 64, dtype
+            a.cosine = a.sine = a.positions = 0x3000
+            if name in "xy":
+                getattr(a, name)[0] += at
+            else:
+                setattr(a, name, 0x3000 + at)
+            assert lib.pg_rotary(ctypes.byref(a), None) == 1, (dtype, name)
+            assert b"aligned" in lib.pg_last_error()
