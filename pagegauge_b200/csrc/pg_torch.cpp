@@ -65,7 +65,8 @@ const Tensor* arg(PyObject* o, const char* name, bool optional = false) {
 void check_no_tangent(std::initializer_list<const Tensor*> tensors) {
   if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
   for (const Tensor* t : tensors)
-    if (t != nullptr && t->_fw_grad(0).defined())
+    if (t != nullptr && t->unsafeGetTensorImpl()->autograd_meta() != nullptr &&
+        t->_fw_grad(0).defined())
       refuse("this operator has no forward-mode derivative: unpack its inputs' duals");
 }
 
