@@ -91,6 +91,15 @@ def rotary_tables(positions: int, rotary_dim: int = 128, theta: float = 1.0e6,
     return (angle.cos() * scale).float(), (angle.sin() * scale).float()
 
 
+def _refuse_capture(rows: torch.Tensor) -> None:
+    """A captured backward pass ends the process where an eager graph of the same
+    leaves lives: what accumulates their gradients belongs to the eager stream."""
+    with torch.cuda.device(rows.device):
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError("a rotation with a gradient cannot be captured; capture the "
+                             "rotation and its adjoint under no_grad")
+
+
 class _Rotate(torch.autograd.Function):
     """The rotation, whose gradient is its transpose.  Rows that the kernel
     leaves (a position outside the tables) are zero, and so are their
@@ -129,9 +138,8 @@ def _rotate_with_gradient(query, key, cosine, sine, positions, interleaved, adjo
         raise ValueError("rows that require gradients are rotated into new tensors")
     if cosine.requires_grad or sine.requires_grad:
         raise ValueError("the rotary tables have no gradient")
-    if torch.cuda.is_current_stream_capturing():
-        raise ValueError("a rotation with a gradient cannot be captured; capture the rotation "
-                         "and its adjoint under no_grad")
+    if query.is_cuda:  # others are refused with the arguments
+        _refuse_capture(query)
     return _Rotate.apply(query, key, cosine, sine, positions, bool(interleaved), bool(adjoint))
 
 

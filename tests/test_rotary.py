@@ -105,3 +105,15 @@ def test_oracle_adjoint_is_the_transpose():
         lhs = (I.rotate(x, cos, sin, interleaved) * y).sum()
         rhs = (x * I.rotate(y, cos, sin, interleaved, adjoint=True)).sum()
         assert abs(lhs - rhs) < 1e-12
+
+
+def test_cpu_rows_that_require_gradients_are_refused_alike():
+    q = torch.zeros(2, 4, 128, requires_grad=True)
+    k = torch.zeros(2, 2, 128, requires_grad=True)
+    cos, sin = rotary_tables(8, 128)
+    positions = torch.zeros(2, dtype=torch.int32)
+    for key in (None, k, k.detach()):
+        with pytest.raises(ValueError, match="CUDA"):
+            apply_rotary(q, key, cos, sin, positions)
+    with pytest.raises(ValueError, match="CUDA"):
+        apply_rotary(q.detach(), k, cos, sin, positions)
