@@ -93,7 +93,8 @@ def rotary_tables(positions: int, rotary_dim: int = 128, theta: float = 1.0e6,
 
 def _refuse_capture(rows: torch.Tensor) -> None:
     """A captured backward pass ends the process where an eager graph of the same
-    leaves lives: what accumulates their gradients belongs to the eager stream."""
+    leaves lives: what accumulates their gradients belongs to the eager stream.
+    So neither direction of a rotation with a gradient is captured."""
     with torch.cuda.device(rows.device):
         if torch.cuda.is_current_stream_capturing():
             raise ValueError("a rotation with a gradient cannot be captured; capture the "
@@ -122,6 +123,8 @@ class _Rotate(torch.autograd.Function):
     def backward(ctx, *grads):
         needed = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[i]]
         # A sum's gradient is one value expanded over the rows.
+        if needed:
+            _refuse_capture(grads[needed[0]])
         rows = [grads[i] if grads[i].stride(-1) == 1 else grads[i].contiguous() for i in needed]
         result = [None] * 7
         if rows:
@@ -154,8 +157,9 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, cosine: torch.Te
     first ``2 * pairs`` dims turn, the others are copied.  Half layout pairs
     dim j with j + pairs, ``interleaved`` 2j with 2j + 1.  ``adjoint`` turns
     back (the gradient of the rotation with respect to its rows, which autograd
-    takes for rows that require one; the call then makes its outputs and is
-    not captured into a graph; forward-mode duals are refused).  Rows are
+    takes for rows that require one; the call then makes its outputs, and neither
+    it nor its backward pass is captured into a graph; forward-mode duals are
+    refused).  Rows are
     float16, bfloat16 or float32 with a contiguous last dimension and any
     other strides.  The outputs may be the inputs (in place); they must not
     overlap them in any other way.  Rows of a token whose position is outside

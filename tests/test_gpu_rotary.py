@@ -332,3 +332,49 @@ def test_refusals(cuda_lib):
         with pytest.raises(ValueError):
             apply_rotary(*args, **kw)
     assert math.isfinite(float(q.float().sum()))
+
+
+def test_a_backward_pass_is_not_captured(cuda_lib):
+    """Forward and backward on one stream, the backward pass within a capture: refused
+    before it reaches the leaves; the same pass then runs outside the capture."""
+    cos, sin = rotary_tables(64, 128, device="cuda")
+    pos = torch.arange(5, dtype=torch.int32, device="cuda")
+    leaf = rows(5, 2, 128, torch.float32, 21).cuda().requires_grad_()
+    weight = rows(5, 2, 128, torch.float32, 22).cuda()
+    other = torch.zeros(4, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y, _ = apply_rotary(leaf, None, cos, sin, pos)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        other.add_(1)
+        with pytest.raises(ValueError, match="captured"):
+            torch.autograd.grad(y, leaf, weight, retain_graph=True)
+    with torch.cuda.stream(side):
+        (grad,) = torch.autograd.grad(y, leaf, weight)
+    torch.cuda.synchronize()
+    exp, _ = apply_rotary(weight, None, cos, sin, pos, adjoint=True)
+    assert torch.equal(grad, exp)
+    graph.replay()
+    assert (other == 1).all() and read_device_error() == 0
+
+
+def test_forward_over_reverse_is_refused(cuda_lib):
+    """A tangent on the gradient of a differentiable backward pass is not dropped."""
+    import torch.autograd.forward_ad as forward
+
+    cos, sin = rotary_tables(64, 128, device="cuda")
+    pos = torch.arange(5, dtype=torch.int32, device="cuda")
+    leaf = rows(5, 2, 128, torch.float32, 23).cuda().requires_grad_()
+    weight = rows(5, 2, 128, torch.float32, 24).cuda()
+    y, _ = apply_rotary(leaf, None, cos, sin, pos)
+    with forward.dual_level():
+        dual = forward.make_dual(weight, torch.ones_like(weight))
+        for graph in (False, True):
+            with pytest.raises((ValueError, RuntimeError, NotImplementedError)):
+                torch.autograd.grad(y, leaf, dual, create_graph=graph, retain_graph=True)
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode(), pytest.raises(ValueError, match="forward-mode"):
+                apply_rotary(dual, None, cos, sin, pos)
