@@ -257,6 +257,13 @@ __device__ __forceinline__ void pages_int4(const uint8_t* rec, const Int4Query& 
       s[i][3] = fmaf(wb, acc[3], s[i][3]);
     }
   }
+  // In log2 units, rounded here: the maximum below and the differences from it
+  // are of the same numbers, so that however large they are (FP32 steps of many
+  // units) the largest gives a weight of 1.
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[i][j] = __fmul_rn(s[i][j], iq.cr[j & 1]);
   if constexpr (MASKED) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -264,8 +271,8 @@ __device__ __forceinline__ void pages_int4(const uint8_t* rec, const Int4Query& 
       if (g + 8 >= valid[i]) s[i][2] = s[i][3] = kNegInf;
     }
   }
-  const float lm0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2])) * iq.cr[0];
-  const float lm1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3])) * iq.cr[1];
+  const float lm0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2]));
+  const float lm1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]));
   if (__any_sync(0xffffffffu, lm0 > st.m[0] + kInt4Slack || lm1 > st.m[1] + kInt4Slack)) {
     const float lm[2] = {warp_max_xor_g(lm0), warp_max_xor_g(lm1)};
     float a[2];
@@ -291,10 +298,10 @@ __device__ __forceinline__ void pages_int4(const uint8_t* rec, const Int4Query& 
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const uint8_t* page = rec + i * kInt4Record;
-    const float p0 = fast_exp2(fmaf(s[i][0], iq.cr[0], -st.ref[0]));
-    const float p1 = fast_exp2(fmaf(s[i][1], iq.cr[1], -st.ref[1]));
-    const float p2 = fast_exp2(fmaf(s[i][2], iq.cr[0], -st.ref[0]));
-    const float p3 = fast_exp2(fmaf(s[i][3], iq.cr[1], -st.ref[1]));
+    const float p0 = fast_exp2(s[i][0] - st.ref[0]);
+    const float p1 = fast_exp2(s[i][1] - st.ref[1]);
+    const float p2 = fast_exp2(s[i][2] - st.ref[0]);
+    const float p3 = fast_exp2(s[i][3] - st.ref[1]);
     st.l[0] += p0 + p2;
     st.l[1] += p1 + p3;
     // Value scales and midpoints of tokens g and g + 8: four groups', or
