@@ -22,9 +22,14 @@
 //   O_d = sum_t (P_t s_tg) z_td - 8 sum_t (P_t s_tg) + sum_t P_t m_tg
 // where P s is formed in FP32 and rounded once to FP16, and the sum times 8
 // comes from tensor-core products of the same rounded operands, so that a
-// rounding of P s weighs (z - 8) s and not z s; the last sum is FP32.  P <= 4
-// (the running maximum is raised when a score passes it by 2 in log2), so P s
-// <= 4 * 8734.
+// rounding of P s weighs (z - 8) s and not z s; the last sum is FP32.  P =
+// 2^(score - ref), all sums relative to a row's reference: not its largest score,
+// which left small scales beside a dominant token of the warp in subnormal halves
+// (700 tokens, one of zero values 10 nats above the rest: 3.7 % off, now 0.2 %, which
+// is the FP16 output's step; values of deviation 0.001: 4.7e-4, now 2.3e-4), but that
+// and the largest value scale, so that P s fills the half's range.  What is left is
+// half a subnormal step, 2^-37 of (largest weight) x (largest scale), per token.  It
+// costs 1-2 %.
 //
 // Bound by the compute of a page, not by its bytes: eight ragged requests of
 // 300,000 tokens in all (384 MB) take 74.5 us, the copies alone 60.1 us.  A
@@ -76,8 +81,23 @@ static_assert(kInt4CombineAt % 16 == 0, "the combine buffer is read in 16-byte r
 // Pages per warp asked of the L2 ahead of the dependency wait: 49,152 tokens
 // 18.2 -> 17.6 us (16 pages would cost 0.5 us).
 constexpr int kInt4Prefetch = 4;
-// The running maximum is raised when a score passes it by this (log2).
-constexpr float kInt4Slack = 2.f;
+// A row's reference before its first token: finite, so that masked scores of -inf
+// give weights of 0.
+constexpr float kInt4NoRef = -3e38f;
+// Where a reference is raised the largest P s is 2^12 to 2^13, 2^26 above the least
+// normal half, and later ones may pass it by the slack: P s < 2^15.
+constexpr float kInt4Headroom = 12.f, kInt4Slack = 2.f;
+// Scores past this are taken without their scale (P <= 1): their own steps are what
+// counts.
+constexpr float kInt4FarScore = 0x1p22f;
+
+// Largest of a token's four value scales, as the half's bits.
+__device__ __forceinline__ uint32_t int4_largest_scale(const uint8_t* scales) {
+  const uint2 x = *reinterpret_cast<const uint2*>(scales);
+  const __half2 pair = __hmax2(*reinterpret_cast<const __half2*>(&x.x),
+                               *reinterpret_cast<const __half2*>(&x.y));
+  return __half_as_ushort(__hmax(__low2half(pair), __high2half(pair)));
+}
 
 // D = A(16x16 f16) * B(16x8 f16) + C.
 __device__ __forceinline__ void mma_16816_c(float* d, uint32_t a0, uint32_t a1, uint32_t a2,
@@ -145,8 +165,7 @@ struct Int4Query {
 };
 
 struct Int4State {
-  float m[2], l[2];  // running max and sum of rows 2t, 2t+1 (this lane's tokens)
-  float ref[2];      // m, or 0 while m is -inf
+  float ref[2], l[2];  // reference and sum of rows 2t, 2t+1's weights (this lane's tokens)
   // Tile 2j + e, rows g: dims d = 32j + 4g + 2e; rows g + 8: d and d + 1 as
   // z_d + 16 z_(d+1) (one AND less than the two nibbles apart).
   float o[8][4];
@@ -271,17 +290,31 @@ __device__ __forceinline__ void pages_int4(const uint8_t* rec, const Int4Query& 
       if (g + 8 >= valid[i]) s[i][2] = s[i][3] = kNegInf;
     }
   }
+  // Lane 16 i + tok looks at the value scales of page i's token tok.  The exponent of
+  // the pages' largest (of 2^-24 where all are zero; finite), less the headroom: a
+  // whole number, so that the weight of a largest score is a power of two and adds
+  // no rounding to its scale.
+  uint32_t scale = int4_largest_scale(rec + (lane >> 4) * kInt4Record + kInt4ValueMeta +
+                                      16 * (lane & 15));
+  if constexpr (MASKED)
+    if ((lane & 15) >= (lane < 16 ? valid[0] : valid[1])) scale = 0u;
+  scale = min(max(__reduce_max_sync(0xffffffffu, scale), 1u), 0x7bffu);
+  scale = __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(scale))));
+  const float ls =
+      __uint_as_float(0x4b000000u | (scale >> 23)) - (8388608.f + 127.f + kInt4Headroom);
   const float lm0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2]));
   const float lm1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]));
-  if (__any_sync(0xffffffffu, lm0 > st.m[0] + kInt4Slack || lm1 > st.m[1] + kInt4Slack)) {
-    const float lm[2] = {warp_max_xor_g(lm0), warp_max_xor_g(lm1)};
+  if (__any_sync(0xffffffffu, lm0 + (ls - kInt4Slack) > st.ref[0] ||
+                                  lm1 + (ls - kInt4Slack) > st.ref[1] ||
+                                  !(fmaxf(fabsf(lm0), fabsf(lm1)) <= kInt4FarScore))) {
+    const float top[2] = {warp_max_xor_g(lm0), warp_max_xor_g(lm1)};
     float a[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float mn = fmaxf(st.m[i], lm[i]);
-      a[i] = mn == kNegInf ? 1.f : fast_exp2(st.m[i] - mn);  // -inf -> 0
-      st.m[i] = mn;
-      st.ref[i] = mn == kNegInf ? 0.f : mn;
+      const float ref =
+          fmaxf(st.ref[i], fabsf(top[i]) <= kInt4FarScore ? top[i] + ls : top[i]);
+      a[i] = st.ref[i] == kInt4NoRef ? 1.f : fast_exp2(st.ref[i] - ref);
+      st.ref[i] = ref;
       st.l[i] *= a[i];
     }
 #pragma unroll
@@ -369,6 +402,14 @@ __device__ __forceinline__ void pages_int4(const uint8_t* rec, const Int4Query& 
       }
     }
   }
+}
+
+// m + log2(sum) of a positive sum.  Its power of two goes to m, which is coarser
+// for it, so that the logarithm is of a number in [1, 2).
+__device__ __forceinline__ float int4_lse(float m, float sum) {
+  const int e = min(static_cast<int>(__float_as_uint(sum) >> 23) - 127, 126);
+  const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  return (m + static_cast<float>(e)) + fast_log2(sum * down);
 }
 
 // Output row element (v, base-2 lse): the value centre is added where the
@@ -500,9 +541,8 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
         next_id = load_volatile(p.indices + next.idx_begin + warp + kInt4Warps * lane);
     }
     Int4State st;
-    st.m[0] = st.m[1] = kNegInf;
     st.l[0] = st.l[1] = 0.f;
-    st.ref[0] = st.ref[1] = 0.f;
+    st.ref[0] = st.ref[1] = kInt4NoRef;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -566,8 +606,8 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
     float* cl = cm + kInt4Warps * 8;                                   // [W][8]
     float* co = cl + kInt4Warps * 8;                                   // [W][8][kCoStride]
     if (g == 0) {
-      cm[warp * 8 + 2 * t] = ok ? st.m[0] : kNegInf;
-      cm[warp * 8 + 2 * t + 1] = ok ? st.m[1] : kNegInf;
+      cm[warp * 8 + 2 * t] = ok ? st.ref[0] : kInt4NoRef;
+      cm[warp * 8 + 2 * t + 1] = ok ? st.ref[1] : kInt4NoRef;
       cl[warp * 8 + 2 * t] = ok ? l0 : 0.f;
       cl[warp * 8 + 2 * t + 1] = ok ? l1 : 0.f;
     }
@@ -609,7 +649,7 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
         O.w += o.w * e;
       }
       const float inv = L == 0.f ? 0.f : 1.f / L;
-      const float lse = L == 0.f ? kNegInf : M + fast_log2(L);
+      const float lse = L == 0.f ? kNegInf : int4_lse(M, L);
       O = make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv);
       if (p.final_mode) {
         int4_store_out<T>(p, r, h, q, d + 0, O.x, lse);

@@ -44,3 +44,9 @@ class Held:
         records = self.pool.records[self.order.cuda(), h].cpu().numpy()
         (ka, km), (va, vm) = I.load(records)
         return [x.reshape(-1, 128)[:self.n] for x in (ka, km, va, vm)]
+
+    def value_scales(self, h):
+        """Value scale of every dim of KV head h, [n, 128]."""
+        meta = self.pool.records[self.order.cuda(), h, 2304:].contiguous().view(torch.float16)
+        s = meta.double().cpu().numpy().reshape(-1, 16, 2, 4)[:, :, 0].reshape(-1, 4)
+        return s.repeat(32, axis=-1)[:self.n]
