@@ -311,3 +311,25 @@ def test_c_entries_refuse_misaligned_words(final_mode):
                 setattr(a, name, 0x3000 + at)
             assert lib.pg_rotary(ctypes.byref(a), None) == 1, (dtype, name)
             assert b"aligned" in lib.pg_last_error()
+
+
+@pytest.mark.parametrize("pages,kv_heads,group", [([256], 8, 4), ([3923] * 4, 4, 7), ([0, 5, 300], 2, 8),
+                                                  ([1], 1, 1)])
+def test_the_wrapper_plans_with_the_split_it_chose(pages, kv_heads, group):
+    """What plan() does on the host: the split goes to the planner as it is, and the
+    items cover every page of every head once, in items of at most it."""
+    from pagegauge_b200.wrapper import Int4DecodeWrapper, plan_items
+
+    indptr = np.concatenate([[0], np.cumsum(pages)]).astype(np.int32)
+    wrapper = object.__new__(Int4DecodeWrapper)
+    split = wrapper._automatic_split(indptr, kv_heads, group, 148)
+    assert split == split_pages(pages, kv_heads, group) and split % wrapper._split_multiple == 0
+    items, off, info = plan_items(len(pages), kv_heads, indptr, None, split, split, 148)
+    assert info.split_pages[0] == split and off[-1] == len(items)
+    seen = np.zeros((kv_heads, indptr[-1]), int)
+    for request, head, begin, count in items:
+        n = count & 0x7FFFFFFF
+        assert 1 <= n <= split and indptr[request] <= begin and begin + n <= indptr[request + 1]
+        assert (count < 0) == (begin + n == indptr[request + 1])
+        seen[head, begin:begin + n] += 1
+    assert (seen == 1).all()
