@@ -513,7 +513,9 @@ typedef struct pg_int4_decode_args {
   int32_t final_mode; /* 1: one item per (request, head): no merge launch */
   int32_t dtype;      /* PG_DTYPE_F16 or PG_DTYPE_BF16 */
   float sm_scale;
-  int32_t reserved;
+  int32_t most_items; /* items of the (request, KV head) that has most
+                         (pg_plan_info.max_items_per_head): chooses how they
+                         are joined; 0: taken as the mean */
 } pg_int4_decode_args;
 
 int32_t pg_decode_int4_run(const pg_int4_decode_args* args, void* stream);

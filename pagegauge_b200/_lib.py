@@ -105,7 +105,7 @@ class PgInt4DecodeArgs(ctypes.Structure):
         ("part_lse", c_vp), ("work_counter", c_vp),
         ("num_items", c_i32), ("batch", c_i32), ("kv_heads", c_i32), ("group", c_i32),
         ("final_mode", c_i32), ("dtype", c_i32), ("sm_scale", ctypes.c_float),
-        ("reserved", c_i32),
+        ("most_items", c_i32),
     ]
 
 

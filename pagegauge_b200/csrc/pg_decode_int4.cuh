@@ -674,8 +674,8 @@ __global__ void __launch_bounds__(kInt4Warps * 32, kInt4CtasPerSm)
 
 // Joins the work items of each (request, query head): R warps per row fold
 // partials w, w + R, ... with four dims per lane and up to eight loads in
-// flight, then a row's warps are combined.  R = 8 (a block per row) where a
-// row has many partials, 1 (eight rows per block) where it has few.
+// flight, then a row's warps are combined.  R = 8 (a block per row) where some
+// row has many partials for the number of rows, else 1 (eight rows per block).
 template <typename T, int R>
 __global__ void __launch_bounds__(256)
     pg_int4_merge_kernel(const __grid_constant__ Int4DecodeParams p) {

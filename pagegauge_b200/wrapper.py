@@ -116,6 +116,7 @@ class PagedDecodePlan:
         item's place in the planner's order beside it (``slots_ptr``)."""
         self.num_items = int(info.num_items)
         self.single = bool(info.single_item_per_head)
+        self.most_items = int(info.max_items_per_head)
         self.split_pages = (int(info.split_pages[0]), int(info.split_pages[1]))
         self.warps = int(info.warps_per_cta)
         self.batch, self.kv_heads, self.group = batch, kv_heads, group
@@ -427,7 +428,7 @@ class Int4DecodeWrapper(BatchDecodeWithPagedKVCacheWrapper):
             0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, self._indices.data_ptr(), self._last_len.data_ptr(),
             plan.items_ptr, plan.slots_ptr, plan.off_ptr, plan.o_ptr, plan.lse_ptr, plan.sem_ptr,
             plan.num_items, plan.batch, plan.kv_heads, plan.group,
-            plan.single and plan.num_items > 0, 0, 0.0, 0)
+            plan.single and plan.num_items > 0, 0, 0.0, plan.most_items)
         self._device_index = device.index
 
     begin_forward = plan

@@ -18,6 +18,7 @@ import pytest
 import torch
 
 from oracle import int4_oracle as I
+from pagegauge_b200 import _lib
 from pagegauge_b200.int4 import Int4PagePool
 from pagegauge_b200.rotary import RotaryScaling, rotary_tables
 from pagegauge_b200.runtime import load_append_extension, read_device_error
@@ -731,3 +732,24 @@ def test_a_workspace_at_an_odd_byte_is_refused(cuda_lib, lengths):
         a.plan()
         with pytest.raises(RuntimeError, match="aligned"):
             a.run()
+
+
+@pytest.mark.parametrize("lengths,hkv,group", [
+    ([16 * 700] + [3] * 20, 1, 4),  # 88 partials on one head, one on the others
+    ([1, 0, 16 * 500 + 5, 17], 3, 8), ([2000] + [9, 0] * 60, 2, 2),
+    ([5] * 70 + [16 * 300], 4, 8)])  # joined by a warp per row: many rows
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_of_skewed_batches(cuda_lib, lengths, hkv, group, dtype):
+    """One long request among short ones, joined as the plan's largest head and as the
+    mean over the heads would have it: the same within the bound, and the choice is
+    the plan's."""
+    a = Attend(lengths, hkv=hkv, group=group, dtype=dtype, split=8, seed=7)
+    p = a.wrapper._plan
+    assert p.most_items == max(np.diff(p.host_off)) == -(-(-(-max(lengths) // 16)) // 8)
+    a.check(*a.run())
+    field = _lib.PgInt4DecodeArgs.most_items.offset
+    block = a.wrapper._block
+    for most in (0, 1, 1 << 30):  # the mean, a warp per row, a block per row
+        a.wrapper._block = block[:field] + most.to_bytes(4, "little") + block[field + 4:]
+        a.check(*a.run())
+    assert read_device_error() == 0
