@@ -484,9 +484,14 @@ int32_t pg_int4_read(const void* records, int64_t num_pages, int32_t kv_heads,
  * log-sum-exp of the scores.  The page table and its plan are those of
  * pg_decode_plan with one segment (indptr0); last_page_len counts the valid
  * tokens of a request's last page (0..16; values outside are clamped).
- * Requests without tokens give zeros (no centre) and -inf.  Pages may have been written by the kernel just before
- * in the stream: they are read after it completes.  A page id outside the
- * pool is left out and reported (PG_DEV_BAD_PAGE_ID).                      */
+ * Requests without tokens give zeros (no centre) and -inf.  Pages may have
+ * been written by the kernel just before in the stream: they are read after
+ * it completes.  A page id outside the pool is left out and reported
+ * (PG_DEV_BAD_PAGE_ID).  The scores are those of the keys held: with key
+ * centres c_K the log-sum-exp lacks q c_K, which cancels within one softmax,
+ * so a state joins another segment's only where both keys are centred alike.
+ * Rows of any size keep their softmax while their scores are finite in FP32,
+ * queries being below 2^115 (PG_DTYPE_BF16).                               */
 typedef struct pg_int4_decode_args {
   const void* q; /* [B, Hq, 128] of dtype, last dim contiguous */
   int64_t q_stride_b, q_stride_h;

@@ -32,11 +32,13 @@
 // costs 1-2 %.
 //
 // Bound by the compute of a page, not by its bytes: eight ragged requests of
-// 300,000 tokens in all (384 MB) take 74.5 us, the copies alone 60.1 us.  A
+// 300,000 tokens in all (384 MB) take 76.3 us in a captured loop (82-87 us per
+// call, sustained, at the power cap's clocks), the copies alone 60.1 us.  A
 // tensor instruction costs about 6 issue cycles here whatever else runs (its
 // pipe is 30 % busy), an AND 2, so the layouts above save instructions first.
-// 49,152 tokens of one request take 17.2 us: 9.7 us of bytes, the rest two
-// dependent launches.
+// 49,152 tokens of one request take 17.7 us (9.7 us of bytes): 24,576 pages and
+// heads at the same rate are 12.5 us, the rest is the first pages' latency and the
+// join's launch.
 #pragma once
 
 #include "pg_decode_core.cuh"

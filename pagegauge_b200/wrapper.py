@@ -390,9 +390,11 @@ class Int4DecodeWrapper(BatchDecodeWithPagedKVCacheWrapper):
     value_center=, out=, lse=, return_lse=)`` with ``q`` and ``out`` float16
     or bfloat16 [B,Hq,128]; ``q`` is 4-byte aligned with even strides.  Of a
     request's last page ``last_page_len`` (0..16) tokens count; requests
-    without tokens give zeros and -inf.  One wrapper's workspace serves one run
-    at a time: concurrent streams (or graphs replayed concurrently) need a
-    wrapper each."""
+    without tokens give zeros and -inf.  ``lse`` is of the scores of the keys
+    held, so a state joins another segment's where both keys are centred alike.
+    A wrapper's workspace holds its plan and serves one run at a time: every
+    wrapper needs one of its own, and concurrent streams (or graphs replayed
+    concurrently) need a wrapper each."""
 
     # The kernel's four warps take pages in pairs: an automatic split is of
     # whole pairs (4,096 tokens: 5 pages 7.9 us, 8 pages 7.1 us; 16,384: 19
