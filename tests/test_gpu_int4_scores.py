@@ -50,3 +50,27 @@ def test_scores_far_from_zero(cuda_lib, group, big, key, sign, dtype):
     assert (np.abs(got - exp) <= bound).all()
     el = rest[:, 0] / math.log(2)
     assert (np.abs(lse - el) <= 2.0 ** -16 * np.abs(score).max(-1) / math.log(2)).all()
+
+
+@pytest.mark.parametrize("exponent", [40, 80, 110, 114])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_queries_of_bfloat16_size(cuda_lib, exponent, sign):
+    """Queries past FP16's range up to the documented 2^115: the same one-token
+    softmax, and a base-2 LSE of the top score."""
+    g = torch.Generator().manual_seed(exponent)
+    signs = torch.randint(0, 2, (128,), generator=g) * 2.0 - 1.0
+    c = torch.tensor([0.5, 1.0, 0.75]) if sign > 0 else torch.tensor([-0.5, -0.1, -0.75])
+    q = (signs * 2.0 ** exponent).expand(1, 4, 128).to(torch.bfloat16)
+    k = (c[:, None] * signs)[:, None].to(torch.bfloat16)
+    v = torch.randn(3, 1, 128, generator=g).to(torch.bfloat16)
+    a = Held(q.contiguous(), k, v, 1, 1)
+    got, lse = a.run()
+    ka, km, va, vm = a.held(0)
+    score = (a.q[0].double().cpu().numpy() @ (ka + km).T) * 128 ** -0.5
+    assert (score.argmax(-1) == 1).all()
+    exp = va[1] + vm[1]
+    bound = 2.0 ** -11 * np.abs(va[1]) + 2.0 ** -18 * (np.abs(va[1]) + np.abs(vm[1]))
+    bound = bound + 2.0 ** -8 * (np.abs(exp) + bound)
+    assert (np.abs(got - exp) <= bound).all()
+    el = score.max(-1) / math.log(2)
+    assert (np.abs(lse - el) <= 2.0 ** -16 * np.abs(score).max(-1) / math.log(2)).all()
